@@ -41,6 +41,7 @@ extern "C" {
 
 #define B200Q_DTYPE_FP16 0
 #define B200Q_DTYPE_BF16 1
+#define B200Q_DTYPE_FP32 2 /* router logits of b200q_moe_balance only */
 
 /* Library version, (major << 16) | minor. */
 int b200q_version(void);
@@ -82,6 +83,17 @@ int b200q_w4a16_gemm(const void* x, const int32_t* qweight, const void* scales, 
                      void* y, int64_t M, int64_t N, int64_t K, int64_t group, int dtype,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* Input gradient of b200q_w4a16_gemm with frozen weights:
+ * dx [M, K] = dy [M, N] . dequant(qweight, scales, zeros)^T, the weight rounded
+ * to the activation type as in the forward, fp32 accumulation, one rounding of
+ * dx.  Same layouts and requirements as b200q_w4a16_gemm; workspace >= 256
+ * bytes (status word).  The reference's module has no backward of its own
+ * (QUANT_REF.forward, generate_tasks.py:54-61, under autograd would multiply by
+ * the transposed weight it dequantises). */
+int b200q_w4a16_dgrad(const void* dy, const int32_t* qweight, const void* scales, const void* zeros, void* dx,
+                      int64_t M, int64_t N, int64_t K, int64_t group, int dtype, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 /* Bytes of zero-initialised workspace b200q_w8a8_gemm needs for this shape. */
 size_t b200q_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K, int device);
 
@@ -104,6 +116,30 @@ int b200q_w8a8_gemm(const void* x_int8, const void* w_int8, const void* x_scale,
  * [T, 2]).  topi [T, 2] int32, gates [T, 2], offsets [E + 1].  2 <= E <= 256. */
 int b200q_moe_route(const void* logits, int64_t T, int64_t E, int dtype, int32_t* topi, void* gates,
                     int32_t* offsets, int32_t* slot_token, int32_t* token_slot, void* stream);
+
+/* Load-balance loss of a top-k router, per-expert counts and the logits'
+ * gradient.  logits [T, E] (fp16, bf16 or fp32), topi [T, k] int32 (for k = 2
+ * b200q_moe_route's), mask [T] bytes or NULL (0: the token counts nowhere and
+ * gets gradient 0; so does a row whose logits are all -inf).  With n live
+ * tokens, p = softmax(logits) in fp32, f_e = counts_e / (k n),
+ * P_e = sum_t p_te / n:
+ *   loss = E sum_e f_e P_e,
+ *   dlogits_tj = dloss (E / n) p_tj (f_j - sum_e f_e p_te),
+ * f carrying no gradient; n = 0 gives 0.  A topi of -1 is a dropped choice and
+ * counts nowhere; any other value outside [0, E) counts nowhere and sets
+ * B200Q_DEV_ERR_BOUNDS in the status word (when workspace is non-NULL).
+ * loss [1] fp32, counts [E], coef [E] fp32 = E f / n, which the gradient call
+ * takes.  scratch: any contents, overwritten, b200q_moe_balance_scratch_bytes
+ * of it; it may be freed or reused once the call has run on the stream.
+ * Results do not depend on timing.  2 <= E <= 256, 1 <= k <= min(8, E),
+ * T <= 2^27.  The reference has no such loss; its router is
+ * FUSED_QMOE_REF.forward's (generate_tasks.py:368-371). */
+size_t b200q_moe_balance_scratch_bytes(int64_t T, int64_t E);
+int b200q_moe_balance(const void* logits, const int32_t* topi, const uint8_t* mask, int64_t T, int64_t E, int64_t k,
+                      int dtype, float* loss, int32_t* counts, float* coef, void* scratch, size_t scratch_bytes,
+                      void* workspace, void* stream);
+int b200q_moe_balance_grad(const void* logits, const uint8_t* mask, const float* coef, const float* dloss, int64_t T,
+                           int64_t E, int dtype, void* dlogits, void* stream);
 
 /* xg[s, :] = x[slot_token[s], :] for s < nslots (rows of D fp16/bf16, D % 8 == 0). */
 int b200q_moe_gather(const void* x, const int32_t* slot_token, int64_t nslots, int64_t D, void* xg, void* stream);

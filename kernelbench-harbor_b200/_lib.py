@@ -20,6 +20,7 @@ ERR_DEVICE = -6
 
 DTYPE_FP16 = 0
 DTYPE_BF16 = 1
+DTYPE_FP32 = 2
 
 _c_i64 = ctypes.c_int64
 _c_vp = ctypes.c_void_p
@@ -34,6 +35,8 @@ SIGNATURES = {
     "b200q_w4a16_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int]),
     "b200q_w4a16_gemm": (ctypes.c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64,
                                         ctypes.c_int, _c_vp, _c_sz, _c_vp]),
+    "b200q_w4a16_dgrad": (ctypes.c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64,
+                                         ctypes.c_int, _c_vp, _c_sz, _c_vp]),
     "b200q_w8a8_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, ctypes.c_int]),
     "b200q_w8a8_gemm": (ctypes.c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_sz,
                                        _c_vp]),
@@ -42,6 +45,11 @@ SIGNATURES = {
                                         _c_vp]),
     "b200q_moe_route": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, ctypes.c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,
                                        _c_vp]),
+    "b200q_moe_balance_scratch_bytes": (_c_sz, [_c_i64, _c_i64]),
+    "b200q_moe_balance": (ctypes.c_int, [_c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_vp, _c_vp,
+                                         _c_vp, _c_vp, _c_sz, _c_vp, _c_vp]),
+    "b200q_moe_balance_grad": (ctypes.c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, ctypes.c_int, _c_vp,
+                                              _c_vp]),
     "b200q_moe_gather": (ctypes.c_int, [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp]),
     "b200q_ep_pack": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, ctypes.c_int, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64,
                                      _c_i64, _c_vp, _c_vp, _c_vp]),

@@ -16,6 +16,10 @@ int w4a16_tc_grouped(const void* x, const int32_t* qw, const void* sc, const voi
                      int64_t N, int64_t K, int64_t group, int dtype, void* workspace, size_t workspace_bytes,
                      cudaStream_t stream);
 
+int w4a16_tc_dgrad(const void* dy, const int32_t* qweight, const void* scales, const void* zeros, void* dx, int64_t M,
+                   int64_t N, int64_t K, int64_t group, int dtype, void* workspace, size_t workspace_bytes,
+                   cudaStream_t stream);
+
 size_t w8a8_ws_bytes(int64_t M, int64_t N, int64_t K, int device);
 int w8a8_tc(const void* x_int8, const void* w_int8, const void* x_scale, const void* w_scale, void* y, int64_t M,
             int64_t N, int64_t K, void* workspace, size_t workspace_bytes, cudaStream_t stream);
@@ -58,6 +62,19 @@ int b200q_w4a16_gemm(const void* x, const int32_t* qweight, const void* scales, 
   if (M >= W4A16_TC_MIN_M)
     return w4a16_tc(x, qweight, scales, zeros, single_out(y, N), M, N, K, group, dtype, workspace, workspace_bytes, st);
   return w4a16_decode(x, qweight, scales, zeros, single_out(y, N), M, N, K, group, dtype, workspace, workspace_bytes, st);
+}
+
+int b200q_w4a16_dgrad(const void* dy, const int32_t* qweight, const void* scales, const void* zeros, void* dx,
+                      int64_t M, int64_t N, int64_t K, int64_t group, int dtype, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  using namespace b200q;
+  int rc = check_w4a16_shape(M, N, K, group, dtype);
+  if (rc) return rc;
+  if (M == 0) return B200Q_OK;
+  if (!dy || !qweight || !scales || !zeros || !dx) return fail(B200Q_ERR_SHAPE, "w4a16 dgrad: null pointer argument");
+  if (reinterpret_cast<uintptr_t>(dx) & 15) return fail(B200Q_ERR_ALIGN, "w4a16 dgrad: dx must be 16-byte aligned");
+  return w4a16_tc_dgrad(dy, qweight, scales, zeros, dx, M, N, K, group, dtype, workspace, workspace_bytes,
+                        reinterpret_cast<cudaStream_t>(stream));
 }
 
 int b200q_moe_grouped_gemm(const void* x, const int32_t* qweight, const void* scales, const void* zeros,

@@ -29,6 +29,20 @@
 // which yields columns (0,4), (1,5), (2,6), (3,7) of a word; the B operand is
 // stored in that column order and the epilogue undoes the permutation in
 // registers.
+//
+// The same skeleton computes the input gradient of the projection (MODE_DX):
+//   dx[M, K] = dy[M, N] . W^T,
+// i.e. output columns are weight rows k and the contraction runs over the
+// weight's columns n.  The packed layout is contiguous along n, so the
+// dequantised stage [256 weight rows x 64 columns] is the K-major B operand:
+// one packed word is one 16-byte chunk of a 128-byte operand row, put into
+// column order by four PRMTs (the nibble pairs lie along the contraction, where
+// dy's order is fixed, not along the output, where the epilogue could undo it).
+// A tile's 256 weight rows span 256 / g groups, so a stage carries that many
+// 64-wide scale and zero rows; a warp's 16 rows lie in one group.
+// Bound: the tensor cores, as the forward; M=4096, N=4096, K=14336 g128 moves
+// 182 MB (28 us at the measured copy rate) against 481 GFLOP (292 us at the
+// measured bf16 rate).
 #include <algorithm>
 
 #include "w4a16_dq.cuh"
@@ -49,7 +63,7 @@ struct Grouped {
   int E;
 };
 
-enum { MODE_PLAIN = 0, MODE_GROUPED = 1, MODE_GLU = 2 };
+enum { MODE_PLAIN = 0, MODE_GROUPED = 1, MODE_GLU = 2, MODE_DX = 3 };
 
 template <bool BF16, int MB, int MODE>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -58,6 +72,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const __grid_constant__ OutSet out, int M, int N, int K, int group, int splits, uint8_t* __restrict__ ws,
                     const __grid_constant__ Grouped grp) {
   constexpr bool GLU = MODE == MODE_GLU;
+  constexpr bool DX = MODE == MODE_DX;  // N: weight rows (output columns), K: weight columns (contraction)
+  // accumulator column p of a group of 8 -> output column
+  auto out_col = [](int p) { return DX ? p : slot_col(p); };
   constexpr int OUTC = GLU ? BN / 2 : BN;  // output columns per tile
   using T = typename DT<BF16>::T;
   using C = Cfg<MB>;
@@ -82,7 +99,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int n0 = n_tile * OUTC;  // first output (and weight) column of the tile
   int m0 = m_tile * BM * MB, m_end = M, wk0 = 0;
   int mb_act = MB;  // 128-row blocks of the tile that hold rows (grouped: an expert's last tile may need one)
-  if (MODE != MODE_PLAIN) {
+  if (MODE == MODE_GROUPED || MODE == MODE_GLU) {
     // find this CTA's expert and row tile; CTAs past the last tile exit
     int e = 0, t = m_tile;
     for (; e < grp.E; ++e) {
@@ -103,7 +120,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int k_begin = (int)((long long)split * nk_total / splits);
   const int k_end = (int)((long long)(split + 1) * nk_total / splits);
   const int nk = k_end - k_begin;
-  const int srows = group >= BK ? 1 : BK / group;
+  const int srows = DX ? BN / group : (group >= BK ? 1 : BK / group);  // scale rows of a stage
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < SX; ++s) {
@@ -138,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == W_PROD) {
     // ---------------------------------------------------------------- weight producer
     if (lane == 0) {
-      const uint32_t stage_tx = WQ_BYTES + 2u * srows * BN * 2u;
+      const uint32_t stage_tx = WQ_BYTES + 2u * srows * (DX ? BK : BN) * 2u;
       for (int it = 0; it < nk; ++it) {
         const int s = it % SW;
         if (it >= SW && !mbar_wait(&w_empty[s], ((it / SW) - 1) & 1, status)) {
@@ -147,7 +164,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         const int kb = wk0 + (k_begin + it) * BK;
         mbar_arrive_expect_tx(&w_full[s], stage_tx);
-        if (!GLU) {
+        if (DX) {
+          tma_load_2d(smem + OFF_WQ + s * WQ_BYTES, &tm_wq, kb / 8, n0, &w_full[s]);
+          tma_load_2d(smem + OFF_S + s * SZ_BYTES, &tm_s, kb, n0 / group, &w_full[s]);
+          tma_load_2d(smem + OFF_Z + s * SZ_BYTES, &tm_z, kb, n0 / group, &w_full[s]);
+        } else if (!GLU) {
           tma_load_2d(smem + OFF_WQ + s * WQ_BYTES, &tm_wq, n0 / 8, kb, &w_full[s]);
           tma_load_2d(smem + OFF_S + s * SZ_BYTES, &tm_s, n0, kb / group, &w_full[s]);
           tma_load_2d(smem + OFF_Z + s * SZ_BYTES, &tm_z, n0, kb / group, &w_full[s]);
@@ -187,7 +208,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp == W_MMA) {
     // ---------------------------------------------------------------- MMA issuer
     if (lane == 0) {
-      const uint32_t idesc = idesc_f16(BM, BN, BF16 ? 1 : 0, /*a_mn=*/0, /*b_mn=*/1);
+      const uint32_t idesc = idesc_f16(BM, BN, BF16 ? 1 : 0, /*a_mn=*/0, /*b_mn=*/DX ? 0 : 1);
       for (int it = 0; it < nk; ++it) {
         const int s = it % SX, j = it % S2;
         if (!mbar_wait(&x_full[s], (it / SX) & 1, status) || !mbar_wait(&b_full[j], (it / S2) & 1, status)) {
@@ -200,8 +221,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int kk = 0; kk < BK / 16; ++kk) {
           // A: K-major, 8-row groups 1024 B apart; B: MN-major, 64-column atoms
-          // 1024 B apart, 8-row K groups 4096 B apart
-          const uint64_t bd = smem_desc(bb + kk * 8192, 1024, 4096, 2);
+          // 1024 B apart, 8-row K groups 4096 B apart (DX: K-major as A)
+          const uint64_t bd = DX ? smem_desc(bb + kk * 32, 16, 1024, 2) : smem_desc(bb + kk * 8192, 1024, 4096, 2);
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb) {
             if (mb >= mb_act) break;
@@ -222,11 +243,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     static_assert(WPR == 2, "a thread's words i < WORDS/2 lie in K rows 0..31 of the stage, the rest in 32..63");
     // loop-invariant parts of every address; ring slots and phases advance
     // incrementally (no divisions in the loop)
+    // DX: warp dw has weight rows 16 dw .. 16 dw + 15 of the tile, four per
+    // word index i; lane = (row within the four, word column)
     const uint32_t* wq_t = reinterpret_cast<const uint32_t*>(smem + OFF_WQ) +
-                           (GLU ? (lane >> 4) * (BK * 16) + (rr + 8 * (dw >> 3)) * 16 + (lane & 15)
+                           (DX ? dw * 128 + lane
+                            : GLU ? (lane >> 4) * (BK * 16) + (rr + 8 * (dw >> 3)) * 16 + (lane & 15)
                                 : (rr + 8 * (dw >> 3)) * 32 + lane);
-    constexpr int WQ_ROW_STEP = GLU ? 8 * WPR * 16 : 8 * WPR * 32;  // words between a thread's words i, i+1
-    uint8_t* b_t = smem + OFF_B + ((dw >> 3) * 4 + nb) * 1024 + rr * 128 + ((ch ^ rr) << 4);
+    constexpr int WQ_ROW_STEP = DX ? 32 : GLU ? 8 * WPR * 16 : 8 * WPR * 32;  // words between a thread's words i, i+1
+    uint8_t* b_t = smem + OFF_B + (DX ? dw * 2048 : ((dw >> 3) * 4 + nb) * 1024 + rr * 128 + ((ch ^ rr) << 4));
+    // DX: operand row (4 (i & 1) + nb) of an 8-row group, chunk ch, for even and odd i
+    const int dx_even = nb * 128 + ((ch ^ nb) << 4), dx_odd = (nb + 4) * 128 + ((ch ^ (nb + 4)) << 4);
+    const int dx_srow = DX ? (dw * 16 / group) * (BK * 2) : 0;
     int s = 0, j = 0;
     uint32_t ph_w = 0, ph_b = 1;
     for (int it = 0; it < nk; ++it) {
@@ -238,14 +265,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         s_err = 1;
         break;
       }
-      const uint8_t* srow0 = smem + OFF_S + s * SZ_BYTES;
-      const uint8_t* zrow0 = smem + OFF_Z + s * SZ_BYTES;
+      const uint8_t* srow0 = smem + OFF_S + s * SZ_BYTES + dx_srow;
+      const uint8_t* zrow0 = smem + OFF_Z + s * SZ_BYTES + dx_srow;
       // packed words and scale/zero constants go to registers first, so the
       // weight slot is released before the dequantised stores start; with
       // group 32 the stage's second scale row serves K rows 32..63 (words
       // i >= WORDS/2), otherwise q1 is q0
-      const ColQ q0 = load_colq<BF16>(srow0, zrow0, lane);
-      const ColQ q1 = srows > 1 ? load_colq<BF16>(srow0 + BN * 2, zrow0 + BN * 2, lane) : q0;
+      const ColQ q0 = load_colq<BF16>(srow0, zrow0, DX ? ch : lane);
+      const ColQ q1 = !DX && srows > 1 ? load_colq<BF16>(srow0 + BN * 2, zrow0 + BN * 2, lane) : q0;
       const uint32_t* wq = wq_t + s * (WQ_BYTES / 4);
       uint32_t wv[WORDS];
 #pragma unroll
@@ -256,7 +283,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
       for (int i = 0; i < WORDS; ++i) {
         const uint4 v = dequant_word<BF16>(wv[i], i >= WORDS / 2 ? q1 : q0);
-        *reinterpret_cast<uint4*>(bt + i * (WPR * 4 * 1024)) = v;
+        if (DX)
+          *reinterpret_cast<uint4*>(bt + (i >> 1) * 1024 + ((i & 1) ? dx_odd : dx_even)) =
+              make_uint4(prmt(v.x, v.y, 0x5410), prmt(v.z, v.w, 0x5410), prmt(v.x, v.y, 0x7632), prmt(v.z, v.w, 0x7632));
+        else
+          *reinterpret_cast<uint4*>(bt + i * (WPR * 4 * 1024)) = v;
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -298,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_ld32(tl + acc * BN + ocol, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int p = 0; p < 32; ++p) v[(p & ~7) | slot_col(p & 7)] = __uint_as_float(r[p]);
+        for (int p = 0; p < 32; ++p) v[(p & ~7) | out_col(p & 7)] = __uint_as_float(r[p]);
         if (GLU) {
           // up columns sit 128 TMEM columns to the right; h = SiLU(g) * u with
           // g and u rounded to the activation type first and one rounding of
@@ -307,9 +338,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           tmem_ld_wait();
 #pragma unroll
           for (int p = 0; p < 32; ++p) {
-            const float g = (float)(T)v[(p & ~7) | slot_col(p & 7)];
+            const float g = (float)(T)v[(p & ~7) | out_col(p & 7)];
             const float u = (float)(T)__uint_as_float(r[p]);
-            v[(p & ~7) | slot_col(p & 7)] = g / (1.f + expf(-g)) * u;
+            v[(p & ~7) | out_col(p & 7)] = g / (1.f + expf(-g)) * u;
           }
         }
         if (splits == 1) {
@@ -388,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_ld_wait();
         float v[32];
 #pragma unroll
-        for (int p = 0; p < 32; ++p) v[(p & ~7) | slot_col(p & 7)] = __uint_as_float(r[p]);
+        for (int p = 0; p < 32; ++p) v[(p & ~7) | out_col(p & 7)] = __uint_as_float(r[p]);
 #pragma unroll
         for (int p = 0; p < 8; ++p)
           st_cluster_v4(base + (cslot + 4 * p) * 4, v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
@@ -488,37 +519,11 @@ Plan plan(int64_t M, int64_t N, int64_t K, int sms) {
   return p;
 }
 
-}  // namespace tc
-
-size_t w4a16_tc_ws_bytes(int64_t M, int64_t N, int64_t K, int device) {
-  return tc::plan(M, N, K, num_sms(device)).ws_bytes;
-}
-
-int w4a16_tc(const void* x, const int32_t* qweight, const void* scales, const void* zeros, const OutSet& out,
-             int64_t M, int64_t N, int64_t K, int64_t group, int dtype, void* workspace, size_t workspace_bytes,
-             cudaStream_t stream) {
-  using namespace tc;
-  Plan p = plan(M, N, K, num_sms(-1));
-  if (!workspace || workspace_bytes < p.ws_bytes)
-    return fail(B200Q_ERR_WORKSPACE, "w4a16: workspace of " + std::to_string(p.ws_bytes) + " bytes required");
-  const CUtensorMapDataType h16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
-  const uint32_t srows = group >= BK ? 1 : (uint32_t)(BK / group);
-  CUtensorMap tx, twq, ts, tz;
-  int rc;
-  if ((rc = encode_2d(&tx, h16, x, K, M, (uint64_t)K * 2, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
-  if ((rc = encode_2d(&twq, CU_TENSOR_MAP_DATA_TYPE_INT32, qweight, N / 8, K, (uint64_t)N / 2, BN / 8, BK,
-                      CU_TENSOR_MAP_SWIZZLE_NONE)))
-    return rc;
-  if ((rc = encode_2d(&ts, h16, scales, N, K / group, (uint64_t)N * 2, BN, srows, CU_TENSOR_MAP_SWIZZLE_NONE)))
-    return rc;
-  if ((rc = encode_2d(&tz, h16, zeros, N, K / group, (uint64_t)N * 2, BN, srows, CU_TENSOR_MAP_SWIZZLE_NONE)))
-    return rc;
-  const bool bf = dtype == B200Q_DTYPE_BF16;
-  auto kern = p.mb == 2 ? (bf ? w4a16_tc_kernel<true, 2, MODE_PLAIN> : w4a16_tc_kernel<false, 2, MODE_PLAIN>)
-                        : (bf ? w4a16_tc_kernel<true, 1, MODE_PLAIN> : w4a16_tc_kernel<false, 1, MODE_PLAIN>);
-  const uint32_t smem = p.mb == 2 ? Cfg<2>::SMEM : Cfg<1>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(w4a16 tc)");
+// Launches `kern` over the plan's tiles, `splits` CTAs of a tile as a cluster.
+template <class Kern>
+int launch(Kern kern, uint32_t smem, Plan p, const CUtensorMap& tx, const CUtensorMap& twq, const CUtensorMap& ts,
+           const CUtensorMap& tz, const OutSet& out, int64_t M, int64_t N, int64_t K, int64_t group, void* workspace,
+           cudaStream_t stream, const char* what) {
   // a cluster of `splits` CTAs (one SM each) must fit in one GPC: shrink the
   // cluster until every cluster of the grid is resident at once
   while (p.splits > 1) {
@@ -552,10 +557,76 @@ int w4a16_tc(const void* x, const int32_t* qweight, const void* scales, const vo
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   Grouped none = {};
-  e = cudaLaunchKernelEx(&cfg, kern, tx, twq, ts, tz, out, (int)M, (int)N, (int)K, (int)group, p.splits,
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, twq, ts, tz, out, (int)M, (int)N, (int)K, (int)group, p.splits,
                          reinterpret_cast<uint8_t*>(workspace), none);
-  if (e != cudaSuccess) return check_cuda(e, "w4a16 tc launch");
-  return check_cuda(cudaGetLastError(), "w4a16 tc launch");
+  if (e != cudaSuccess) return check_cuda(e, what);
+  return check_cuda(cudaGetLastError(), what);
+}
+
+}  // namespace tc
+
+size_t w4a16_tc_ws_bytes(int64_t M, int64_t N, int64_t K, int device) {
+  return tc::plan(M, N, K, num_sms(device)).ws_bytes;
+}
+
+int w4a16_tc(const void* x, const int32_t* qweight, const void* scales, const void* zeros, const OutSet& out,
+             int64_t M, int64_t N, int64_t K, int64_t group, int dtype, void* workspace, size_t workspace_bytes,
+             cudaStream_t stream) {
+  using namespace tc;
+  Plan p = plan(M, N, K, num_sms(-1));
+  if (!workspace || workspace_bytes < p.ws_bytes)
+    return fail(B200Q_ERR_WORKSPACE, "w4a16: workspace of " + std::to_string(p.ws_bytes) + " bytes required");
+  const CUtensorMapDataType h16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  const uint32_t srows = group >= BK ? 1 : (uint32_t)(BK / group);
+  CUtensorMap tx, twq, ts, tz;
+  int rc;
+  if ((rc = encode_2d(&tx, h16, x, K, M, (uint64_t)K * 2, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+  if ((rc = encode_2d(&twq, CU_TENSOR_MAP_DATA_TYPE_INT32, qweight, N / 8, K, (uint64_t)N / 2, BN / 8, BK,
+                      CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return rc;
+  if ((rc = encode_2d(&ts, h16, scales, N, K / group, (uint64_t)N * 2, BN, srows, CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return rc;
+  if ((rc = encode_2d(&tz, h16, zeros, N, K / group, (uint64_t)N * 2, BN, srows, CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return rc;
+  const bool bf = dtype == B200Q_DTYPE_BF16;
+  auto kern = p.mb == 2 ? (bf ? w4a16_tc_kernel<true, 2, MODE_PLAIN> : w4a16_tc_kernel<false, 2, MODE_PLAIN>)
+                        : (bf ? w4a16_tc_kernel<true, 1, MODE_PLAIN> : w4a16_tc_kernel<false, 1, MODE_PLAIN>);
+  const uint32_t smem = p.mb == 2 ? Cfg<2>::SMEM : Cfg<1>::SMEM;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(w4a16 tc)");
+  return launch(kern, smem, p, tx, twq, ts, tz, out, M, N, K, group, workspace, stream, "w4a16 tc launch");
+}
+
+// dx[M, K] = dy[M, N] . W^T: the kernel's output columns are the weight's K
+// rows and its contraction the weight's N columns.
+int w4a16_tc_dgrad(const void* dy, const int32_t* qweight, const void* scales, const void* zeros, void* dx, int64_t M,
+                   int64_t N, int64_t K, int64_t group, int dtype, void* workspace, size_t workspace_bytes,
+                   cudaStream_t stream) {
+  using namespace tc;
+  Plan p = plan(M, K, N, num_sms(-1));
+  if (p.tiles_m > 65535) return fail(B200Q_ERR_SHAPE, "w4a16 dgrad: M too large");
+  if (!workspace || workspace_bytes < p.ws_bytes)
+    return fail(B200Q_ERR_WORKSPACE, "w4a16 dgrad: workspace of " + std::to_string(p.ws_bytes) + " bytes required");
+  const CUtensorMapDataType h16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  const uint32_t srows = (uint32_t)(BN / group);
+  CUtensorMap tdy, twq, ts, tz;
+  int rc;
+  if ((rc = encode_2d(&tdy, h16, dy, N, M, (uint64_t)N * 2, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+  if ((rc = encode_2d(&twq, CU_TENSOR_MAP_DATA_TYPE_INT32, qweight, N / 8, K, (uint64_t)N / 2, BK / 8, BN,
+                      CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return rc;
+  if ((rc = encode_2d(&ts, h16, scales, N, K / group, (uint64_t)N * 2, BK, srows, CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return rc;
+  if ((rc = encode_2d(&tz, h16, zeros, N, K / group, (uint64_t)N * 2, BK, srows, CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return rc;
+  const bool bf = dtype == B200Q_DTYPE_BF16;
+  auto kern = p.mb == 2 ? (bf ? w4a16_tc_kernel<true, 2, MODE_DX> : w4a16_tc_kernel<false, 2, MODE_DX>)
+                        : (bf ? w4a16_tc_kernel<true, 1, MODE_DX> : w4a16_tc_kernel<false, 1, MODE_DX>);
+  const uint32_t smem = p.mb == 2 ? Cfg<2>::SMEM : Cfg<1>::SMEM;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(w4a16 dgrad)");
+  return launch(kern, smem, p, tdy, twq, ts, tz, single_out(dx, K), M, K, N, group, workspace, stream,
+                "w4a16 dgrad launch");
 }
 
 // Grouped W4A16 over E experts (the MoE expert GEMMs in one launch): rows of

@@ -57,6 +57,28 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+class _NoSwitch:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_no_switch = _NoSwitch()
+
+
+def _device(device: torch.device):
+    """Context in which ``device`` is the current one (kernels launch on the current device)."""
+    return _no_switch if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _same_device(op: str, first: torch.Tensor, *rest: Optional[torch.Tensor]) -> None:
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{op}: tensors on {first.device} and {t.device}")
+
+
 @torch.library.custom_op("b200q::w4a16_gemm", mutates_args=())
 def w4a16_gemm(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
                group: int) -> torch.Tensor:
@@ -95,6 +117,62 @@ def w4a16_gemm(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zer
 @w4a16_gemm.register_fake
 def _(x, qweight, scales, zeros, group):
     return x.new_empty((x.shape[0], qweight.shape[1] * 8))
+
+
+@torch.library.custom_op("b200q::w4a16_dgrad", mutates_args=())
+def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
+                group: int) -> torch.Tensor:
+    """dx[M, K] = dy[M, N] . ((unpack(qweight) - zeros) * scales)^T, dx in dy.dtype:
+    the input gradient of w4a16_gemm (the weights are frozen)."""
+    if not dy.is_cuda:
+        raise RuntimeError("b200q::w4a16_dgrad runs on CUDA tensors only (no CPU implementation)")
+    if dy.dim() != 2 or qweight.dim() != 2:
+        raise ValueError("dy must be [M, N] and qweight [K, N/8]")
+    if qweight.dtype != torch.int32:
+        raise TypeError("qweight must be int32")
+    M, N = dy.shape
+    K = qweight.shape[0]
+    if qweight.shape[1] * 8 != N:
+        raise ValueError(f"qweight has {qweight.shape[1] * 8} columns, dy has N={N}")
+    if group <= 0 or K % group:
+        raise ValueError(f"K={K} is not a multiple of group={group}")
+    for name, t in (("scales", scales), ("zeros", zeros)):
+        if tuple(t.shape) != (K // group, N):
+            raise ValueError(f"{name} must be [{K // group}, {N}], got {tuple(t.shape)}")
+    dt = _dtype_code(dy.dtype)
+    _same_device("w4a16_dgrad", dy, qweight, scales, zeros)
+    dy, qweight, scales, zeros = (_aligned(t) for t in (dy, qweight, scales.to(dy.dtype), zeros.to(dy.dtype)))
+    dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
+    if M == 0:
+        return dx
+    with _device(dy.device):
+        ws = workspace(dy.device, 256)
+        _lib.check(_lib.lib().b200q_w4a16_dgrad(dy.data_ptr(), qweight.data_ptr(), scales.data_ptr(),
+                                                zeros.data_ptr(), dx.data_ptr(), M, N, K, group, dt, ws.data_ptr(),
+                                                ws.numel(), _stream_ptr(dy.device)))
+    return dx
+
+
+@w4a16_dgrad.register_fake
+def _(dy, qweight, scales, zeros, group):
+    return dy.new_empty((dy.shape[0], qweight.shape[0]))
+
+
+def _w4a16_setup(ctx, inputs, output):
+    x, qweight, scales, zeros, group = inputs
+    if scales.requires_grad or zeros.requires_grad:
+        raise ValueError("w4a16_gemm: the quantised weight is frozen, scales and zeros have no gradient")
+    ctx.save_for_backward(qweight, scales, zeros)
+    ctx.group = group
+
+
+def _w4a16_backward(ctx, dy):
+    qweight, scales, zeros = ctx.saved_tensors
+    dx = w4a16_dgrad(dy, qweight, scales, zeros, ctx.group) if ctx.needs_input_grad[0] else None
+    return dx, None, None, None, None
+
+
+w4a16_gemm.register_autograd(_w4a16_backward, setup_context=_w4a16_setup)
 
 
 def _ptr_array(ptrs) -> "ctypes.Array":
@@ -251,6 +329,80 @@ def _(router_logits):
     return (router_logits.new_empty((T, 2), **i32), router_logits.new_empty((T, 2)),
             router_logits.new_empty((E + 1,), **i32), router_logits.new_empty((2 * T,), **i32),
             router_logits.new_empty((T, 2), **i32))
+
+
+_LOGITS_CODES = {torch.float16: _lib.DTYPE_FP16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_FP32}
+
+
+def _balance_forward(logits, topi, mask):
+    T, E = logits.shape
+    dev = logits.device
+    L = _lib.lib()
+    nbytes = L.b200q_moe_balance_scratch_bytes(T, E)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    coef = torch.empty((E,), dtype=torch.float32, device=dev)
+    counts = torch.empty((E,), dtype=torch.int32, device=dev)
+    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    with _device(dev):
+        ws = workspace(dev, 256)
+        _lib.check(L.b200q_moe_balance(logits.data_ptr(), topi.data_ptr(), mask.data_ptr() if mask is not None else None,
+                                       T, E, topi.shape[1], _LOGITS_CODES[logits.dtype], loss.data_ptr(),
+                                       counts.data_ptr(), coef.data_ptr(), scratch.data_ptr(), nbytes, ws.data_ptr(),
+                                       _stream_ptr(dev)))
+    return loss, counts, coef
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topi, mask):
+        lg = logits.contiguous()
+        loss, counts, coef = _balance_forward(lg, topi, mask)
+        ctx.save_for_backward(lg, mask, coef)
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss, _):
+        lg, mask, coef = ctx.saved_tensors
+        T, E = lg.shape
+        dloss = dloss.to(torch.float32).contiguous()
+        d = torch.empty_like(lg)
+        with _device(lg.device):
+            _lib.check(_lib.lib().b200q_moe_balance_grad(lg.data_ptr(), mask.data_ptr() if mask is not None else None,
+                                                         coef.data_ptr(), dloss.data_ptr(), T, E,
+                                                         _LOGITS_CODES[lg.dtype], d.data_ptr(), _stream_ptr(lg.device)))
+        return d, None, None
+
+
+def moe_balance_loss(router_logits: torch.Tensor, topi: torch.Tensor,
+                     token_mask: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Load-balance loss of a top-k router and the per-expert token counts.
+
+    router_logits [T, E] fp16 / bf16 / fp32, topi [T, k] integer (moe_route's
+    first output for k = 2; -1 is a dropped choice), token_mask [T] bool (False:
+    padding, counts nowhere).  loss = E sum_e f_e P_e, fp32 scalar, with f_e the
+    share of the live choices that went to expert e and P_e the mean softmax
+    probability of e; counts [E] int32.  The loss is differentiable in
+    router_logits (f is a count and carries no gradient); see include/b200q.h
+    for rows that are all -inf and for indices out of range."""
+    if not router_logits.is_cuda:
+        raise RuntimeError("b200q moe_balance_loss runs on CUDA tensors only")
+    if router_logits.dim() != 2 or topi.dim() != 2 or topi.shape[0] != router_logits.shape[0]:
+        raise ValueError("router_logits must be [T, E] and topi [T, k]")
+    if router_logits.dtype not in _LOGITS_CODES:
+        raise TypeError(f"router_logits must be float16, bfloat16 or float32, got {router_logits.dtype}")
+    if topi.dtype not in (torch.int32, torch.int64):
+        raise TypeError("topi must be int32 or int64")
+    _same_device("moe_balance_loss", router_logits, topi, token_mask)
+    if token_mask is not None:
+        if token_mask.dtype != torch.bool or tuple(token_mask.shape) != (router_logits.shape[0],):
+            raise ValueError("token_mask must be bool [T]")
+        token_mask = token_mask.contiguous()
+    topi = topi.to(torch.int32).contiguous()
+    if torch.is_grad_enabled() and router_logits.requires_grad:
+        return _BalanceLoss.apply(router_logits, topi, token_mask)
+    return _balance_forward(router_logits.contiguous(), topi, token_mask)[:2]
 
 
 def moe_grouped_gemm(x: torch.Tensor, offsets: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
