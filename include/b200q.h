@@ -250,6 +250,43 @@ int b200q_lora_shrink(const void* x, const void* A, const int64_t* lora_ids, int
 int b200q_lora_expand_add(const void* base, const void* lo, const void* B, const int64_t* lora_ids, int64_t T,
                           int64_t r, int64_t N, int64_t L, int dtype, void* y, void* stream);
 
+/* Adapters of many requests beside one shared projection, with gradients.
+ * Addition to LORA_REF (generate_tasks.py:397-424), whose form
+ * b200q_lora_shrink / b200q_lora_expand_add keep: tokens without an adapter, a
+ * scaling per adapter, tokens of one adapter multiplied together, and
+ *   lo[t]  = s[id_t] x[t] . A[id_t]         y[t]  = base[t] + lo[t] . B[id_t]
+ *   dlo[t] = s[id_t] dy[t] . B[id_t]^T      dx[t] = base[t] + dlo[t] . A[id_t]^T
+ *   dA[a] = sum_{id_t = a} x[t]^T dlo[t]    dB[a] = sum_{id_t = a} lo[t]^T dy[t]
+ * x [T, D], dy and y [T, N], A [L, D, r], B [L, r, N] in fp16 or bf16, s =
+ * scaling [L] fp32 or NULL (1).  fp32 accumulation, lo and dlo in fp32, one
+ * rounding of each result.  Results do not depend on timing.  1 <= r <= 64,
+ * 1 <= L <= 1023, D and N any width up to 2^22 (multiples of 8, with r a
+ * multiple of 8, run fastest), 16-byte aligned pointers.
+ *
+ * plan: groups the batch's tokens by adapter, once for every projection of
+ * that batch.  lora_ids [T] int64, -1 = no adapter; any other id outside [0, L)
+ * counts as none and sets B200Q_DEV_ERR_BOUNDS in the status word (when
+ * workspace is non-NULL).  plan_bytes >= b200q_lora_plan_bytes(T, L) (0: sizes
+ * out of range). */
+size_t b200q_lora_plan_bytes(int64_t T, int64_t L);
+int b200q_lora_plan(const int64_t* lora_ids, int64_t T, int64_t L, int32_t* plan, size_t plan_bytes, void* workspace,
+                    void* stream);
+
+/* y from x (transposed = 0) or dx from dy (transposed = 1: x is dy [T, N] and
+ * y is dx [T, D]).  base: NULL for zeros; may be y itself; a token without an
+ * adapter gets base.  y: NULL to compute mid alone.  mid: lo (or dlo), fp32,
+ * b200q_lora_mid_bytes(T, r) of it, any contents; rows of tokens without an
+ * adapter are left as they were. */
+size_t b200q_lora_mid_bytes(int64_t T, int64_t r);
+int b200q_lora_apply(const void* x, const void* base, const void* A, const void* B, const float* scaling,
+                     const int32_t* plan, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype,
+                     int transposed, void* y, float* mid, void* stream);
+
+/* dA (from x and dlo) and dB (from lo and dy), either NULL to leave it out; an
+ * adapter without tokens gets zeros. */
+int b200q_lora_grads(const void* x, const void* dy, const float* lo, const float* dlo, const int32_t* plan, int64_t T,
+                     int64_t D, int64_t N, int64_t r, int64_t L, int dtype, void* dA, void* dB, void* stream);
+
 /* Grouped W4A16 GEMM over the experts of a MoE layer, one launch for all
  * experts.  x [rows, K] holds every expert's rows contiguously, expert e's at
  * [offsets[e], offsets[e+1]) (offsets [E+1] int32 on the device, as written

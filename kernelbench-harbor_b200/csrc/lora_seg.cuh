@@ -1,0 +1,266 @@
+// Shared pieces of the multi-adapter kernels (lora_plan.cu, lora_small.cu,
+// lora_tiles.cu, lora_grads.cu): adapters of many requests beside one shared
+// projection,
+//   y[t]  = base[t] + s[id_t] (x[t] . A[id_t]) . B[id_t]
+//   dx[t] = base[t] + s[id_t] (dy[t] . B[id_t]^T) . A[id_t]^T
+// Both are "shrink" (contract a wide row with a thin matrix, P) and "expand"
+// (times a thin matrix, Q, added to a wide row); the backward form takes B and
+// A transposed (TR).  Tokens are grouped by adapter (the plan), so a tile of
+// rows shares one adapter and the products run on the tensor cores; mid, the
+// row between the two (s included), stays in fp32.
+//
+// mma.sync m16n8k16 is used, not tcgen05: the operators read and write wide
+// rows once and do 2 r flops per value (r <= 64), so memory bounds them
+// up to r = 64 and the register fragments let a row go from HBM into the
+// multiply without shared memory: of the contraction index, any order serves
+// that both operands share, so a thread takes 8 consecutive values of a row
+// (one 16-byte load) as its parts of two k16 steps; of the output columns, the
+// order is chosen so that a thread ends with 8 consecutive ones.
+#pragma once
+#include "common.cuh"
+
+namespace b200q {
+namespace lora {
+
+constexpr int MAX_RANK = 64;
+constexpr int MAX_ADAPTERS = 1023;
+constexpr int64_t MAX_TOKENS = 1ll << 24;
+constexpr int ROWS_S = 16, ROWS_L = 128;  // rows of a small / large tile
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+
+// ------------------------------------------------------------------ plan layout (int32 words)
+//   [0] small tiles, [1] large tiles, [2..8) unused
+//   seg_off [L + 2]: adapter a's rows are order[seg_off[a] .. seg_off[a + 1]);
+//                    segment L holds the tokens without an adapter
+//   order [T]: token indices, ascending within a segment
+//   tiles_s, tiles_l: {adapter or -1, first position in order, rows, 0} each
+struct PlanLayout {
+  int64_t seg, order, small, large, words, max_small, max_large;
+};
+
+inline int64_t max_tiles(int64_t T, int64_t L, int64_t rows) {
+  const int64_t n = T / rows + L + 1;
+  return n < T ? n : T;
+}
+
+inline PlanLayout plan_layout(int64_t T, int64_t L) {
+  PlanLayout p;
+  auto up4 = [](int64_t v) { return (v + 3) / 4 * 4; };
+  p.max_small = max_tiles(T, L, ROWS_S);
+  p.max_large = max_tiles(T, L, ROWS_L);
+  p.seg = 8;
+  p.order = up4(p.seg + L + 2);
+  p.small = up4(p.order + T);
+  p.large = p.small + 4 * p.max_small;
+  p.words = p.large + 4 * p.max_large;
+  return p;
+}
+
+// Row pitch of mid: the rank rounded up to a multiple of the MMA's 16 that the kernels are built for.
+inline int mid_pitch(int64_t r) { return r <= 16 ? 16 : r <= 32 ? 32 : 64; }
+
+// ------------------------------------------------------------------ element types
+template <class T>
+__device__ __forceinline__ float tf(T v);
+template <>
+__device__ __forceinline__ float tf<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float tf<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T ft(float v);
+template <>
+__device__ __forceinline__ __half ft<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 ft<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(T a, T b) {
+  return (uint32_t) * reinterpret_cast<uint16_t*>(&a) | ((uint32_t) * reinterpret_cast<uint16_t*>(&b) << 16);
+}
+
+template <class T>
+__device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
+  T v[2];
+  *reinterpret_cast<uint32_t*>(v) = w;
+  a = tf<T>(v[0]);
+  b = tf<T>(v[1]);
+}
+
+// v = hi + lo to twice the type's significand: the products of mid with the
+// thin matrix keep fp32's accuracy to ~2^-16 (bf16) or 2^-22 (fp16) of a value.
+// An infinity or NaN stays in hi alone.
+template <class T>
+__device__ __forceinline__ void split(float v, T& hi, T& lo) {
+  hi = ft<T>(v);
+  const float rest = v - tf<T>(hi);
+  lo = ft<T>(fabsf(rest) < INFINITY ? rest : 0.f);
+}
+
+// Power-of-two factor of a value's exponent and its inverse, so that v * inv
+// lies in [1, 2): fp16 has 5 exponent bits, and mid may leave their range.
+// 0, subnormals, infinities and NaN give 1.
+__device__ __forceinline__ void pow2_of(float v, float& fac, float& inv) {
+  const uint32_t e = (__float_as_uint(v) >> 23) & 0xffu;
+  fac = 1.f;
+  inv = 1.f;
+  if (e != 0 && e != 255) {
+    const uint32_t c = e > 253 ? 253 : e;
+    fac = __uint_as_float(c << 23);
+    inv = __uint_as_float((254 - c) << 23);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void mma16816(float* d, const uint32_t a0, const uint32_t a1, const uint32_t a2,
+                                         const uint32_t a3, const uint32_t b0, const uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float* d, const uint32_t a0, const uint32_t a1, const uint32_t a2,
+                                                 const uint32_t a3, const uint32_t b0, const uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float* d, const uint32_t a0, const uint32_t a1,
+                                                        const uint32_t a2, const uint32_t a3, const uint32_t b0,
+                                                        const uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ------------------------------------------------------------------ rows of any width
+// Values [k, k + 8) of a row of K, zeros past its end.  VEC: K % 8 == 0 and
+// 16-byte aligned rows, k a multiple of 8: all in or all out.
+template <class T, bool VEC>
+__device__ __forceinline__ uint4 ld8(const T* row, int k, int K) {
+  if constexpr (VEC) {
+    return k < K ? __ldg(reinterpret_cast<const uint4*>(row + k)) : make_uint4(0, 0, 0, 0);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = k + 2 * i < K ? reinterpret_cast<const uint16_t*>(row)[k + 2 * i] : 0;
+      const uint32_t b = k + 2 * i + 1 < K ? reinterpret_cast<const uint16_t*>(row)[k + 2 * i + 1] : 0;
+      w[i] = a | (b << 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ uint2 ld4(const T* row, int k, int K) {
+  if constexpr (VEC) {
+    return k < K ? __ldg(reinterpret_cast<const uint2*>(row + k)) : make_uint2(0, 0);
+  } else {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t a = k + 2 * i < K ? reinterpret_cast<const uint16_t*>(row)[k + 2 * i] : 0;
+      const uint32_t b = k + 2 * i + 1 < K ? reinterpret_cast<const uint16_t*>(row)[k + 2 * i + 1] : 0;
+      w[i] = a | (b << 16);
+    }
+    return make_uint2(w[0], w[1]);
+  }
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void st8(T* row, int k, int K, const uint4 v) {
+  if constexpr (VEC) {
+    if (k < K) *reinterpret_cast<uint4*>(row + k) = v;
+  } else {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i < K) reinterpret_cast<uint16_t*>(row)[k + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+  }
+}
+
+// 16 bytes of a row into shared memory: asynchronous where alignment allows.
+template <class T, bool VEC>
+__device__ __forceinline__ void stage8(void* dst, const T* row, int k, int K, bool in, const T* any) {
+  if constexpr (VEC)
+    cp_async16(smem_u32(dst), in && k < K ? row + k : any, in && k < K);
+  else
+    *reinterpret_cast<uint4*>(dst) = in ? ld8<T, false>(row, k, K) : make_uint4(0, 0, 0, 0);
+}
+
+// base + fac * c for the 8 consecutive columns of one row: c[p][h], c[p][h + 1] are columns 2p, 2p + 1
+template <class T>
+__device__ __forceinline__ uint4 add8(const uint4 b, const float (*c)[4], int h, float fac) {
+  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    float u, v;
+    unpack2<T>(w[p], u, v);
+    o[p] = pack2<T>(ft<T>(fmaf(fac, c[p][h], u)), ft<T>(fmaf(fac, c[p][h + 1], v)));
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Position of contraction row k in shared memory so that one ldmatrix row group
+// is what a fragment wants: with 8 consecutive k per thread (32-row groups)
+__device__ __forceinline__ int row32(int k) { return (k & ~31) | (((k >> 1) & 3) << 3) | (((k >> 3) & 3) << 1) | (k & 1); }
+// and the k at position p when a thread holds 4 consecutive k (16-row groups)
+__device__ __forceinline__ int k_of_row16(int p) { return (p & ~15) | (((p >> 1) & 3) << 2) | (((p >> 3) & 1) << 1) | (p & 1); }
+
+// Rows [0, count) of a tile without an adapter: y = base (zeros without one), columns [n0, n1).
+template <class T, bool VEC>
+__device__ __forceinline__ void copy_rows(const T* base, T* y, const int32_t* rows, int count, int N, int n0, int n1) {
+  if (base == y) return;
+  const int g8 = (n1 - n0 + 7) / 8;
+  for (int i = threadIdx.x; i < count * g8; i += THREADS) {
+    const size_t off = (size_t)rows[i / g8] * N;
+    const int n = n0 + i % g8 * 8;
+    st8<T, VEC>(y + off, n, n1, base ? ld8<T, VEC>(base + off, n, N) : make_uint4(0, 0, 0, 0));
+  }
+}
+
+struct Args {
+  const void *x, *base, *P, *Q;
+  const float* scaling;
+  const int32_t* plan;
+  PlanLayout lay;
+  int D, N, r, mp;  // contraction width, output width, rank, mid pitch
+  void* y;
+  float* mid;
+  int64_t T, L;
+};
+
+int launch_small(const Args& a, int dtype, bool tr, cudaStream_t st);
+int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st);
+
+// Calls f(type, rank, aligned) with compile-time values; widths or ranks that
+// are not multiples of 8 take the general variant, built for the largest rank only.
+template <class F>
+int by_type(int dtype, int64_t r, bool vec, F f) {
+  auto rank = [&](auto t) {
+    if (!vec) return f(t, std::integral_constant<int, 64>{}, std::false_type{});
+    if (r <= 16) return f(t, std::integral_constant<int, 16>{}, std::true_type{});
+    if (r <= 32) return f(t, std::integral_constant<int, 32>{}, std::true_type{});
+    return f(t, std::integral_constant<int, 64>{}, std::true_type{});
+  };
+  return dtype == B200Q_DTYPE_FP16 ? rank(__half{}) : rank(__nv_bfloat16{});
+}
+
+}  // namespace lora
+}  // namespace b200q

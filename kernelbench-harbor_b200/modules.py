@@ -145,6 +145,39 @@ class MultiLoRAW4(nn.Module):
         return ops.lora_expand_add(base, lo, B, lora_ids, out=base)
 
 
+class LoRAW4A16Linear(nn.Module):
+    """W4A16 projection shared by many requests, each with an adapter of its
+    own or none: forward(x [..., K], qweight [K, N/8], scales, zeros
+    [K/g, N], A [L, K, r], B [L, r, N], lora_ids, scaling=None) -> [..., N] =
+    x . dequant(W) + scaling[id] (x . A[id]) . B[id].
+
+    lora_ids: one id per token (-1: no adapter), or the ops.lora_plan of those
+    ids, made once for all projections of a batch.  Differentiable in x, A and
+    B; the quantised weight is frozen."""
+
+    def forward(self, x, qweight, scales, zeros, A, B, lora_ids, scaling=None):
+        K = qweight.shape[0]
+        if scales.shape[0] == 0 or K % scales.shape[0]:
+            raise ValueError(f"scales rows ({scales.shape[0]}) must divide K ({K})")
+        lead = x.shape[:-1]
+        x2 = x.reshape(-1, K)
+        ids = lora_ids.reshape(-1) if isinstance(lora_ids, torch.Tensor) else lora_ids
+        base = ops.w4a16_gemm(x2, qweight, scales, zeros, K // scales.shape[0])
+        grad = torch.is_grad_enabled() and (base.requires_grad or A.requires_grad or B.requires_grad)
+        y = ops.lora_apply(base, x2, A, B, ids, scaling, out=None if grad else base)
+        return y.reshape(*lead, y.shape[-1])
+
+
+class MoEBalanceLoss(nn.Module):
+    """Load-balance loss of a top-k router: forward(router_logits [T, E],
+    topi [T, k], token_mask=None) -> (loss, counts [E]); see
+    ops.moe_balance_loss.  topi: ops.moe_route's first output for QuantizedMoE's
+    top 2."""
+
+    def forward(self, router_logits, topi, token_mask=None):
+        return ops.moe_balance_loss(router_logits, topi, token_mask)
+
+
 class FusedSiluFp8(nn.Module):
     """Drop-in for FUSED_SILU_REF.Model (generate_tasks.py:321-348):
     forward(y [T, 2H]) -> fp32 [T, H], SiLU(gate) * up quantised per 128

@@ -9,7 +9,7 @@ tensor is an error."""
 from __future__ import annotations
 
 import threading
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -551,6 +551,141 @@ def lora_expand_add(base: torch.Tensor, lo: torch.Tensor, B: torch.Tensor, lora_
                                                 N, L, _dtype_code(base.dtype), y.data_ptr(),
                                                 _stream_ptr(base.device)))
     return y
+
+
+class LoraPlan:
+    """A batch's tokens grouped by adapter: made once by lora_plan, used by
+    every projection that the batch passes through."""
+
+    __slots__ = ("data", "tokens", "adapters", "device")
+
+    def __init__(self, data: torch.Tensor, tokens: int, adapters: int):
+        self.data, self.tokens, self.adapters, self.device = data, tokens, adapters, data.device
+
+
+def lora_plan(lora_ids: torch.Tensor, n_adapters: int) -> LoraPlan:
+    """Groups the tokens of lora_ids [T] (integer; -1 = no adapter) for
+    lora_apply over ``n_adapters`` adapters.  Any other id outside
+    [0, n_adapters) counts as none and sets the device status bit.  The ids
+    are read on the device: no host synchronisation."""
+    if not lora_ids.is_cuda:
+        raise RuntimeError("b200q lora_plan runs on CUDA tensors only")
+    if lora_ids.dim() != 1 or lora_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError("lora_ids must be int32 or int64 [T]")
+    ids = lora_ids.to(torch.int64).contiguous()
+    T, dev = ids.numel(), ids.device
+    L = _lib.lib()
+    nbytes = L.b200q_lora_plan_bytes(T, n_adapters)
+    data = torch.empty((max(nbytes, 4) // 4,), dtype=torch.int32, device=dev)
+    with _device(dev):
+        ws = workspace(dev, 256)
+        _lib.check(L.b200q_lora_plan(ids.data_ptr(), T, n_adapters, data.data_ptr(), nbytes, ws.data_ptr(),
+                                     _stream_ptr(dev)))
+    return LoraPlan(data, T, n_adapters)
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _lora_run(x, base, A, B, scaling, plan, transposed, out, want_out=True):
+    """(y or dx, lo or dlo) of one lora_apply call on contiguous, aligned tensors."""
+    T = x.shape[0]
+    n_adapters, D, r = A.shape
+    N = B.shape[2]
+    dev = x.device
+    L = _lib.lib()
+    mid = torch.empty((L.b200q_lora_mid_bytes(T, r) // 4,), dtype=torch.float32, device=dev)
+    if out is None and want_out:
+        out = torch.empty((T, D if transposed else N), dtype=x.dtype, device=dev)
+    with _device(dev):
+        _lib.check(L.b200q_lora_apply(x.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling),
+                                      plan.data_ptr(), T, D, N, r, n_adapters, _dtype_code(x.dtype), transposed,
+                                      _ptr(out), mid.data_ptr(), _stream_ptr(dev)))
+    return out, mid
+
+
+class _LoraApply(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, base, x, A, B, scaling, plan):
+        base, x, A, B = _aligned(base), _aligned(x), _aligned(A), _aligned(B)
+        y, lo = _lora_run(x, base, A, B, scaling, plan, 0, None)
+        ctx.save_for_backward(x, A, B, scaling, plan, lo)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, A, B, scaling, plan, lo = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        d = _aligned(dy)
+        dx = dlo = dA = dB = None
+        if need[1] or need[2]:
+            dx, dlo = _lora_run(d, None, A, B, scaling, plan, 1, None, want_out=need[1])
+        if need[2] or need[3]:
+            dA = torch.empty_like(A) if need[2] else None
+            dB = torch.empty_like(B) if need[3] else None
+            n_adapters, D, r = A.shape
+            with _device(x.device):
+                _lib.check(_lib.lib().b200q_lora_grads(x.data_ptr(), d.data_ptr(), lo.data_ptr(), _ptr(dlo),
+                                                       plan.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters,
+                                                       _dtype_code(x.dtype), _ptr(dA), _ptr(dB),
+                                                       _stream_ptr(x.device)))
+        return dy if need[0] else None, dx, dA, dB, None, None
+
+
+def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
+               plan: Union[LoraPlan, torch.Tensor], scaling: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[t] = base[t] + scaling[id_t] * (x[t] . A[id_t]) . B[id_t]: the adapters
+    of many requests beside one shared projection's output ``base``.
+
+    base [T, N] and x [T, D] fp16 / bf16, A [L, D, r], B [L, r, N] (r <= 64),
+    plan: lora_plan's result, or the ids [T] themselves (-1 = no adapter: y =
+    base), scaling [L] or None (1).  The row between the two products stays in
+    fp32; y is rounded once.  Differentiable in base, x, A and B (scaling is a
+    constant).  ``out`` (which may be ``base``: in place) takes the result
+    where no gradient is wanted."""
+    if not x.is_cuda:
+        raise RuntimeError("b200q lora_apply runs on CUDA tensors only")
+    if x.dim() != 2 or base.dim() != 2 or A.dim() != 3 or B.dim() != 3:
+        raise ValueError("lora_apply: base [T, N], x [T, D], A [L, D, r] and B [L, r, N] expected")
+    T, D = x.shape
+    n_adapters, _, r = A.shape
+    N = B.shape[2]
+    if base.shape[0] != T or base.shape[1] != N or A.shape[1] != D or B.shape[0] != n_adapters or B.shape[1] != r:
+        raise ValueError(f"lora_apply: shapes do not fit: base {tuple(base.shape)}, x {tuple(x.shape)}, "
+                         f"A {tuple(A.shape)}, B {tuple(B.shape)}")
+    dt = x.dtype
+    _dtype_code(dt)
+    if base.dtype != dt:
+        raise TypeError(f"lora_apply: base is {base.dtype}, x is {dt}")
+    if isinstance(plan, torch.Tensor):
+        plan = lora_plan(plan, n_adapters)
+    if plan.tokens != T or plan.adapters != n_adapters:
+        raise ValueError(f"lora_apply: the plan is for {plan.tokens} tokens and {plan.adapters} adapters, "
+                         f"not {T} and {n_adapters}")
+    _same_device("lora_apply", x, base, A, B, plan.data, scaling, out)
+    if scaling is not None:
+        if scaling.shape != (n_adapters,):
+            raise ValueError(f"lora_apply: scaling must be [{n_adapters}]")
+        if scaling.requires_grad:
+            raise ValueError("lora_apply: scaling is a constant and has no gradient")
+        scaling = scaling.to(torch.float32).contiguous()
+    if A.dtype != dt:
+        A = A.to(dt)
+    if B.dtype != dt:
+        B = B.to(dt)
+    if torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad or base.requires_grad):
+        if out is not None:
+            raise ValueError("lora_apply: out cannot be given where a gradient is wanted")
+        return _LoraApply.apply(base, x, A, B, scaling, plan.data)
+    in_place = out is base
+    if out is not None and (out.shape != base.shape or out.dtype != dt or not out.is_contiguous()
+                            or out.data_ptr() % 16):
+        raise ValueError("lora_apply: out must be a contiguous, 16-byte aligned [T, N] tensor of x's dtype")
+    base = out if in_place else _aligned(base)
+    return _lora_run(_aligned(x), base, _aligned(A), _aligned(B), scaling, plan.data, 0, out)[0]
 
 
 def moe_gather(x: torch.Tensor, slot_token: torch.Tensor) -> torch.Tensor:
