@@ -276,7 +276,7 @@ int b200q_lora_plan(const int64_t* lora_ids, int64_t T, int64_t L, int32_t* plan
  * y is dx [T, D]).  base: NULL for zeros; may be y itself; a token without an
  * adapter gets base.  y: NULL to compute mid alone.  mid: lo (or dlo), fp32,
  * b200q_lora_mid_bytes(T, r) of it, any contents; rows of tokens without an
- * adapter are left as they were. */
+ * adapter are left as they were; NULL is enough for y alone at T <= 256. */
 size_t b200q_lora_mid_bytes(int64_t T, int64_t r);
 int b200q_lora_apply(const void* x, const void* base, const void* A, const void* B, const float* scaling,
                      const int32_t* plan, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype,

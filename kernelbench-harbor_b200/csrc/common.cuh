@@ -89,6 +89,11 @@ int num_sms(int device);
 // before the programmatic-dependent-launch wait
 bool weight_prefetch_enabled();
 int current_device();
+// cudaFuncSetAttribute(MaxDynamicSharedMemorySize), once per kernel and device
+// (`kernel` identifies the instantiation: its host-side function pointer)
+int allow_smem(const void* kernel, int bytes, const char* what);
+// Clusters of `size` CTAs that fit on the current device at once (looked up once per kernel, size and device)
+int resident_clusters(const void* kernel, int threads, int smem, int size);
 
 // encodes a 2D tiled tensor map; returns 0 or a negative b200q status
 int encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner,
@@ -361,6 +366,11 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t b
 __device__ __forceinline__ void named_barrier_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+
+// Programmatic dependent launch: lets the next kernel of the stream start, and
+// waits for the previous one's memory (no effect without the launch attribute).
+__device__ __forceinline__ void pdl_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t elect_one_sync() {
   uint32_t pred = 0;

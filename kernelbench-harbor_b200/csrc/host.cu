@@ -2,8 +2,10 @@
 // properties, tensor-map encoding through the driver entry point, the device
 // status word.
 #include <atomic>
+#include <map>
 #include <mutex>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "common.cuh"
@@ -45,6 +47,45 @@ int num_sms(int device) {
     cache[device] = n;
   }
   return cache[device];
+}
+
+int allow_smem(const void* kernel, int bytes, const char* what) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, int> done;  // largest size set so far
+  const std::pair<const void*, int> key(kernel, current_device());
+  std::lock_guard<std::mutex> lk(mu);
+  auto it = done.find(key);
+  if (it != done.end() && it->second >= bytes) return B200Q_OK;
+  const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+  if (rc == B200Q_OK) done[key] = bytes;
+  return rc;
+}
+
+int resident_clusters(const void* kernel, int threads, int smem, int size) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, int, int>, int> known;
+  const auto key = std::make_tuple(kernel, smem, size, current_device());
+  std::lock_guard<std::mutex> lk(mu);
+  auto it = known.find(key);
+  if (it != known.end()) return it->second;
+  cudaLaunchConfig_t q = {};
+  q.gridDim = dim3((unsigned)size);
+  q.blockDim = dim3((unsigned)threads);
+  q.dynamicSmemBytes = (size_t)smem;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = (unsigned)size;
+  a[0].val.clusterDim.y = 1;
+  a[0].val.clusterDim.z = 1;
+  q.attrs = a;
+  q.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &q) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = 1;
+  }
+  known[key] = n;
+  return n;
 }
 
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

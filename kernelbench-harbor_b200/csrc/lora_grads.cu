@@ -5,12 +5,13 @@
 //
 // Both are one product, thin^T . wide over the tokens, so one launch does both:
 // a CTA owns CT columns of x or of dy, one adapter and 1/S of its tokens, and
-// steps through them 32 at a time: the wide rows by asynchronous copies into a
-// ring, the thin rows through registers, split into two halves of the type
-// (fp16: scaled by a power of two that follows the largest value seen, the sums
-// with it).  Each wide value is read once from HBM and once from shared memory.  The S parts of a token range are a cluster;
-// their sums meet in rank order in distributed shared memory: deterministic.
-// Bound: HBM, x and dy once; at r = 64 the legacy tensor rate is close (two
+// steps through them TK at a time: the wide rows by asynchronous copies into a
+// ring of GSTG stages, the thin rows through registers, split into two halves
+// of the type one stage ahead (fp16: scaled by a power of two that follows the
+// largest value seen, the sums with it).  A warp takes 32 columns and one half
+// of the stage's tokens.  The two halves, and the S parts of a token range,
+// which form a cluster, are added in a fixed order: deterministic.
+// Bound: HBM, x and dy once; at r = 64 the legacy tensor rate is as near (two
 // halves: 4 T r (D + N) flop).
 #include <type_traits>
 
@@ -20,19 +21,20 @@ namespace b200q {
 namespace lora {
 
 constexpr int CT = 128;  // columns of a CTA
-constexpr int TK = 32;   // tokens of a stage
+constexpr int TK = 64;   // tokens of a stage
 constexpr int GSTG = 4;  // stages of the wide rows
 constexpr int WPITCH = CT * 2 + 16;
 constexpr int OPITCH = CT + 1;
+constexpr int TOKS = 8;  // stages of token indices kept (a power of two > GSTG + 1)
 
 template <int RP>
 struct GradCfg {
   static constexpr int TPITCH = RP * 2 + 16;
   static constexpr int WIDE = GSTG * TK * WPITCH;
-  static constexpr int THIN = TK * TPITCH;  // one half of one stage
+  static constexpr int THIN = TK * TPITCH;  // one half of one stage; two stages are kept
   static constexpr int OUT = RP * OPITCH * 4;
-  static constexpr int SMEM = WIDE + 2 * THIN > OUT ? WIDE + 2 * THIN : OUT;
-  static constexpr int VPT = TK * RP / 4 / THREADS > 0 ? TK * RP / 4 / THREADS : 1;  // float4 of the thin rows per thread
+  static constexpr int SMEM = WIDE + 4 * THIN > OUT ? WIDE + 4 * THIN : OUT;
+  static constexpr int VPT = TK * RP / 4 / THREADS;  // float4 of the thin rows per thread
 };
 
 struct GradArgs {
@@ -45,11 +47,12 @@ struct GradArgs {
 };
 
 template <class T, int RP, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2) lora_grads_kernel(const GradArgs a, int S) {
+__global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_grads_kernel(const GradArgs a, int S) {
   using C = GradCfg<RP>;
   constexpr bool F16 = std::is_same<T, __half>::value;
-  extern __shared__ __align__(16) uint8_t sm[];
-  __shared__ unsigned s_max[2];
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ int s_tok[TOKS][TK];
+  __shared__ unsigned s_max[4];
   const bool da = (int)blockIdx.x < a.nbd;  // columns of x (dA) or of dy (dB)
   const T* wide = reinterpret_cast<const T*>(da ? a.x : a.dy);
   const float* thin = da ? a.dlo : a.lo;
@@ -59,144 +62,166 @@ __global__ void __launch_bounds__(THREADS, 2) lora_grads_kernel(const GradArgs a
   const int b0 = a.plan[a.lay.seg + seg], b1 = a.plan[a.lay.seg + seg + 1];
   const int nst_all = (b1 - b0 + TK - 1) / TK;
   // whole stages per rank
-  const int f0 = b0 + rank * nst_all / S * TK, f1 = min(b1, b0 + (rank + 1) * nst_all / S * TK);
+  const int f0 = b0 + (int)((int64_t)rank * nst_all / S) * TK;
+  const int f1 = min(b1, b0 + (int)((int64_t)(rank + 1) * nst_all / S) * TK);
   const int nst = (f1 - f0 + TK - 1) / TK;
   const int32_t* order = a.plan + a.lay.order;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int cg = warp & 3, half = warp >> 2;
 
-  // token of this thread's wide pieces (rows tid / 16 and 16 + tid / 16) and thin values, one stage ahead of their use
-  auto token = [&](int st, int row) { return f0 + st * TK + row < f1 ? order[f0 + st * TK + row] : -1; };
-  int wt[2];
-  auto tokens_of = [&](int st) {
-    wt[0] = token(st, tid >> 4);
-    wt[1] = token(st, 16 + (tid >> 4));
+  auto load_tokens = [&](int st) {  // threads 0 .. TK - 1
+    const int i = f0 + st * TK + tid;
+    s_tok[st % TOKS][tid] = i < f1 ? order[i] : -1;
   };
   auto stage_wide = [&](int st) {
     uint8_t* buf = sm + st % GSTG * TK * WPITCH;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      stage8<T, VEC>(buf + (16 * i + (tid >> 4)) * WPITCH + (tid & 15) * 16, wide + (size_t)max(wt[i], 0) * W,
-                     w0 + (tid & 15) * 8, W, wt[i] >= 0, wide);
+    for (int i = 0; i < TK / 16; ++i) {
+      const int row = 16 * i + (tid >> 4), tok = s_tok[st % TOKS][row];
+      stage8<T, VEC>(buf + row * WPITCH + (tid & 15) * 16, wide + (size_t)max(tok, 0) * W, w0 + (tid & 15) * 8, W,
+                     tok >= 0, wide);
+    }
   };
   float4 tv[C::VPT];
   auto load_thin = [&](int st) {
 #pragma unroll
     for (int i = 0; i < C::VPT; ++i) {
       const int idx = tid + i * THREADS, row = idx / (RP / 4), col = idx % (RP / 4) * 4;
-      tv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < TK && (VEC || col < a.mp)) {
-        const int tok = token(st, row);
-        if (tok >= 0) tv[i] = *reinterpret_cast<const float4*>(thin + (size_t)tok * a.mp + col);
-      }
+      const int tok = s_tok[st % TOKS][row];
+      tv[i] = tok >= 0 && (VEC || col < a.mp) ? *reinterpret_cast<const float4*>(thin + (size_t)tok * a.mp + col)
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
-  float acc[RP / 16][2][4] = {};
-  float fac = 1.f, inv = 1.f;  // fp16: acc holds the sums times inv = 1 / fac
+  auto note_max = [&](int st) {  // fp16: the largest exponent of the finite values in tv
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < C::VPT; ++i) {
+      const float f[4] = {tv[i].x, tv[i].y, tv[i].z, tv[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned x = (__float_as_uint(f[e]) >> 23) & 0xffu;
+        if (x != 255) m = max(m, x);
+      }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) atomicMax(&s_max[st & 3], m);
+  };
+  float acc[RP / 16][4][4] = {};
+  float fac = 1.f, inv = 1.f;  // fp16: sums and thin rows carry inv = 1 / fac
   unsigned emax = 0;
-  uint8_t* thin_hi = sm + C::WIDE;
-  uint8_t* thin_lo = thin_hi + C::THIN;
-  if (F16 && tid < 2) s_max[tid] = 0;
-
-  if (nst > 0) {
-    load_thin(0);
-#pragma unroll
-    for (int i = 0; i < GSTG - 1; ++i) {
-      if (i < nst) {
-        tokens_of(i);
-        stage_wide(i);
-      }
-      cp_async_commit();
-    }
-    if (GSTG - 1 < nst) tokens_of(GSTG - 1);
-  }
-  if (F16) __syncthreads();
-  for (int st = 0; st < nst; ++st) {
+  // splits tv into stage st's buffer; returns what the sums have to be multiplied by before they take that stage
+  auto put_thin = [&](int st) {
+    float scale = 1.f;
     if (F16) {
-      // largest exponent of the stage's finite values
-      unsigned m = 0;
-#pragma unroll
-      for (int i = 0; i < C::VPT; ++i) {
-        const float f[4] = {tv[i].x, tv[i].y, tv[i].z, tv[i].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned x = (__float_as_uint(f[e]) >> 23) & 0xffu;
-          if (x != 255) m = max(m, x);
-        }
-      }
-      m = __reduce_max_sync(0xffffffffu, m);
-      if (lane == 0) atomicMax(&s_max[st & 1], m);
-    }
-    cp_async_wait<GSTG - 2>();
-    __syncthreads();  // stage st has landed; everyone is done with stage st - 1's slots
-    if (F16) {
-      const unsigned m = s_max[st & 1];
-      if (tid == 0) s_max[(st + 1) & 1] = 0;  // used next after the barrier below
+      const unsigned m = s_max[st & 3];
       if (m > emax) {
         float nf, ni;
         pow2_of(__uint_as_float(m << 23), nf, ni);
-        const float scale = fac * ni;  // both powers of two
-#pragma unroll
-        for (int i = 0; i < RP / 16; ++i)
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              acc[i][p][e] *= scale;
+        scale = fac * ni;  // both powers of two
         fac = nf;
         inv = ni;
         emax = m;
       }
     }
+    uint8_t* hi_ = sm + C::WIDE + (st & 1) * 2 * C::THIN;
+    uint8_t* lo_ = hi_ + C::THIN;
 #pragma unroll
     for (int i = 0; i < C::VPT; ++i) {
       const int idx = tid + i * THREADS, row = idx / (RP / 4), col = idx % (RP / 4) * 4;
-      if (row < TK) {
-        T hi[4], lo[4];
-        split(tv[i].x * inv, hi[0], lo[0]);
-        split(tv[i].y * inv, hi[1], lo[1]);
-        split(tv[i].z * inv, hi[2], lo[2]);
-        split(tv[i].w * inv, hi[3], lo[3]);
-        *reinterpret_cast<uint2*>(thin_hi + row * C::TPITCH + col * 2) = make_uint2(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]));
-        *reinterpret_cast<uint2*>(thin_lo + row * C::TPITCH + col * 2) = make_uint2(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]));
-      }
+      T hi[4], lo[4];
+      split(tv[i].x * inv, hi[0], lo[0]);
+      split(tv[i].y * inv, hi[1], lo[1]);
+      split(tv[i].z * inv, hi[2], lo[2]);
+      split(tv[i].w * inv, hi[3], lo[3]);
+      *reinterpret_cast<uint2*>(hi_ + row * C::TPITCH + col * 2) = make_uint2(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]));
+      *reinterpret_cast<uint2*>(lo_ + row * C::TPITCH + col * 2) = make_uint2(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]));
     }
+    return scale;
+  };
+
+  if (tid < 4) s_max[tid] = 0;
+  if (tid < TK) {
+    for (int i = 0; i < GSTG + 1; ++i) load_tokens(i);
+  }
+  __syncthreads();
+  float rescale = 1.f;
+  if (nst > 0) {
+    load_thin(0);
+#pragma unroll
+    for (int i = 0; i < GSTG - 1; ++i) {
+      if (i < nst) stage_wide(i);
+      cp_async_commit();
+    }
+    if (F16) {
+      note_max(0);
+      __syncthreads();
+    }
+    put_thin(0);
+    load_thin(1);
+    if (F16) note_max(1);
+  }
+  for (int st = 0; st < nst; ++st) {
+    cp_async_wait<GSTG - 2>();
+    __syncthreads();  // stage st's wide and thin rows are in place; everyone is done with stage st - 1
+    rescale = 1.f;
+    if (st + 1 < nst) rescale = put_thin(st + 1);
+    if (F16 && tid == 0) s_max[(st + 3) & 3] = 0;  // next used by note_max(st + 3), a barrier from here
     if (st + GSTG - 1 < nst) stage_wide(st + GSTG - 1);
     cp_async_commit();
-    __syncthreads();  // thin rows are in place
-    if (st + GSTG < nst) tokens_of(st + GSTG);
-    if (st + 1 < nst) load_thin(st + 1);
-    // A: thin^T (rank rows), B: wide (this warp's 16 columns), k: tokens
-    const uint32_t wb = smem_u32(sm + st % GSTG * TK * WPITCH) + (8 * ((lane >> 3) & 1) + (lane & 7)) * WPITCH +
-                        (warp * 16 + 8 * (lane >> 4)) * 2;
-    const uint32_t ta = (8 * (lane >> 4) + (lane & 7)) * C::TPITCH + 16 * ((lane >> 3) & 1);
-    const uint32_t th = smem_u32(thin_hi) + ta, tl = smem_u32(thin_lo) + ta;
+    if (st + 2 < nst) load_thin(st + 2);
+    if (tid < TK) load_tokens(st + GSTG + 1);
+    // A: thin^T (rank rows), B: wide (this warp's 32 columns), k: this warp's half of the tokens
+    const uint32_t wb = smem_u32(sm + st % GSTG * TK * WPITCH) + (32 * half + 8 * ((lane >> 3) & 1) + (lane & 7)) * WPITCH +
+                        (cg * 32 + 8 * (lane >> 4)) * 2;
+    const uint32_t th = smem_u32(sm + C::WIDE + (st & 1) * 2 * C::THIN) +
+                        (32 * half + 8 * (lane >> 4) + (lane & 7)) * C::TPITCH + 16 * ((lane >> 3) & 1);
 #pragma unroll
-    for (int k = 0; k < TK / 16; ++k) {
-      uint32_t b[4];
+    for (int k = 0; k < 2; ++k) {
+      uint32_t b[8];
       ldmatrix_x4_trans(b, wb + k * 16 * WPITCH);
+      ldmatrix_x4_trans(b + 4, wb + k * 16 * WPITCH + 32);
 #pragma unroll
       for (int i = 0; i < RP / 16; ++i) {
         uint32_t h[4], l[4];
         ldmatrix_x4_trans(h, th + k * 16 * C::TPITCH + i * 32);
-        ldmatrix_x4_trans(l, tl + k * 16 * C::TPITCH + i * 32);
+        ldmatrix_x4_trans(l, th + C::THIN + k * 16 * C::TPITCH + i * 32);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
+        for (int p = 0; p < 4; ++p) {
           mma16816<T>(acc[i][p], h[0], h[1], h[2], h[3], b[2 * p], b[2 * p + 1]);
           mma16816<T>(acc[i][p], l[0], l[1], l[2], l[3], b[2 * p], b[2 * p + 1]);
         }
       }
+    }
+    if (F16) {
+      if (rescale != 1.f) {
+#pragma unroll
+        for (int i = 0; i < RP / 16; ++i)
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][p][e] *= rescale;
+      }
+      if (st + 2 < nst) note_max(st + 2);
     }
   }
   cp_async_wait<0>();
   __syncthreads();
   float* out = reinterpret_cast<float*>(sm);
 #pragma unroll
-  for (int i = 0; i < RP / 16; ++i)
+  for (int h = 1; h >= 0; --h) {
+    if (half == h) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
+      for (int i = 0; i < RP / 16; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        out[(16 * i + g + 8 * (e >> 1)) * OPITCH + warp * 16 + 8 * p + 2 * t + (e & 1)] = acc[i][p][e] * fac;
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float* o = out + (16 * i + g + 8 * (e >> 1)) * OPITCH + cg * 32 + 8 * p + 2 * t + (e & 1);
+            *o = acc[i][p][e] * fac + (h == 0 ? *o : 0.f);
+          }
+    }
+    if (h) __syncthreads();
+  }
   if (S > 1)
     cluster_sync();
   else
@@ -245,12 +270,18 @@ int launch_grads(const void* x, const void* dy, const float* lo, const float* dl
     constexpr bool VEC = decltype(vc)::value;
     auto kern = lora_grads_kernel<T, RP, VEC>;
     constexpr int smem = GradCfg<RP>::SMEM;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(lora grads)");
-    // split the tokens while the grid does not fill the SMs twice over and a part keeps two stages or more
-    const int64_t blocks = (int64_t)(a.nbd + nbn) * L;
+    const int rc2 = allow_smem((const void*)kern, smem, "cudaFuncSetAttribute(lora grads)");
+    if (rc2) return rc2;
+    // the split of the tokens with the shortest estimate, for adapters of equal
+    // shares: rounds of co-resident clusters x (stages of a part + 5)
+    const int64_t blocks = (int64_t)(a.nbd + nbn) * L, nst = (T_ + TK * L - 1) / (TK * L);
     int S = 1;
-    while (S < 8 && blocks * S < 2 * num_sms(-1) && T_ >= 4 * TK * S) S *= 2;
+    int64_t best = INT64_MAX;
+    for (int s = 1; s <= 8 && (s == 1 || T_ >= 4 * TK * s); s *= 2) {
+      const int64_t fit = resident_clusters((const void*)kern, THREADS, smem, s);
+      const int64_t cost = ((blocks + fit - 1) / fit) * ((nst + s - 1) / s + 5);
+      if (cost < best) best = cost, S = s;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.nbd + nbn), (unsigned)L, (unsigned)S);
     cfg.blockDim = dim3(THREADS);

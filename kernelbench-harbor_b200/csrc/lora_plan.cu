@@ -169,8 +169,7 @@ int b200q_lora_plan(const int64_t* lora_ids, int64_t T, int64_t L, int32_t* plan
   if (misaligned({plan})) return fail(B200Q_ERR_ALIGN, "lora_plan: plan must be 16-byte aligned");
   const int smem = (int)((PLAN_WARPS * (L + 1) + 3 * (L + 2)) * 4);
   if (smem > 48 * 1024) {
-    const int rc = check_cuda(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                              "cudaFuncSetAttribute(lora plan)");
+    const int rc = allow_smem((const void*)plan_kernel, smem, "cudaFuncSetAttribute(lora plan)");
     if (rc) return rc;
   }
   plan_kernel<<<1, PLAN_THREADS, smem, reinterpret_cast<cudaStream_t>(stream)>>>(
@@ -191,7 +190,7 @@ int b200q_lora_apply(const void* x, const void* base, const void* A, const void*
   int rc = check_sizes("lora_apply", T, D, N, r, L, dtype);
   if (rc) return rc;
   if (T == 0) return B200Q_OK;
-  if (!x || !A || !B || !plan || !mid) return fail(B200Q_ERR_SHAPE, "lora_apply: null pointer argument");
+  if (!x || !A || !B || !plan || (!y && !mid) || (!mid && T > SMALL_MAX_T)) return fail(B200Q_ERR_SHAPE, "lora_apply: null pointer argument");
   if (misaligned({x, base, A, B, plan, y, mid})) return fail(B200Q_ERR_ALIGN, "lora_apply: pointers must be 16-byte aligned");
   Args a;
   a.x = x;

@@ -203,6 +203,15 @@ __device__ __forceinline__ void stage8(void* dst, const T* row, int k, int K, bo
     *reinterpret_cast<uint4*>(dst) = in ? ld8<T, false>(row, k, K) : make_uint4(0, 0, 0, 0);
 }
 
+// The same from a pointer to the piece itself; `left`: values of the row from there on.
+template <class T, bool VEC>
+__device__ __forceinline__ void stage16(void* dst, const T* piece, int left, bool in, const T* any) {
+  if constexpr (VEC)
+    cp_async16(smem_u32(dst), in && left > 0 ? piece : any, in && left > 0);
+  else
+    *reinterpret_cast<uint4*>(dst) = in ? ld8<T, false>(piece, 0, left) : make_uint4(0, 0, 0, 0);
+}
+
 // base + fac * c for the 8 consecutive columns of one row: c[p][h], c[p][h + 1] are columns 2p, 2p + 1
 template <class T>
 __device__ __forceinline__ uint4 add8(const uint4 b, const float (*c)[4], int h, float fac) {

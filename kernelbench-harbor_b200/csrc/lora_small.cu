@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(THREADS) lora_small_kernel(const Args a) {
     v[e] = mcol + e < r ? v[e] * scale : 0.f;  // past the rank: an exact 0, whatever x holds
     if (fabsf(v[e]) < INFINITY) mx = fmaxf(mx, fabsf(v[e]));
   }
-  if (rank == 0 && mrow < count) {
+  if (a.mid && rank == 0 && mrow < count) {
     float* mid = a.mid + (size_t)rows[mrow] * a.mp;
 #pragma unroll
     for (int e = 0; e < EPT; ++e)
@@ -289,8 +289,8 @@ int launch_small(const Args& a, int dtype, bool tr, cudaStream_t st) {
     constexpr bool VEC = decltype(vc)::value;
     auto kern = tr ? lora_small_kernel<T, RP, true, VEC> : lora_small_kernel<T, RP, false, VEC>;
     constexpr int smem = SmallCfg<RP>::SMEM;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(lora small)");
+    const int rc2 = allow_smem((const void*)kern, smem, "cudaFuncSetAttribute(lora small)");
+    if (rc2) return rc2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.lay.max_small * CL));
     cfg.blockDim = dim3(THREADS);

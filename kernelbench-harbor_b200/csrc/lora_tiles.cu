@@ -1,14 +1,20 @@
 // Many tokens (prefill, training): shrink and expand as two launches over tiles
-// of up to 128 rows of one adapter.
+// of up to 128 rows of one adapter, both streaming wide rows through a ring of
+// STG stages of 128 rows x 64 columns in shared memory (asynchronous 16-byte
+// copies, 8 lanes to a row's 128 bytes), so that two CTAs keep ~96 KB of HBM
+// reads in flight on each SM.
 //
-// shrink: 8 warps of 16 rows; rows go from HBM straight into the multiply's
-// fragments (two 64-wide stages ahead, in registers), P comes through a
-// 4-stage ring in shared memory that all warps read.  The contraction of a tile
-// is split over a cluster of S CTAs, so that short batches fill the GPU; the
-// partial sums meet through distributed shared memory in rank order.
-// expand: a CTA takes a tile's 128 output columns: mid split into two halves of
-// the type in registers, Q staged once, base requested before anything else.
+// shrink: a warp takes 32 rows and one 32-wide half of every stage (a piece of
+// P then serves two row blocks; at rank 64, where their sums would fill the
+// registers, 16 rows and both halves); the halves and, with the contraction of
+// a tile split over a cluster of S CTAs, the CTAs' sums are added in a fixed
+// order.
+// expand: the stage is base's, beside the 64 columns of Q, whose words are put
+// in the order in which a thread ends with 8 consecutive columns, so that base
+// and y pass as 16-byte pieces.  A warp takes 16 rows; mid is split into two
+// halves of the type once, in registers, and serves all the CTA's columns.
 // Bound: HBM -- x once, base once, y once; mid (4 r bytes a token) stays in L2.
+#include <algorithm>
 #include <type_traits>
 
 #include "lora_seg.cuh"
@@ -16,23 +22,31 @@
 namespace b200q {
 namespace lora {
 
-constexpr int SK = 64;   // contraction depth of a stage
-constexpr int SSTG = 4;  // stages of P in shared memory
+constexpr int SK = 64;  // columns of a stage
+constexpr int STG = 4;
+constexpr int ROWB = SK * 2;               // bytes of a stage's wide row; 16-byte pieces are XOR-swizzled by the row
+constexpr int WIDE = ROWS_L * ROWB;        // bytes of a stage's wide rows
 constexpr int MAX_SPLIT = 8;
-constexpr int NC = 128;  // output columns of an expand CTA
 
+// Swizzle of a row's 16-byte pieces: 8 rows x 1 piece (a fragment's words) and
+// 2 rows x 4 pieces (a quarter warp's 16-byte loads) both meet all banks once.
+__device__ __forceinline__ int swz(int row) { return ((row & 1) << 2) | ((row >> 1) & 3); }
+
+// The 64 contraction rows of P / the rank rows of Q lie RP or 64 values wide.
 template <int RP, bool TR>
 struct ShrinkCfg {
-  static constexpr int PITCH = RP * 2 + 16;                              // !TR: bytes per contraction row
-  static constexpr int STAGE = TR ? RP * SK * 2 : SK * PITCH;            // TR: rank rows of 64 values
-  static constexpr int PART = ROWS_L * (RP + 4) * 4;                     // partial sums, over the ring
-  static constexpr int SMEM = SSTG * STAGE > PART ? SSTG * STAGE : PART;
+  static constexpr int PITCH = RP * 2 + 16;                    // !TR: bytes per contraction row
+  static constexpr int THIN = TR ? RP * ROWB : SK * PITCH;     // TR: rank rows of 64 values
+  static constexpr int STAGE = WIDE + THIN;
+  static constexpr int PP = RP + 4;                            // floats per row of the partial sums, over the ring
+  static constexpr int PART = ROWS_L * PP * 4;
+  static constexpr int SMEM = STG * STAGE > PART ? STG * STAGE : PART;
 };
 
 template <class T, int RP, bool TR, bool VEC>
 __global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_shrink_tile_kernel(const Args a, int S) {
   using C = ShrinkCfg<RP, TR>;
-  extern __shared__ __align__(16) uint8_t sm[];
+  extern __shared__ __align__(128) uint8_t sm[];
   const int tile = blockIdx.x / S, rank = S > 1 ? (int)cluster_ctarank() : 0;
   const int32_t* plan = a.plan;
   if (tile >= plan[1]) return;
@@ -41,188 +55,248 @@ __global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_shrink_tile_kernel(
   const int32_t* rows = plan + a.lay.order + tl.y;
   const int count = tl.z, D = a.D, r = a.r;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int m = warp * 16 + g;
-  const int64_t ra = m < count ? rows[m] : -1, rb = m + 8 < count ? rows[m + 8] : -1;
+  // a warp's rows are 16 NM mg .., its 32-wide parts of a stage half .. half + NH - 1
+  constexpr int NM = RP == 64 ? 1 : 2, NH = RP == 64 ? 2 : 1;
+  const int mg = NM == 1 ? warp : warp & 3, half = NM == 1 ? 0 : warp >> 2;
   const T* x = reinterpret_cast<const T*>(a.x);
   const T* P = reinterpret_cast<const T*>(a.P) + (size_t)tl.x * D * r;
   const int nst = (D + SK - 1) / SK;
   const int s0 = (int)((int64_t)rank * nst / S), s1 = (int)((int64_t)(rank + 1) * nst / S);
 
-  auto stage_p = [&](int st) {
-    uint8_t* buf = sm + (st - s0) % SSTG * C::STAGE;
-    constexpr int PIECES = SK * RP / 8;
+  // this thread's pieces of a stage: 16 bytes of rows tid / 8 + 32 i, and of P; pointers advance by a stage
+  const int pc = tid & 7, prow = tid >> 3;
+  const int active = (count + 31) / 32;  // 32-row blocks that hold rows
+  const T* src[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool in = prow + 32 * i < count;
+    src[i] = in ? x + (size_t)rows[prow + 32 * i] * D + s0 * SK + pc * 8 : nullptr;
+  }
+  constexpr int PIECES = SK * RP / 8, PSTEP = TR ? THREADS / 8 : THREADS / (RP / 8);  // rows of P between a thread's pieces
+  const int q = TR ? tid & 7 : tid % (RP / 8), prk = TR ? tid >> 3 : tid / (RP / 8);
+  const T* psrc = TR ? P + (size_t)prk * D + s0 * SK + q * 8 : P + (size_t)(s0 * SK + prk) * r + q * 8;
+  const uint32_t wdst = prow * ROWB + ((pc ^ swz(prow)) << 4);
+  int kst = s0 * SK, slot_in = 0;  // first column and ring slot of the stage that is requested next
+  auto stage = [&]() {
+    uint8_t* buf = sm + slot_in * C::STAGE;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < active) {
+        stage16<T, VEC>(buf + wdst + 32 * i * ROWB, src[i], D - kst - pc * 8, src[i] != nullptr, x);
+        if (src[i]) src[i] += SK;
+      }
+    uint8_t* thin = buf + WIDE;
 #pragma unroll
     for (int i = 0; i < (PIECES + THREADS - 1) / THREADS; ++i) {
-      const int idx = tid + i * THREADS;
-      if (PIECES % THREADS && idx >= PIECES) break;
-      if (!TR) {
-        const int k = idx / (RP / 8), pc = idx % (RP / 8), kk = st * SK + k;
-        stage8<T, VEC>(buf + row32(k) * C::PITCH + pc * 16, P + (size_t)kk * r, pc * 8, r, kk < D, P);
-      } else {
-        const int n = idx / (SK / 8), pc = idx % (SK / 8);  // odd rows have their 64-byte halves swapped: no bank conflicts
-        stage8<T, VEC>(buf + n * (SK * 2) + ((pc ^ ((n & 1) << 2)) << 4), P + (size_t)n * D, st * SK + pc * 8, D, n < r, P);
-      }
+      const int row = prk + i * PSTEP;
+      if (PIECES % THREADS && row >= (TR ? RP : SK)) break;
+      if constexpr (!TR)
+        stage16<T, VEC>(thin + row32(row) * C::PITCH + q * 16, psrc + (size_t)(i * PSTEP) * r, r - q * 8, kst + row < D, P);
+      else
+        stage16<T, VEC>(thin + row * ROWB + ((q ^ swz(row)) << 4), psrc + (size_t)(i * PSTEP) * D, D - kst - q * 8, row < r, P);
     }
+    psrc += TR ? SK : (size_t)SK * r;
+    kst += SK;
+    slot_in = slot_in + 1 == STG ? 0 : slot_in + 1;
   };
-  auto load_x = [&](int st, uint4* v) {
+  float acc[NM][RP / 8][4] = {};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = st * SK + 32 * h + 8 * t;
-      v[2 * h] = ra >= 0 ? ld8<T, VEC>(x + ra * D, k, D) : make_uint4(0, 0, 0, 0);
-      v[2 * h + 1] = rb >= 0 ? ld8<T, VEC>(x + rb * D, k, D) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  float acc[RP / 8][4] = {};
-  auto multiply = [&](int st, const uint4* v) {
-    const uint8_t* buf = sm + (st - s0) % SSTG * C::STAGE;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 xa = v[2 * h], xb = v[2 * h + 1];
-      const uint32_t row = smem_u32(buf + (32 * h + lane) * C::PITCH);
-#pragma unroll
-      for (int j = 0; j < RP / 8; ++j) {
-        uint32_t b[4];
-        if (!TR) {
-          ldmatrix_x4_trans(b, row + j * 16);
-        } else {
-          const int n = 8 * j + g;
-          const uint4 w = *reinterpret_cast<const uint4*>(buf + n * (SK * 2) + (((4 * h + t) ^ ((n & 1) << 2)) << 4));
-          b[0] = w.x, b[1] = w.y, b[2] = w.z, b[3] = w.w;
-        }
-        mma16816<T>(acc[j], xa.x, xb.x, xa.y, xb.y, b[0], b[1]);
-        mma16816<T>(acc[j], xa.z, xb.z, xa.w, xb.w, b[2], b[3]);
-      }
-    }
-  };
-  uint4 xr[3][4] = {};
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (s0 + i < s1) load_x(s0 + i, xr[i]);
-#pragma unroll
-  for (int i = 0; i < SSTG - 1; ++i) {
-    if (s0 + i < s1) stage_p(s0 + i);
+  for (int i = 0; i < STG - 1; ++i) {
+    if (s0 + i < s1) stage();
     cp_async_commit();
   }
-  for (int st = s0; st < s1; st += 3) {
+  int slot = 0;
+  for (int st = s0; st < s1; ++st) {
+    cp_async_wait<STG - 2>();
+    __syncthreads();  // stage st has landed for every thread; the slot filled next was read before
+    if (st + STG - 1 < s1) stage();
+    cp_async_commit();
+    const uint8_t* buf = sm + slot * C::STAGE;
+    slot = slot + 1 == STG ? 0 : slot + 1;
+    if (16 * NM * mg < count) {
 #pragma unroll
-    for (int u = 0; u < 3; ++u) {
-      const int c = st + u;
-      if (c < s1) {
-        if (c + 2 < s1) load_x(c + 2, xr[(u + 2) % 3]);
-        cp_async_wait<SSTG - 2>();
-        __syncthreads();  // stage c has landed for every thread; the slot filled next was read before
-        if (c + SSTG - 1 < s1) stage_p(c + SSTG - 1);
-        cp_async_commit();
-        multiply(c, xr[u]);
+      for (int h = half; h < half + NH; ++h) {
+        uint4 xv[NM][2];
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            xv[m][e] = *reinterpret_cast<const uint4*>(buf + (16 * (NM * mg + m) + 8 * e + g) * ROWB + (((4 * h + t) ^ swz(g)) << 4));
+        const uint32_t row = smem_u32(buf + WIDE + (32 * h + lane) * C::PITCH);
+#pragma unroll
+        for (int j = 0; j < RP / 8; ++j) {
+          uint32_t b[4];
+          if constexpr (!TR) {
+            ldmatrix_x4_trans(b, row + j * 16);
+          } else {
+            const uint4 w = *reinterpret_cast<const uint4*>(buf + WIDE + (8 * j + g) * ROWB + (((4 * h + t) ^ swz(g)) << 4));
+            b[0] = w.x, b[1] = w.y, b[2] = w.z, b[3] = w.w;
+          }
+#pragma unroll
+          for (int m = 0; m < NM; ++m) {
+            mma16816<T>(acc[m][j], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, b[0], b[1]);
+            mma16816<T>(acc[m][j], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, b[2], b[3]);
+          }
+        }
       }
     }
   }
-  const float scale = a.scaling ? a.scaling[tl.x] : 1.f;
-  if (S == 1) {
-#pragma unroll
-    for (int j = 0; j < RP / 8; ++j) {
-      const int col = 8 * j + 2 * t;
-      if (!VEC && col >= a.mp) break;
-      const bool in0 = col < r, in1 = col + 1 < r;  // past the rank: an exact 0, whatever x holds
-      if (ra >= 0)
-        *reinterpret_cast<float2*>(a.mid + ra * a.mp + col) =
-            make_float2(in0 ? acc[j][0] * scale : 0.f, in1 ? acc[j][1] * scale : 0.f);
-      if (rb >= 0)
-        *reinterpret_cast<float2*>(a.mid + rb * a.mp + col) =
-            make_float2(in0 ? acc[j][2] * scale : 0.f, in1 ? acc[j][3] * scale : 0.f);
-    }
-    return;
-  }
+  pdl_launch_next();
   cp_async_wait<0>();
   __syncthreads();
+  // the two halves of the stages, then the CTAs of the cluster
   float* part = reinterpret_cast<float*>(sm);
-  constexpr int PP = RP + 4;
 #pragma unroll
-  for (int j = 0; j < RP / 8; ++j) {
-    *reinterpret_cast<float2*>(part + m * PP + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
-    *reinterpret_cast<float2*>(part + (m + 8) * PP + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+  for (int h = NM - 1; h >= 0; --h) {
+    if (half == h) {
+#pragma unroll
+      for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float2* p = reinterpret_cast<float2*>(part + (16 * (NM * mg + m) + 8 * e + g) * C::PP + 8 * j + 2 * t);
+            float2 v = make_float2(acc[m][j][2 * e], acc[m][j][2 * e + 1]);
+            if (NM == 2 && h == 0) v.x += p->x, v.y += p->y;
+            *p = v;
+          }
+    }
+    if (h) __syncthreads();
   }
-  cluster_sync();
+  if (S > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  const float scale = a.scaling ? a.scaling[tl.x] : 1.f;
   const int q0 = rank * ROWS_L / S, q1 = min((rank + 1) * ROWS_L / S, count);
   for (int i = tid; i < (q1 - q0) * (RP / 4); i += THREADS) {
     const int row = q0 + i / (RP / 4), col = i % (RP / 4) * 4;
-    const uint32_t addr = smem_u32(part + row * PP + col);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < S; ++c) {
-      float4 u;
-      asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-                   : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w)
-                   : "r"(map_shared_rank(addr, c))
-                   : "memory");
-      s.x += u.x, s.y += u.y, s.z += u.z, s.w += u.w;
+    if (S == 1) {
+      s = *reinterpret_cast<const float4*>(part + row * C::PP + col);
+    } else {
+      const uint32_t addr = smem_u32(part + row * C::PP + col);
+      for (int c = 0; c < S; ++c) {
+        float4 u;
+        asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                     : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w)
+                     : "r"(map_shared_rank(addr, c))
+                     : "memory");
+        s.x += u.x, s.y += u.y, s.z += u.z, s.w += u.w;
+      }
     }
+    // past the rank: an exact 0, whatever x holds
     if (VEC || col < a.mp)
       *reinterpret_cast<float4*>(a.mid + (size_t)rows[row] * a.mp + col) =
           make_float4(col < r ? s.x * scale : 0.f, col + 1 < r ? s.y * scale : 0.f, col + 2 < r ? s.z * scale : 0.f,
                       col + 3 < r ? s.w * scale : 0.f);
   }
-  cluster_sync();  // the others have read this CTA's part
+  if (S > 1) cluster_sync();  // the others have read this CTA's part
 }
 
 template <int RP, bool TR>
 struct ExpandCfg {
-  static constexpr int QWORDS = NC / 2 + 4;                                   // !TR: words per rank row
-  static constexpr int APITCH = RP == 16 ? 32 : RP == 32 ? 96 : 160;          // TR: bytes per column row, 8 words mod 32 (no conflicts)
-  static constexpr int SMEM = TR ? NC * APITCH : RP * QWORDS * 4;
+  // !TR: bytes per rank row of 64 columns; TR: per column row of RP ranks, 8 words mod 32 (no bank conflicts)
+  static constexpr int PITCH = !TR ? ROWB + 16 : RP == 16 ? 32 : RP == 32 ? 96 : 160;
+  static constexpr int THIN = (TR ? SK : RP) * PITCH;
+  static constexpr int STAGE = WIDE + THIN;
+  static constexpr int SMEM = STG * STAGE;
 };
 
+// CTA = (tile, part): `steps` 64-column steps from step part * steps on.
 template <class T, int RP, bool TR, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2) lora_expand_tile_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_expand_tile_kernel(const Args a, int parts, int steps) {
   using C = ExpandCfg<RP, TR>;
-  extern __shared__ __align__(16) uint8_t sm[];
+  extern __shared__ __align__(128) uint8_t sm[];
   const int32_t* plan = a.plan;
-  const int nb = (a.N + NC - 1) / NC, tile = blockIdx.x / nb;  // a tile's column blocks run side by side
-  if (tile >= plan[1]) return;
+  const int tile = blockIdx.x / parts;  // a tile's parts run side by side
+  if (tile >= plan[1]) {
+    pdl_wait_previous();
+    return;
+  }
   const int4 tl = reinterpret_cast<const int4*>(plan + a.lay.large)[tile];
   const int32_t* rows = plan + a.lay.order + tl.y;
-  const int count = tl.z, N = a.N, r = a.r, n0 = blockIdx.x % nb * NC;
+  const int count = tl.z, N = a.N, r = a.r, n0 = blockIdx.x % parts * steps * SK;
+  const int nst = min(steps, (N - n0 + SK - 1) / SK);
   const T* base = reinterpret_cast<const T*>(a.base);
   T* y = reinterpret_cast<T*>(a.y);
   if (tl.x < 0) {
-    copy_rows<T, VEC>(base, y, rows, count, N, n0, min(n0 + NC, N));
+    copy_rows<T, VEC>(base, y, rows, count, N, n0, min(n0 + steps * SK, N));
+    pdl_wait_previous();
     return;
   }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int m = warp * 16 + g;
-  const int64_t ra = m < count ? rows[m] : -1, rb = m + 8 < count ? rows[m + 8] : -1;
-  uint4 bv[NC / 32][2];
-#pragma unroll
-  for (int q = 0; q < NC / 32; ++q) {
-    const int n = n0 + q * 32 + 8 * t;
-    bv[q][0] = base && ra >= 0 ? ld8<T, VEC>(base + ra * N, n, N) : make_uint4(0, 0, 0, 0);
-    bv[q][1] = base && rb >= 0 ? ld8<T, VEC>(base + rb * N, n, N) : make_uint4(0, 0, 0, 0);
-  }
   const T* Q = reinterpret_cast<const T*>(a.Q) + (size_t)tl.x * r * N;
-  if (!TR) {
-    uint32_t* qb = reinterpret_cast<uint32_t*>(sm);
+  const int pc = tid & 7, prow = tid >> 3;
+  const int active = (count + 31) / 32;
+  const T* src[4];
 #pragma unroll
-    for (int i = 0; i < RP * (NC / 8) / THREADS; ++i) {
-      // 8 rank rows in fragment order x 4 lanes of 8 columns, warps over the column groups
-      const int idx = i * WARPS + warp, q = idx % (NC / 32), row = idx / (NC / 32) * 8 + g, k = k_of_row16(row);
-      const uint4 v = k < r ? ld8<T, VEC>(Q + (size_t)k * N, n0 + q * 32 + 8 * t, N) : make_uint4(0, 0, 0, 0);
-      uint32_t* dst = qb + row * C::QWORDS + q * 16 + t;
-      dst[0] = v.x;
-      dst[4] = v.y;
-      dst[8] = v.z;
-      dst[12] = v.w;
-    }
-  } else {
-    constexpr int PIECES = NC * RP / 8;
+  for (int i = 0; i < 4; ++i) {
+    const bool in = base && prow + 32 * i < count;
+    src[i] = in ? base + (size_t)rows[prow + 32 * i] * N + n0 + pc * 8 : nullptr;
+  }
+  constexpr int PIECES = SK * RP / 8, NP = (PIECES + THREADS - 1) / THREADS;
+  constexpr int PSTEP = TR ? THREADS / (RP / 8) : THREADS / 8;  // rows of Q between a thread's pieces
+  const int q = TR ? tid % (RP / 8) : tid & 7, qrow = TR ? tid / (RP / 8) : tid >> 3;
+  const uint32_t wdst = prow * ROWB + ((pc ^ swz(prow)) << 4);
+  int cst = n0, slot_in = 0;
+  // base (and, TR, A's rows) by asynchronous copies
+  auto stage = [&]() {
+    uint8_t* buf = sm + slot_in * C::STAGE;
+    if (base) {
 #pragma unroll
-    for (int i = 0; i < PIECES / THREADS; ++i) {
-      const int idx = tid + i * THREADS, c = idx / (RP / 8), pc = idx % (RP / 8), col = n0 + c;
-      // column 32 q + 8 a + 2 p + b is row 32 q + 8 p + 2 a + b: a fragment's columns together
-      const int row = (c & ~31) | (((c >> 1) & 3) << 3) | (((c >> 3) & 3) << 1) | (c & 1);
-      stage8<T, VEC>(sm + row * C::APITCH + pc * 16, Q + (size_t)col * r, pc * 8, r, col < N, Q);
+      for (int i = 0; i < 4; ++i)
+        if (i < active) {
+          stage16<T, VEC>(buf + wdst + 32 * i * ROWB, src[i], N - cst - pc * 8, src[i] != nullptr, base);
+          if (src[i]) src[i] += SK;
+        }
     }
+    if constexpr (TR) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int c = qrow + i * PSTEP;
+        if (PIECES % THREADS && c >= SK) break;
+        // column 32 w + 8 a + 2 p + b is row 32 w + 8 p + 2 a + b: a fragment's columns together
+        const int row = (c & 32) | (((c >> 1) & 3) << 3) | (((c >> 3) & 3) << 1) | (c & 1);
+        stage16<T, VEC>(buf + WIDE + row * C::PITCH + q * 16, Q + (size_t)(cst + c) * r + q * 8, r - q * 8, cst + c < N, Q);
+      }
+    }
+    cst += SK;
+    slot_in = slot_in + 1 == STG ? 0 : slot_in + 1;
+  };
+  // !TR: Q through registers, since its words change places: word p of the 8
+  // columns of lane t goes to tile p, place t; rank rows in fragment order
+  uint4 qv[TR ? 1 : NP];
+  auto load_q = [&](int st) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int p = qrow + i * PSTEP, k = k_of_row16(p);
+      qv[i] = p < RP && k < r ? ld8<T, VEC>(Q + (size_t)k * N, n0 + st * SK + q * 8, N) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  auto put_q = [&](int slot) {
+    uint32_t* thin = reinterpret_cast<uint32_t*>(sm + slot * C::STAGE + WIDE);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int p = qrow + i * PSTEP;
+      if (PIECES % THREADS && p >= RP) break;
+      uint32_t* dst = thin + p * (C::PITCH / 4) + (q >> 2) * 16 + (q & 3);
+      dst[0] = qv[i].x;
+      dst[4] = qv[i].y;
+      dst[8] = qv[i].z;
+      dst[12] = qv[i].w;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < STG - 1; ++i) {
+    if (i < nst) stage();
     cp_async_commit();
   }
+  if constexpr (!TR) load_q(0);
+  pdl_wait_previous();  // mid comes from the kernel before; all else was there when that one began
   // mid: rows m, m + 8; values 4t .. 4t + 3 of each 16 ranks, split into hi + lo
+  const int m = warp * 16 + g;
+  const int64_t ra = m < count ? rows[m] : -1, rb = m + 8 < count ? rows[m + 8] : -1;
   float fac[2];
   uint2 ha[RP / 16][2], la[RP / 16][2];
 #pragma unroll
@@ -255,36 +329,57 @@ __global__ void __launch_bounds__(THREADS, 2) lora_expand_tile_kernel(const Args
       la[k][h] = make_uint2(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]));
     }
   }
-  if (TR) cp_async_wait<0>();
-  __syncthreads();
+  T* ya = y + (ra >= 0 ? ra : 0) * N + n0 + 8 * t;
+  T* yb = y + (rb >= 0 ? rb : 0) * N + n0 + 8 * t;
+  int slot = 0;
+  for (int st = 0; st < nst; ++st) {
+    if constexpr (!TR) put_q(slot);  // this slot's last readers are two barriers back
+    cp_async_wait<STG - 2>();
+    __syncthreads();
+    if (st + STG - 1 < nst) stage();
+    cp_async_commit();
+    if constexpr (!TR) {
+      if (st + 1 < nst) load_q(st + 1);
+    }
+    const uint8_t* buf = sm + slot * C::STAGE;
+    slot = slot + 1 == STG ? 0 : slot + 1;
+    if (16 * warp < count) {
 #pragma unroll
-  for (int q = 0; q < NC / 32; ++q) {
-    float c[4][4] = {};
+      for (int w = 0; w < 2; ++w) {  // 32 columns each
+        float c[4][4] = {};
 #pragma unroll
-    for (int k = 0; k < RP / 16; ++k) {
-      uint32_t b[8];
-      if (!TR) {
-        const uint32_t addr = smem_u32(reinterpret_cast<uint32_t*>(sm) +
-                                       (16 * k + 8 * ((lane >> 3) & 1) + (lane & 7)) * C::QWORDS + q * 16 + (lane >> 4) * 4);
-        ldmatrix_x4_trans(b, addr);
-        ldmatrix_x4_trans(b + 4, addr + 32);
-      } else {
+        for (int k = 0; k < RP / 16; ++k) {
+          uint32_t b[8];
+          if constexpr (!TR) {
+            const uint32_t addr = smem_u32(buf + WIDE + (16 * k + 8 * ((lane >> 3) & 1) + (lane & 7)) * C::PITCH +
+                                           w * 64 + (lane >> 4) * 16);
+            ldmatrix_x4_trans(b, addr);
+            ldmatrix_x4_trans(b + 4, addr + 32);
+          } else {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const uint2 w = *reinterpret_cast<const uint2*>(sm + (32 * q + 8 * p + g) * C::APITCH + (16 * k + 4 * t) * 2);
-          b[2 * p] = w.x;
-          b[2 * p + 1] = w.y;
+            for (int p = 0; p < 4; ++p) {
+              const uint2 u = *reinterpret_cast<const uint2*>(buf + WIDE + (32 * w + 8 * p + g) * C::PITCH + (16 * k + 4 * t) * 2);
+              b[2 * p] = u.x;
+              b[2 * p + 1] = u.y;
+            }
+          }
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            mma16816<T>(c[p], ha[k][0].x, ha[k][1].x, ha[k][0].y, ha[k][1].y, b[2 * p], b[2 * p + 1]);
+            mma16816<T>(c[p], la[k][0].x, la[k][1].x, la[k][0].y, la[k][1].y, b[2 * p], b[2 * p + 1]);
+          }
         }
-      }
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        mma16816<T>(c[p], ha[k][0].x, ha[k][1].x, ha[k][0].y, ha[k][1].y, b[2 * p], b[2 * p + 1]);
-        mma16816<T>(c[p], la[k][0].x, la[k][1].x, la[k][0].y, la[k][1].y, b[2 * p], b[2 * p + 1]);
+        const int left = N - n0 - st * SK - 32 * w - 8 * t;  // columns of the row from this lane's on
+        uint4 ua = make_uint4(0, 0, 0, 0), ub = ua;
+        if (base) {
+          const uint32_t piece = ((4 * w + t) ^ swz(g)) << 4;
+          ua = *reinterpret_cast<const uint4*>(buf + m * ROWB + piece);
+          ub = *reinterpret_cast<const uint4*>(buf + (m + 8) * ROWB + piece);
+        }
+        if (ra >= 0) st8<T, VEC>(ya + st * SK + 32 * w, 0, left, add8<T>(ua, c, 0, fac[0]));
+        if (rb >= 0) st8<T, VEC>(yb + st * SK + 32 * w, 0, left, add8<T>(ub, c, 2, fac[1]));
       }
     }
-    const int n = n0 + q * 32 + 8 * t;
-    if (ra >= 0) st8<T, VEC>(y + ra * N, n, N, add8<T>(bv[q][0], c, 0, fac[0]));
-    if (rb >= 0) st8<T, VEC>(y + rb * N, n, N, add8<T>(bv[q][1], c, 2, fac[1]));
   }
 }
 
@@ -298,15 +393,29 @@ int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
     auto expand = tr ? lora_expand_tile_kernel<T, RP, true, VEC> : lora_expand_tile_kernel<T, RP, false, VEC>;
     const int smem_s = tr ? ShrinkCfg<RP, true>::SMEM : ShrinkCfg<RP, false>::SMEM;
     const int smem_e = tr ? ExpandCfg<RP, true>::SMEM : ExpandCfg<RP, false>::SMEM;
-    const int64_t blocks = a.lay.max_large * ((a.N + NC - 1) / NC);
-    if (blocks > (1ll << 31) - 1) return fail(B200Q_ERR_SHAPE, "lora_apply: size too large");
-    cudaError_t e = cudaFuncSetAttribute(shrink, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_s);
-    if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(lora shrink)");
-    // the contraction is split until the tiles' clusters fill the SMs twice
-    // over, as long as a part keeps two stages
+    int rc2 = allow_smem((const void*)shrink, smem_s, "cudaFuncSetAttribute(lora shrink)");
+    if (rc2 || (rc2 = allow_smem((const void*)expand, smem_e, "cudaFuncSetAttribute(lora expand)"))) return rc2;
+    // shrink: the split with the shortest estimate, rounds of co-resident
+    // clusters x (stages of a part + 5 for start, joining and ending)
     const int64_t tiles = (a.T + ROWS_L - 1) / ROWS_L, nst = (a.D + SK - 1) / SK;
     int S = 1;
-    while (S < MAX_SPLIT && tiles * S < 2 * num_sms(-1) && nst >= 4 * S) S *= 2;
+    int64_t best = INT64_MAX;
+    for (int s = 1; s <= MAX_SPLIT && (s == 1 || nst >= 4 * s); s *= 2) {
+      const int64_t fit = resident_clusters((const void*)shrink, THREADS, smem_s, s);
+      const int64_t cost = ((tiles + fit - 1) / fit) * ((nst + s - 1) / s + 5);
+      if (cost < best) best = cost, S = s;
+    }
+    // expand: likewise the number of 64-column steps per CTA (start: 2 steps)
+    const int64_t nsteps = (a.N + SK - 1) / SK, slots = resident_clusters((const void*)expand, THREADS, smem_e, 1);
+    int steps = 2;
+    best = INT64_MAX;
+    for (int s = 2; s <= 16; ++s) {
+      const int64_t cost = ((tiles * ((nsteps + s - 1) / s) + slots - 1) / slots) * (s + 2);
+      if (cost < best) best = cost, steps = s;
+    }
+    const int parts = (int)((nsteps + steps - 1) / steps);
+    const int64_t blocks = a.lay.max_large * parts;
+    if (blocks > (1ll << 31) - 1) return fail(B200Q_ERR_SHAPE, "lora_apply: size too large");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.lay.max_large * S));
     cfg.blockDim = dim3(THREADS);
@@ -319,11 +428,15 @@ int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, shrink, a, S);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, shrink, a, S);
     if (e != cudaSuccess) return check_cuda(e, "lora shrink launch");
     if (!a.y) return B200Q_OK;  // mid alone was asked for
-    expand<<<(unsigned)blocks, THREADS, smem_e, st>>>(a);
-    return check_cuda(cudaGetLastError(), "lora expand launch");
+    // the expand kernel's start overlaps the shrink kernel's end
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.dynamicSmemBytes = smem_e;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    return check_cuda(cudaLaunchKernelEx(&cfg, expand, a, parts, steps), "lora expand launch");
   });
 }
 

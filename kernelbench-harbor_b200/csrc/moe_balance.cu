@@ -28,7 +28,8 @@ namespace balance {
 constexpr int THREADS = 256;
 constexpr int MAX_EXPERTS = 256, MAX_K = 8;
 constexpr int64_t SINGLE_ELEMS = 16384;
-constexpr int MAX_BLOCKS = 296;  // two per SM: enough loads in flight, few partials to add
+constexpr int MAX_BLOCKS = 296;  // two per SM: few partials to add
+constexpr int UNROLL = 4;        // rows per lane requested before the first is used
 
 template <class T>
 __device__ __forceinline__ float tf(T v);
@@ -66,6 +67,18 @@ __device__ __forceinline__ void load8(const T* row, int e0, int E, float* v) {
   for (int i = 0; i < 8; ++i) v[i] = !VEC && e0 + i < E ? tf<T>(row[e0 + i]) : -INFINITY;
 }
 
+// The same of row t, -inf where the row is past the batch or masked.
+template <class T, bool VEC>
+__device__ __forceinline__ void load_row(const T* logits, const uint8_t* mask, int64_t t, int64_t T_, int e0, int E,
+                                         float* v) {
+  // both loads at once: what a masked row holds is dropped after it has come
+  const bool in = t < T_, keep = in && (!mask || mask[t]);
+  if (in) load8<T, VEC>(logits + t * E, e0, E, v);
+  if (!keep)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = -INFINITY;
+}
+
 // Softmax of a row over its G lanes, in place (zeros past E); returns whether
 // the row has a logit above -inf.  A NaN anywhere makes the row NaN.
 template <int G>
@@ -99,30 +112,33 @@ __device__ __forceinline__ bool softmax8(float* v) {
 
 // Adds nb blocks' partials in block order and writes loss, counts and coef
 // (coef[e] = E f_e / n, the per-expert factor of the gradient).
+template <int NT>
 __device__ void finish(const float* p_part, const int* c_part, const int* n_part, int nb, int E, int k, float* loss,
                        int32_t* counts, float* coef) {
-  __shared__ float s_p[THREADS], s_loss[THREADS / 32];
-  __shared__ int s_c[THREADS], s_n[THREADS / 32];
+  __shared__ float s_p[NT], s_loss[NT / 32];
+  __shared__ int s_c[NT], s_n[NT / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int n = 0;
-  for (int b = tid; b < nb; b += THREADS) n += n_part[b];
+  for (int b = tid; b < nb; b += NT) n += n_part[b];
   n = __reduce_add_sync(0xffffffffu, n);
   if (lane == 0) s_n[warp] = n;
   // thread (slice, expert): SL slices of the blocks per expert
   const int EP = E <= 8 ? 8 : E <= 16 ? 16 : E <= 32 ? 32 : E <= 64 ? 64 : E <= 128 ? 128 : 256;
-  const int SL = THREADS / EP, e = tid % EP, sl = tid / EP;
+  const int SL = NT / EP, e = tid % EP, sl = tid / EP;
   float p = 0.f;
   int c = 0;
-  if (e < E)
+  if (e < E) {
+#pragma unroll 8
     for (int b = sl * nb / SL; b < (sl + 1) * nb / SL; ++b) {
       p += p_part[(size_t)b * E + e];
       c += c_part[(size_t)b * E + e];
     }
+  }
   s_p[tid] = p;
   s_c[tid] = c;
   __syncthreads();
   n = 0;
-  for (int w = 0; w < THREADS / 32; ++w) n += s_n[w];
+  for (int w = 0; w < NT / 32; ++w) n += s_n[w];
   float term = 0.f;
   if (tid < E) {
     for (int s = 1; s < SL; ++s) {
@@ -141,7 +157,7 @@ __device__ void finish(const float* p_part, const int* c_part, const int* n_part
   __syncthreads();
   if (tid == 0) {
     float t = 0.f;
-    for (int w = 0; w < THREADS / 32; ++w) t += s_loss[w];
+    for (int w = 0; w < NT / 32; ++w) t += s_loss[w];
     *loss = t;
   }
 }
@@ -166,29 +182,32 @@ __global__ void __launch_bounds__(THREADS) partial_kernel(const T* __restrict__ 
   bool bad = false;
   const int64_t step = (int64_t)gridDim.x * (THREADS / 32) * RPW;
   // every lane of a warp makes the same number of steps (shuffles inside)
-  for (int64_t t0 = ((int64_t)blockIdx.x * (THREADS / 32) + warp) * RPW; t0 < T_; t0 += step) {
-    const int64_t t = t0 + gr;
-    const bool in = t < T_ && (!mask || mask[t]);
-    float v[8];
-    if (in)
-      load8<T, VEC>(logits + t * E, e0, E, v);
-    else
+  for (int64_t t0 = ((int64_t)blockIdx.x * (THREADS / 32) + warp) * RPW; t0 < T_; t0 += UNROLL * step) {
+    float v[UNROLL][8];
+    int choice[UNROLL];  // this lane's first choice of each row
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = -INFINITY;
-    const bool live = softmax8<G>(v);
-    if (live) {
+    for (int u = 0; u < UNROLL; ++u) {
+      const int64_t t = t0 + u * step + gr;
+      load_row<T, VEC>(logits, mask, t, T_, e0, E, v[u]);
+      choice[u] = t < T_ && gl < k ? topi[t * k + gl] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      if (!softmax8<G>(v[u])) continue;  // not live; the row's G lanes agree and the shuffles are behind
+      const int64_t t = t0 + u * step + gr;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (e0 + i < E) acc[i] += v[i];
+        if (e0 + i < E) acc[i] += v[u][i];
       n += gl == 0;
       for (int j = gl; j < k; j += G) {
-        const int e = topi[t * k + j];
+        const int e = j == gl ? choice[u] : topi[t * k + j];
         if (e >= 0 && e < E)
           atomicAdd(&s_c[e], 1);
         else if (e != -1)
           bad = true;
       }
     }
+    __syncwarp();
   }
   if (bad && status) atomicOr(status, B200Q_DEV_ERR_BOUNDS);
   n = __reduce_add_sync(0xffffffffu, n);
@@ -207,16 +226,20 @@ __global__ void __launch_bounds__(THREADS) partial_kernel(const T* __restrict__ 
     c_part[(size_t)blockIdx.x * E + e] = s_c[e];
   }
   if (tid == 0) n_part[blockIdx.x] = s_n;
+  pdl_launch_next();
   if (gridDim.x == 1) {
     __syncthreads();  // the block's own global writes are visible to all its threads
-    finish(p_part, c_part, n_part, 1, E, k, loss, counts, coef);
+    finish<THREADS>(p_part, c_part, n_part, 1, E, k, loss, counts, coef);
   }
 }
 
-__global__ void __launch_bounds__(THREADS) finish_kernel(const float* p_part, const int* c_part, const int* n_part,
+constexpr int FINISH_THREADS = 1024;
+
+__global__ void __launch_bounds__(FINISH_THREADS) finish_kernel(const float* p_part, const int* c_part, const int* n_part,
                                                          int nb, int E, int k, float* loss, int32_t* counts,
                                                          float* coef) {
-  finish(p_part, c_part, n_part, nb, E, k, loss, counts, coef);
+  pdl_wait_previous();
+  finish<FINISH_THREADS>(p_part, c_part, n_part, nb, E, k, loss, counts, coef);
 }
 
 template <class T, int G, bool VEC>
@@ -234,13 +257,8 @@ __global__ void __launch_bounds__(THREADS) grad_kernel(const T* __restrict__ log
   const int64_t step = (int64_t)gridDim.x * (THREADS / 32) * RPW;
   for (int64_t t0 = ((int64_t)blockIdx.x * (THREADS / 32) + warp) * RPW; t0 < T_; t0 += step) {
     const int64_t t = t0 + gr;
-    const bool in = t < T_ && (!mask || mask[t]);
     float v[8];
-    if (in)
-      load8<T, VEC>(logits + t * E, e0, E, v);
-    else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = -INFINITY;
+    load_row<T, VEC>(logits, mask, t, T_, e0, E, v);
     const bool live = softmax8<G>(v);
     float dot = 0.f;
 #pragma unroll
@@ -318,7 +336,18 @@ void launch_forward(const void* logits, const int32_t* topi, const uint8_t* mask
         <<<nb, THREADS, 0, st>>>(reinterpret_cast<const T*>(logits), topi, mask, T_, E, k, pp, cp, np, loss, counts,
                                  coef, status);
   });
-  if (nb > 1) finish_kernel<<<1, THREADS, 0, st>>>(pp, cp, np, nb, E, k, loss, counts, coef);
+  if (nb > 1) {  // its start overlaps the partial kernel's end
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1);
+    cfg.blockDim = dim3(FINISH_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, finish_kernel, (const float*)pp, (const int*)cp, (const int*)np, nb, E, k, loss, counts, coef);
+  }
 }
 
 template <class T>

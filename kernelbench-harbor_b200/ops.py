@@ -23,8 +23,7 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Zero-initialised scratch owned by this process, one per (device, stream).
     Kernels return it to the zero state, so it is allocated (and zeroed) once
     and reused; it is never shared by two streams, whose launches could overlap."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    key = (device.index, stream)
+    key = (device.index, _stream_ptr(device))
     with _ws_lock:
         buf = _ws.get(key)
         if buf is None or buf.numel() < nbytes:
@@ -54,7 +53,8 @@ def _dtype_code(dt: torch.dtype) -> int:
 
 
 def _stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # torch.cuda.current_stream(device).cuda_stream without the Stream object (0.1 us instead of 2.2)
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class _NoSwitch:
@@ -71,6 +71,19 @@ _no_switch = _NoSwitch()
 def _device(device: torch.device):
     """Context in which ``device`` is the current one (kernels launch on the current device)."""
     return _no_switch if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _once(backward, ctx, *grads):
+    """Runs a backward pass that has no gradient of its own; under create_graph
+    its results refuse to be differentiated (the wrapper for that costs 5 us,
+    so it is taken only there)."""
+    if torch.is_grad_enabled():
+        return torch.autograd.function.once_differentiable(backward)(ctx, *grads)
+    return backward(ctx, *grads)
 
 
 def _same_device(op: str, first: torch.Tensor, *rest: Optional[torch.Tensor]) -> None:
@@ -119,13 +132,12 @@ def _(x, qweight, scales, zeros, group):
     return x.new_empty((x.shape[0], qweight.shape[1] * 8))
 
 
-@torch.library.custom_op("b200q::w4a16_dgrad", mutates_args=())
 def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
                 group: int) -> torch.Tensor:
     """dx[M, K] = dy[M, N] . ((unpack(qweight) - zeros) * scales)^T, dx in dy.dtype:
     the input gradient of w4a16_gemm (the weights are frozen)."""
     if not dy.is_cuda:
-        raise RuntimeError("b200q::w4a16_dgrad runs on CUDA tensors only (no CPU implementation)")
+        raise RuntimeError("b200q w4a16_dgrad runs on CUDA tensors only (no CPU implementation)")
     if dy.dim() != 2 or qweight.dim() != 2:
         raise ValueError("dy must be [M, N] and qweight [K, N/8]")
     if qweight.dtype != torch.int32:
@@ -142,7 +154,7 @@ def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, z
     dt = _dtype_code(dy.dtype)
     _same_device("w4a16_dgrad", dy, qweight, scales, zeros)
     dy, qweight, scales, zeros = (_aligned(t) for t in (dy, qweight, scales.to(dy.dtype), zeros.to(dy.dtype)))
-    dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
+    dx = dy.new_empty((M, K))
     if M == 0:
         return dx
     with _device(dy.device):
@@ -151,11 +163,6 @@ def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, z
                                                 zeros.data_ptr(), dx.data_ptr(), M, N, K, group, dt, ws.data_ptr(),
                                                 ws.numel(), _stream_ptr(dy.device)))
     return dx
-
-
-@w4a16_dgrad.register_fake
-def _(dy, qweight, scales, zeros, group):
-    return dy.new_empty((dy.shape[0], qweight.shape[0]))
 
 
 def _w4a16_setup(ctx, inputs, output):
@@ -340,15 +347,14 @@ def _balance_forward(logits, topi, mask):
     L = _lib.lib()
     nbytes = L.b200q_moe_balance_scratch_bytes(T, E)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    coef = torch.empty((E,), dtype=torch.float32, device=dev)
+    coef = torch.empty((E + nbytes // 4,), dtype=torch.float32, device=dev)  # the kernel's scratch behind it
     counts = torch.empty((E,), dtype=torch.int32, device=dev)
-    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
     with _device(dev):
         ws = workspace(dev, 256)
-        _lib.check(L.b200q_moe_balance(logits.data_ptr(), topi.data_ptr(), mask.data_ptr() if mask is not None else None,
-                                       T, E, topi.shape[1], _LOGITS_CODES[logits.dtype], loss.data_ptr(),
-                                       counts.data_ptr(), coef.data_ptr(), scratch.data_ptr(), nbytes, ws.data_ptr(),
-                                       _stream_ptr(dev)))
+        p = coef.data_ptr()
+        _lib.check(L.b200q_moe_balance(logits.data_ptr(), topi.data_ptr(), _ptr(mask), T, E, topi.shape[1],
+                                       _LOGITS_CODES[logits.dtype], loss.data_ptr(), counts.data_ptr(), p, p + 4 * E,
+                                       nbytes, ws.data_ptr(), _stream_ptr(dev)))
     return loss, counts, coef
 
 
@@ -362,17 +368,18 @@ class _BalanceLoss(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dloss, _):
-        lg, mask, coef = ctx.saved_tensors
-        T, E = lg.shape
-        dloss = dloss.to(torch.float32).contiguous()
-        d = torch.empty_like(lg)
-        with _device(lg.device):
-            _lib.check(_lib.lib().b200q_moe_balance_grad(lg.data_ptr(), mask.data_ptr() if mask is not None else None,
-                                                         coef.data_ptr(), dloss.data_ptr(), T, E,
-                                                         _LOGITS_CODES[lg.dtype], d.data_ptr(), _stream_ptr(lg.device)))
-        return d, None, None
+        return _once(_balance_backward, ctx, dloss)
+
+
+def _balance_backward(ctx, dloss):
+    lg, mask, coef = ctx.saved_tensors
+    T, E = lg.shape
+    d = torch.empty_like(lg)
+    with _device(lg.device):
+        _lib.check(_lib.lib().b200q_moe_balance_grad(lg.data_ptr(), _ptr(mask), coef.data_ptr(), dloss.data_ptr(), T, E,
+                                                     _LOGITS_CODES[lg.dtype], d.data_ptr(), _stream_ptr(lg.device)))
+    return d, None, None
 
 
 def moe_balance_loss(router_logits: torch.Tensor, topi: torch.Tensor,
@@ -553,6 +560,9 @@ def lora_expand_add(base: torch.Tensor, lo: torch.Tensor, B: torch.Tensor, lora_
     return y
 
 
+_LORA_SMALL = 256  # tokens up to which b200q_lora_apply takes mid = NULL
+
+
 class LoraPlan:
     """A batch's tokens grouped by adapter: made once by lora_plan, used by
     every projection that the batch passes through."""
@@ -584,54 +594,52 @@ def lora_plan(lora_ids: torch.Tensor, n_adapters: int) -> LoraPlan:
     return LoraPlan(data, T, n_adapters)
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _lora_run(x, base, A, B, scaling, plan, transposed, out, want_out=True):
-    """(y or dx, lo or dlo) of one lora_apply call on contiguous, aligned tensors."""
-    T = x.shape[0]
+def _lora_run(x, base, A, B, scaling, plan, transposed, out, mid):
+    """One lora_apply call on contiguous, aligned tensors (see include/b200q.h)."""
     n_adapters, D, r = A.shape
-    N = B.shape[2]
     dev = x.device
-    L = _lib.lib()
-    mid = torch.empty((L.b200q_lora_mid_bytes(T, r) // 4,), dtype=torch.float32, device=dev)
-    if out is None and want_out:
-        out = torch.empty((T, D if transposed else N), dtype=x.dtype, device=dev)
     with _device(dev):
-        _lib.check(L.b200q_lora_apply(x.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling),
-                                      plan.data_ptr(), T, D, N, r, n_adapters, _dtype_code(x.dtype), transposed,
-                                      _ptr(out), mid.data_ptr(), _stream_ptr(dev)))
-    return out, mid
+        _lib.check(_lib.lib().b200q_lora_apply(x.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling),
+                                               plan.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters,
+                                               _dtype_code(x.dtype), transposed, _ptr(out), _ptr(mid),
+                                               _stream_ptr(dev)))
+
+
+def _lora_mid(x: torch.Tensor, r: int) -> torch.Tensor:
+    return torch.empty((_lib.lib().b200q_lora_mid_bytes(x.shape[0], r) // 4,), dtype=torch.float32, device=x.device)
 
 
 class _LoraApply(torch.autograd.Function):
     @staticmethod
     def forward(ctx, base, x, A, B, scaling, plan):
         base, x, A, B = _aligned(base), _aligned(x), _aligned(A), _aligned(B)
-        y, lo = _lora_run(x, base, A, B, scaling, plan, 0, None)
+        y, lo = torch.empty_like(base), _lora_mid(x, A.shape[2])
+        _lora_run(x, base, A, B, scaling, plan, 0, y, lo)
         ctx.save_for_backward(x, A, B, scaling, plan, lo)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, A, B, scaling, plan, lo = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        d = _aligned(dy)
-        dx = dlo = dA = dB = None
-        if need[1] or need[2]:
-            dx, dlo = _lora_run(d, None, A, B, scaling, plan, 1, None, want_out=need[1])
-        if need[2] or need[3]:
-            dA = torch.empty_like(A) if need[2] else None
-            dB = torch.empty_like(B) if need[3] else None
-            n_adapters, D, r = A.shape
-            with _device(x.device):
-                _lib.check(_lib.lib().b200q_lora_grads(x.data_ptr(), d.data_ptr(), lo.data_ptr(), _ptr(dlo),
-                                                       plan.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters,
-                                                       _dtype_code(x.dtype), _ptr(dA), _ptr(dB),
-                                                       _stream_ptr(x.device)))
-        return dy if need[0] else None, dx, dA, dB, None, None
+        return _once(_lora_backward, ctx, dy)
+
+
+def _lora_backward(ctx, dy):
+    x, A, B, scaling, plan, lo = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    d = _aligned(dy)
+    dx = dlo = dA = dB = None
+    if need[1] or need[2]:
+        dx, dlo = torch.empty_like(x) if need[1] else None, torch.empty_like(lo)
+        _lora_run(d, None, A, B, scaling, plan, 1, dx, dlo)
+    if need[2] or need[3]:
+        dA = torch.empty_like(A) if need[2] else None
+        dB = torch.empty_like(B) if need[3] else None
+        n_adapters, D, r = A.shape
+        with _device(x.device):
+            _lib.check(_lib.lib().b200q_lora_grads(x.data_ptr(), d.data_ptr(), lo.data_ptr(), _ptr(dlo),
+                                                   plan.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters,
+                                                   _dtype_code(x.dtype), _ptr(dA), _ptr(dB), _stream_ptr(x.device)))
+    return dy if need[0] else None, dx, dA, dB, None, None
 
 
 def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
@@ -648,12 +656,12 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     where no gradient is wanted."""
     if not x.is_cuda:
         raise RuntimeError("b200q lora_apply runs on CUDA tensors only")
-    if x.dim() != 2 or base.dim() != 2 or A.dim() != 3 or B.dim() != 3:
+    if x.dim() != 2 or A.dim() != 3 or B.dim() != 3:
         raise ValueError("lora_apply: base [T, N], x [T, D], A [L, D, r] and B [L, r, N] expected")
     T, D = x.shape
-    n_adapters, _, r = A.shape
-    N = B.shape[2]
-    if base.shape[0] != T or base.shape[1] != N or A.shape[1] != D or B.shape[0] != n_adapters or B.shape[1] != r:
+    n_adapters, Da, r = A.shape
+    Lb, rb, N = B.shape
+    if base.shape != (T, N) or Da != D or Lb != n_adapters or rb != r:
         raise ValueError(f"lora_apply: shapes do not fit: base {tuple(base.shape)}, x {tuple(x.shape)}, "
                          f"A {tuple(A.shape)}, B {tuple(B.shape)}")
     dt = x.dtype
@@ -671,7 +679,8 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
             raise ValueError(f"lora_apply: scaling must be [{n_adapters}]")
         if scaling.requires_grad:
             raise ValueError("lora_apply: scaling is a constant and has no gradient")
-        scaling = scaling.to(torch.float32).contiguous()
+        if scaling.dtype != torch.float32 or not scaling.is_contiguous():
+            scaling = scaling.to(torch.float32).contiguous()
     if A.dtype != dt:
         A = A.to(dt)
     if B.dtype != dt:
@@ -680,12 +689,19 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
         if out is not None:
             raise ValueError("lora_apply: out cannot be given where a gradient is wanted")
         return _LoraApply.apply(base, x, A, B, scaling, plan.data)
-    in_place = out is base
-    if out is not None and (out.shape != base.shape or out.dtype != dt or not out.is_contiguous()
-                            or out.data_ptr() % 16):
-        raise ValueError("lora_apply: out must be a contiguous, 16-byte aligned [T, N] tensor of x's dtype")
-    base = out if in_place else _aligned(base)
-    return _lora_run(_aligned(x), base, _aligned(A), _aligned(B), scaling, plan.data, 0, out)[0]
+    if out is None:
+        base = _aligned(base)
+        out = torch.empty_like(base)
+    else:
+        if out.shape != (T, N) or out.dtype != dt or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError("lora_apply: out must be a contiguous, 16-byte aligned [T, N] tensor of x's dtype")
+        if out is not base:
+            base = _aligned(base)
+    x = _aligned(x)
+    # the one-launch kernel needs no room for the row between
+    mid = None if T <= _LORA_SMALL else _lora_mid(x, r)
+    _lora_run(x, base, _aligned(A), _aligned(B), scaling, plan.data, 0, out, mid)
+    return out
 
 
 def moe_gather(x: torch.Tensor, slot_token: torch.Tensor) -> torch.Tensor:

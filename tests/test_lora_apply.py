@@ -437,7 +437,7 @@ def test_refusals_without_gpu():
         return L.b200q_lora_apply(x, p, p, p, None, p, T, D, N, r, nl, dtype, 0, y, mid, None)
 
     assert call(r=65) == call(r=0) == call(D=0) == call(N=1 << 23) == call(nl=1024) == call(T=-1) == _lib.ERR_SHAPE
-    assert call(x=None) == call(mid=None) == _lib.ERR_SHAPE
+    assert call(x=None) == call(mid=None, T=257) == call(mid=None, y=None) == _lib.ERR_SHAPE
     assert call(y=24) == call(x=8) == _lib.ERR_ALIGN
     assert call(dtype=2) == _lib.ERR_UNSUPPORTED
     assert call(T=0) == _lib.OK
