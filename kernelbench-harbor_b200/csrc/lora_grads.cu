@@ -22,13 +22,14 @@ namespace lora {
 
 constexpr int CT = 128;  // columns of a CTA
 constexpr int TK = 64;   // tokens of a stage
-constexpr int GSTG = 4;  // stages of the wide rows
 constexpr int WPITCH = CT * 2 + 16;
 constexpr int OPITCH = CT + 1;
-constexpr int TOKS = 8;  // stages of token indices kept (a power of two > GSTG + 1)
+constexpr int TOKS = 8;  // stages of token indices kept (more than GSTG + 2)
 
 template <int RP>
 struct GradCfg {
+  // stages of the wide rows and CTAs per SM: as many bytes in flight either way, more warps where they fit
+  static constexpr int GSTG = RP == 64 ? 4 : 3, CTAS = RP == 64 ? 2 : 3;
   static constexpr int TPITCH = RP * 2 + 16;
   static constexpr int WIDE = GSTG * TK * WPITCH;
   static constexpr int THIN = TK * TPITCH;  // one half of one stage; two stages are kept
@@ -47,8 +48,9 @@ struct GradArgs {
 };
 
 template <class T, int RP, bool VEC>
-__global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_grads_kernel(const GradArgs a, int S) {
+__global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 1) lora_grads_kernel(const GradArgs a, int S) {
   using C = GradCfg<RP>;
+  constexpr int GSTG = C::GSTG;
   constexpr bool F16 = std::is_same<T, __half>::value;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int s_tok[TOKS][TK];
@@ -186,10 +188,9 @@ __global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_grads_kernel(const 
         ldmatrix_x4_trans(h, th + k * 16 * C::TPITCH + i * 32);
         ldmatrix_x4_trans(l, th + C::THIN + k * 16 * C::TPITCH + i * 32);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          mma16816<T>(acc[i][p], h[0], h[1], h[2], h[3], b[2 * p], b[2 * p + 1]);
-          mma16816<T>(acc[i][p], l[0], l[1], l[2], l[3], b[2 * p], b[2 * p + 1]);
-        }
+        for (int p = 0; p < 4; ++p) mma16816<T>(acc[i][p], h[0], h[1], h[2], h[3], b[2 * p], b[2 * p + 1]);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) mma16816<T>(acc[i][p], l[0], l[1], l[2], l[3], b[2 * p], b[2 * p + 1]);
       }
     }
     if (F16) {
@@ -277,7 +278,7 @@ int launch_grads(const void* x, const void* dy, const float* lo, const float* dl
     const int64_t blocks = (int64_t)(a.nbd + nbn) * L, nst = (T_ + TK * L - 1) / (TK * L);
     int S = 1;
     int64_t best = INT64_MAX;
-    for (int s = 1; s <= 8 && (s == 1 || T_ >= 4 * TK * s); s *= 2) {
+    for (int s = 1; s <= 8 && (s == 1 || T_ >= 4 * TK * s); ++s) {
       const int64_t fit = resident_clusters((const void*)kern, THREADS, smem, s);
       const int64_t cost = ((blocks + fit - 1) / fit) * ((nst + s - 1) / s + 5);
       if (cost < best) best = cost, S = s;

@@ -116,7 +116,7 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t a0, const uint
 template <>
 __device__ __forceinline__ void mma16816<__half>(float* d, const uint32_t a0, const uint32_t a1, const uint32_t a2,
                                                  const uint32_t a3, const uint32_t b0, const uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -125,7 +125,7 @@ template <>
 __device__ __forceinline__ void mma16816<__nv_bfloat16>(float* d, const uint32_t a0, const uint32_t a1,
                                                         const uint32_t a2, const uint32_t a3, const uint32_t b0,
                                                         const uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -140,6 +140,10 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, uint32_t addr) {
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+// The same for the wide rows: a row's next 128 bytes, the next stage's, come to L2 along with these.
+__device__ __forceinline__ void cp_async16_ahead(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -204,9 +208,11 @@ __device__ __forceinline__ void stage8(void* dst, const T* row, int k, int K, bo
 }
 
 // The same from a pointer to the piece itself; `left`: values of the row from there on.
-template <class T, bool VEC>
+template <class T, bool VEC, bool WIDE_ROW = false>
 __device__ __forceinline__ void stage16(void* dst, const T* piece, int left, bool in, const T* any) {
-  if constexpr (VEC)
+  if constexpr (VEC && WIDE_ROW)
+    cp_async16_ahead(smem_u32(dst), in && left > 0 ? piece : any, in && left > 0);
+  else if constexpr (VEC)
     cp_async16(smem_u32(dst), in && left > 0 ? piece : any, in && left > 0);
   else
     *reinterpret_cast<uint4*>(dst) = in ? ld8<T, false>(piece, 0, left) : make_uint4(0, 0, 0, 0);

@@ -1,8 +1,8 @@
 // Many tokens (prefill, training): shrink and expand as two launches over tiles
 // of up to 128 rows of one adapter, both streaming wide rows through a ring of
-// STG stages of 128 rows x 64 columns in shared memory (asynchronous 16-byte
-// copies, 8 lanes to a row's 128 bytes), so that two CTAs keep ~96 KB of HBM
-// reads in flight on each SM.
+// 3 or 4 stages of 128 rows x 64 columns in shared memory (asynchronous 16-byte
+// copies, 8 lanes to a row's 128 bytes), so that the CTAs of an SM keep ~96 KB
+// of HBM reads in flight.
 //
 // shrink: a warp takes 32 rows and one 32-wide half of every stage (a piece of
 // P then serves two row blocks; at rank 64, where their sums would fill the
@@ -23,10 +23,14 @@ namespace b200q {
 namespace lora {
 
 constexpr int SK = 64;  // columns of a stage
-constexpr int STG = 4;
 constexpr int ROWB = SK * 2;               // bytes of a stage's wide row; 16-byte pieces are XOR-swizzled by the row
 constexpr int WIDE = ROWS_L * ROWB;        // bytes of a stage's wide rows
 constexpr int MAX_SPLIT = 8;
+
+// Stages of the ring and CTAs per SM: 2 x 4 at rank 64, else 3 x 3 -- as many
+// bytes in flight, and half as many warps again to hide each other's latencies.
+__host__ __device__ constexpr int stages_of(int rp) { return rp == 64 ? 4 : 3; }
+__host__ __device__ constexpr int ctas_of(int rp, bool vec) { return !vec ? 1 : rp == 64 ? 2 : 3; }
 
 // Swizzle of a row's 16-byte pieces: 8 rows x 1 piece (a fragment's words) and
 // 2 rows x 4 pieces (a quarter warp's 16-byte loads) both meet all banks once.
@@ -35,6 +39,7 @@ __device__ __forceinline__ int swz(int row) { return ((row & 1) << 2) | ((row >>
 // The 64 contraction rows of P / the rank rows of Q lie RP or 64 values wide.
 template <int RP, bool TR>
 struct ShrinkCfg {
+  static constexpr int STG = stages_of(RP);
   static constexpr int PITCH = RP * 2 + 16;                    // !TR: bytes per contraction row
   static constexpr int THIN = TR ? RP * ROWB : SK * PITCH;     // TR: rank rows of 64 values
   static constexpr int STAGE = WIDE + THIN;
@@ -44,8 +49,9 @@ struct ShrinkCfg {
 };
 
 template <class T, int RP, bool TR, bool VEC>
-__global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_shrink_tile_kernel(const Args a, int S) {
+__global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_shrink_tile_kernel(const Args a, int S) {
   using C = ShrinkCfg<RP, TR>;
+  constexpr int STG = C::STG;
   extern __shared__ __align__(128) uint8_t sm[];
   const int tile = blockIdx.x / S, rank = S > 1 ? (int)cluster_ctarank() : 0;
   const int32_t* plan = a.plan;
@@ -82,7 +88,7 @@ __global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_shrink_tile_kernel(
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (i < active) {
-        stage16<T, VEC>(buf + wdst + 32 * i * ROWB, src[i], D - kst - pc * 8, src[i] != nullptr, x);
+        stage16<T, VEC, true>(buf + wdst + 32 * i * ROWB, src[i], D - kst - pc * 8, src[i] != nullptr, x);
         if (src[i]) src[i] += SK;
       }
     uint8_t* thin = buf + WIDE;
@@ -123,20 +129,30 @@ __global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_shrink_tile_kernel(
           for (int e = 0; e < 2; ++e)
             xv[m][e] = *reinterpret_cast<const uint4*>(buf + (16 * (NM * mg + m) + 8 * e + g) * ROWB + (((4 * h + t) ^ swz(g)) << 4));
         const uint32_t row = smem_u32(buf + WIDE + (32 * h + lane) * C::PITCH);
+        // fragments of 4 column tiles at a time, then their products: none waits for the one before
+        constexpr int JB = RP / 8 < 4 ? RP / 8 : 4;
 #pragma unroll
-        for (int j = 0; j < RP / 8; ++j) {
-          uint32_t b[4];
-          if constexpr (!TR) {
-            ldmatrix_x4_trans(b, row + j * 16);
-          } else {
-            const uint4 w = *reinterpret_cast<const uint4*>(buf + WIDE + (8 * j + g) * ROWB + (((4 * h + t) ^ swz(g)) << 4));
-            b[0] = w.x, b[1] = w.y, b[2] = w.z, b[3] = w.w;
+        for (int j0 = 0; j0 < RP / 8; j0 += JB) {
+          uint32_t b[JB][4];
+#pragma unroll
+          for (int j = 0; j < JB; ++j) {
+            if constexpr (!TR) {
+              ldmatrix_x4_trans(b[j], row + (j0 + j) * 16);
+            } else {
+              const uint4 w = *reinterpret_cast<const uint4*>(buf + WIDE + (8 * (j0 + j) + g) * ROWB + (((4 * h + t) ^ swz(g)) << 4));
+              b[j][0] = w.x, b[j][1] = w.y, b[j][2] = w.z, b[j][3] = w.w;
+            }
           }
 #pragma unroll
-          for (int m = 0; m < NM; ++m) {
-            mma16816<T>(acc[m][j], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, b[0], b[1]);
-            mma16816<T>(acc[m][j], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, b[2], b[3]);
-          }
+          for (int m = 0; m < NM; ++m)
+#pragma unroll
+            for (int j = 0; j < JB; ++j)
+              mma16816<T>(acc[m][j0 + j], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, b[j][0], b[j][1]);
+#pragma unroll
+          for (int m = 0; m < NM; ++m)
+#pragma unroll
+            for (int j = 0; j < JB; ++j)
+              mma16816<T>(acc[m][j0 + j], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, b[j][2], b[j][3]);
         }
       }
     }
@@ -196,6 +212,7 @@ __global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_shrink_tile_kernel(
 
 template <int RP, bool TR>
 struct ExpandCfg {
+  static constexpr int STG = stages_of(RP);
   // !TR: bytes per rank row of 64 columns; TR: per column row of RP ranks, 8 words mod 32 (no bank conflicts)
   static constexpr int PITCH = !TR ? ROWB + 16 : RP == 16 ? 32 : RP == 32 ? 96 : 160;
   static constexpr int THIN = (TR ? SK : RP) * PITCH;
@@ -205,8 +222,9 @@ struct ExpandCfg {
 
 // CTA = (tile, part): `steps` 64-column steps from step part * steps on.
 template <class T, int RP, bool TR, bool VEC>
-__global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_expand_tile_kernel(const Args a, int parts, int steps) {
+__global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_kernel(const Args a, int parts, int steps) {
   using C = ExpandCfg<RP, TR>;
+  constexpr int STG = C::STG;
   extern __shared__ __align__(128) uint8_t sm[];
   const int32_t* plan = a.plan;
   const int tile = blockIdx.x / parts;  // a tile's parts run side by side
@@ -247,7 +265,7 @@ __global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_expand_tile_kernel(
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (i < active) {
-          stage16<T, VEC>(buf + wdst + 32 * i * ROWB, src[i], N - cst - pc * 8, src[i] != nullptr, base);
+          stage16<T, VEC, true>(buf + wdst + 32 * i * ROWB, src[i], N - cst - pc * 8, src[i] != nullptr, base);
           if (src[i]) src[i] += SK;
         }
     }
@@ -364,10 +382,11 @@ __global__ void __launch_bounds__(THREADS, VEC ? 2 : 1) lora_expand_tile_kernel(
             }
           }
 #pragma unroll
-          for (int p = 0; p < 4; ++p) {
+          for (int p = 0; p < 4; ++p)
             mma16816<T>(c[p], ha[k][0].x, ha[k][1].x, ha[k][0].y, ha[k][1].y, b[2 * p], b[2 * p + 1]);
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
             mma16816<T>(c[p], la[k][0].x, la[k][1].x, la[k][0].y, la[k][1].y, b[2 * p], b[2 * p + 1]);
-          }
         }
         const int left = N - n0 - st * SK - 32 * w - 8 * t;  // columns of the row from this lane's on
         uint4 ua = make_uint4(0, 0, 0, 0), ub = ua;
@@ -397,10 +416,11 @@ int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
     if (rc2 || (rc2 = allow_smem((const void*)expand, smem_e, "cudaFuncSetAttribute(lora expand)"))) return rc2;
     // shrink: the split with the shortest estimate, rounds of co-resident
     // clusters x (stages of a part + 5 for start, joining and ending)
-    const int64_t tiles = (a.T + ROWS_L - 1) / ROWS_L, nst = (a.D + SK - 1) / SK;
+    // (about half a tile more than T / 128 for each adapter that ends inside one)
+    const int64_t full = (a.T + ROWS_L - 1) / ROWS_L, tiles = full + std::min(a.L, full) / 2, nst = (a.D + SK - 1) / SK;
     int S = 1;
     int64_t best = INT64_MAX;
-    for (int s = 1; s <= MAX_SPLIT && (s == 1 || nst >= 4 * s); s *= 2) {
+    for (int s = 1; s <= MAX_SPLIT && (s == 1 || nst >= 4 * s); ++s) {
       const int64_t fit = resident_clusters((const void*)shrink, THREADS, smem_s, s);
       const int64_t cost = ((tiles + fit - 1) / fit) * ((nst + s - 1) / s + 5);
       if (cost < best) best = cost, S = s;

@@ -365,6 +365,7 @@ class _BalanceLoss(torch.autograd.Function):
         loss, counts, coef = _balance_forward(lg, topi, mask)
         ctx.save_for_backward(lg, mask, coef)
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)  # no zeros for counts
         return loss, counts
 
     @staticmethod
@@ -373,6 +374,8 @@ class _BalanceLoss(torch.autograd.Function):
 
 
 def _balance_backward(ctx, dloss):
+    if dloss is None:
+        return None, None, None
     lg, mask, coef = ctx.saved_tensors
     T, E = lg.shape
     d = torch.empty_like(lg)
