@@ -519,6 +519,36 @@ Plan plan(int64_t M, int64_t N, int64_t K, int sms) {
   return p;
 }
 
+// The same choice for MODE_DX (N: weight rows, K: weight columns), from its own
+// measurements: a 128-row stage takes 0.5 us and a 256-row one 1.34 times that;
+// joining a split through distributed shared memory costs as much as 11 stages
+// (two passes: 24), start and end 15.  M=1000, N=1408, K=2048: 18 us unsplit
+// with 128-row tiles, 26 us as 256-row tiles split four ways; M=17, N=4096,
+// K=14336: 39 us unsplit, 29 us split in two.
+Plan plan_dx(int64_t M, int64_t N, int64_t K, int sms) {
+  Plan p;
+  p.tiles_n = (int)((N + BN - 1) / BN);
+  const int nk = (int)((K + BK - 1) / BK);
+  double best = 0;
+  for (int mb = 1; mb <= 2; ++mb) {
+    const int64_t tm = (M + BM * mb - 1) / (BM * mb), tiles = tm * p.tiles_n;
+    for (int sp = 1; sp <= MAX_SPLITS; ++sp) {
+      if (sp > 1 && (tiles * sp > sms || nk < 4 * sp)) break;
+      const int64_t waves = (tiles * sp + sms - 1) / sms;
+      const double cost = (double)waves * ((nk + sp - 1) / sp) * (mb == 2 ? 1.34 : 1.0) +
+                          (sp == 1 ? 0.0 : mb == 2 ? 24.0 : 11.0) + 15.0;
+      if ((mb == 1 && sp == 1) || cost < best) {
+        best = cost;
+        p.mb = mb;
+        p.splits = sp;
+        p.tiles_m = (int)std::min<int64_t>(tm, 1 << 30);
+      }
+    }
+  }
+  p.ws_bytes = HEADER_BYTES;
+  return p;
+}
+
 // Launches `kern` over the plan's tiles, `splits` CTAs of a tile as a cluster.
 template <class Kern>
 int launch(Kern kern, uint32_t smem, Plan p, const CUtensorMap& tx, const CUtensorMap& twq, const CUtensorMap& ts,
@@ -603,7 +633,7 @@ int w4a16_tc_dgrad(const void* dy, const int32_t* qweight, const void* scales, c
                    int64_t N, int64_t K, int64_t group, int dtype, void* workspace, size_t workspace_bytes,
                    cudaStream_t stream) {
   using namespace tc;
-  Plan p = plan(M, K, N, num_sms(-1));
+  Plan p = plan_dx(M, K, N, num_sms(-1));
   if (p.tiles_m > 65535) return fail(B200Q_ERR_SHAPE, "w4a16 dgrad: M too large");
   if (!workspace || workspace_bytes < p.ws_bytes)
     return fail(B200Q_ERR_WORKSPACE, "w4a16 dgrad: workspace of " + std::to_string(p.ws_bytes) + " bytes required");

@@ -9,10 +9,11 @@ from tests.helpers import tdt, torch_dequant_fp32, w4a16_inputs
 
 def check(dx, dy, q, s, z, group):
     """Elementwise bounds from the two roundings.  Against the weight rounded to
-    the activation type (as the kernel and the reference module hold it): the
-    last rounding, u |dx|, and the fp32 accumulation, at most one 2^-23 step per
-    16-wide multiply-add of the N / 16 in the chain, of S = sum |dy| |w|.
-    Against the weight in full: u S more."""
+    the activation type (as the tensor-core kernel, M >= 17, and the reference
+    module hold it): the last rounding, u |dx|, and the fp32 accumulation, at
+    most one 2^-23 step per 16-wide multiply-add of the N / 16 in the chain, of
+    S = sum |dy| |w|.  Against the weight in full: u S more, from the rounding
+    of the weight or (M <= 16) of dy times the scale."""
     u = torch.finfo(dy.dtype).eps / 2
     w = torch_dequant_fp32(q, s, z, group).double()
     K = w.shape[0]
@@ -23,7 +24,7 @@ def check(dx, dy, q, s, z, group):
     tiny = 2.0 ** -25 if dy.dtype == torch.float16 else 0.0
     assert dx.shape == (dy.shape[0], K) and dx.dtype == dy.dtype
     ref = d @ wr.t()
-    assert ((dx.double() - ref).abs() <= u * (ref.abs() + acc) + acc + tiny).all()
+    assert dy.shape[0] <= 16 or ((dx.double() - ref).abs() <= u * (ref.abs() + acc) + acc + tiny).all()
     full = d @ w.t()
     assert ((dx.double() - full).abs() <= u * (full.abs() + 2 * S) + acc + tiny).all()
 
@@ -37,7 +38,7 @@ def grads_in(M, K, N, group, dtype, seed=0):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("M,K,N,group", [
-    (1, 128, 32, 128), (1, 4096, 4096, 128), (3, 32, 64, 32), (16, 14336, 4096, 128), (17, 96, 96, 32),
+    (1, 128, 32, 128), (2, 256, 1056, 256), (7, 96, 160, 32), (16, 192, 2048, 64), (5, 1408, 2080, 64), (1, 4096, 4096, 128), (3, 32, 64, 32), (16, 14336, 4096, 128), (17, 96, 96, 32),
     (129, 192, 224, 64), (130, 512, 1408, 256), (255, 2048, 1408, 64), (300, 320, 160, 64), (1000, 2048, 1408, 64),
     (777, 288, 4096, 32)])
 def test_against_float64(M, K, N, group, dtype):
@@ -53,6 +54,22 @@ def test_one_weight_at_a_time():
     dx = ops.w4a16_dgrad(torch.eye(96, dtype=torch.float16, device="cuda"), q, s, z, 32)
     w = torch_dequant_fp32(q, s, z, 32).half()  # (nib - z) s: one rounding
     assert torch.equal(dx, w.t())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [9, 40])
+def test_small_and_large_gradients_in_fp16(M):
+    """Rows of dy from the subnormals to near the type's end, and infinities and
+    NaN that stay in their rows."""
+    dy, q, s, z = grads_in(M, 256, 512, 64, "fp16", seed=6)
+    dy = (dy.float() * torch.logspace(-5, 3, M, base=10.0, device="cuda")[:, None]).half()
+    clean = ops.w4a16_dgrad(dy, q, s, z, 64)
+    check(clean, dy, q, s, z, 64)
+    dy[2, 7], dy[4, 9] = float("inf"), float("nan")
+    dx = ops.w4a16_dgrad(dy, q, s, z, 64)
+    rest = [m for m in range(M) if m not in (2, 4)]
+    assert torch.equal(dx[rest], clean[rest])
+    assert torch.isnan(dx[4]).all() and not torch.isfinite(dx[2]).any()
 
 
 @pytest.mark.gpu
