@@ -75,14 +75,16 @@ __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 1) lora_gra
     const int i = f0 + st * TK + tid;
     s_tok[st % TOKS][tid] = i < f1 ? order[i] : -1;
   };
+  const T* wcol = wide + w0 + (tid & 15) * 8;
+  const int wleft = W - w0 - (tid & 15) * 8;
   auto stage_wide = [&](int st) {
-    uint8_t* buf = sm + st % GSTG * TK * WPITCH;
-#pragma unroll
-    for (int i = 0; i < TK / 16; ++i) {
-      const int row = 16 * i + (tid >> 4), tok = s_tok[st % TOKS][row];
-      stage8<T, VEC>(buf + row * WPITCH + (tid & 15) * 16, wide + (size_t)max(tok, 0) * W, w0 + (tid & 15) * 8, W,
-                     tok >= 0, wide);
-    }
+    // this thread's 16 bytes of rows tid / 16 + 16 i
+    const uint32_t dst = smem_u32(sm) + st % GSTG * (TK * WPITCH) + (tid >> 4) * WPITCH + (tid & 15) * 16;
+    const int* toks = &s_tok[st % TOKS][tid >> 4];
+    static_for<TK / 16>([&](auto i) {
+      const int tok = toks[16 * i];
+      stage16<T, VEC, true, 16 * i * WPITCH>(dst, wcol + (size_t)max(tok, 0) * W, wleft, tok >= 0, wide);
+    });
   };
   float4 tv[C::VPT];
   auto load_thin = [&](int st) {
@@ -177,22 +179,20 @@ __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 1) lora_gra
                         (cg * 32 + 8 * (lane >> 4)) * 2;
     const uint32_t th = smem_u32(sm + C::WIDE + (st & 1) * 2 * C::THIN) +
                         (32 * half + 8 * (lane >> 4) + (lane & 7)) * C::TPITCH + 16 * ((lane >> 3) & 1);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    static_for<2>([&](auto k) {
       uint32_t b[8];
-      ldmatrix_x4_trans(b, wb + k * 16 * WPITCH);
-      ldmatrix_x4_trans(b + 4, wb + k * 16 * WPITCH + 32);
-#pragma unroll
-      for (int i = 0; i < RP / 16; ++i) {
+      ldmatrix_x4_trans<k * 16 * WPITCH>(b, wb);
+      ldmatrix_x4_trans<k * 16 * WPITCH + 32>(b + 4, wb);
+      static_for<RP / 16>([&](auto i) {
         uint32_t h[4], l[4];
-        ldmatrix_x4_trans(h, th + k * 16 * C::TPITCH + i * 32);
-        ldmatrix_x4_trans(l, th + C::THIN + k * 16 * C::TPITCH + i * 32);
+        ldmatrix_x4_trans<k * 16 * C::TPITCH + i * 32>(h, th);
+        ldmatrix_x4_trans<C::THIN + k * 16 * C::TPITCH + i * 32>(l, th);
 #pragma unroll
         for (int p = 0; p < 4; ++p) mma16816<T>(acc[i][p], h[0], h[1], h[2], h[3], b[2 * p], b[2 * p + 1]);
 #pragma unroll
         for (int p = 0; p < 4; ++p) mma16816<T>(acc[i][p], l[0], l[1], l[2], l[3], b[2 * p], b[2 * p + 1]);
-      }
-    }
+      });
+    });
     if (F16) {
       if (rescale != 1.f) {
 #pragma unroll

@@ -17,6 +17,9 @@
 // (one 16-byte load) as its parts of two k16 steps; of the output columns, the
 // order is chosen so that a thread ends with 8 consecutive ones.
 #pragma once
+#include <type_traits>
+#include <utility>
+
 #include "common.cuh"
 
 namespace b200q {
@@ -131,19 +134,55 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float* d, const uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Shared-memory accesses at a register plus an immediate: the loops over stages
+// are bound by the length of a warp's instruction chain, so no address is
+// computed in them that a constant can hold.
+template <int OFF = 0>
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
+               : "r"(addr), "n"(OFF)
                : "memory");
 }
+template <int OFF = 0>
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr), "n"(OFF)
+               : "memory");
+  return v;
+}
+template <int OFF = 0>
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2+%3];" : "=r"(v.x), "=r"(v.y) : "r"(addr), "n"(OFF) : "memory");
+  return v;
+}
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+// f(0), ..., f(N - 1) with the index as a compile-time value
+template <int V>
+struct Index {
+  __host__ __device__ constexpr operator int() const { return V; }
+};
+template <int... I, class F>
+__device__ __forceinline__ void static_for_impl(std::integer_sequence<int, I...>, F&& f) {
+  (f(Index<I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+  static_for_impl(std::make_integer_sequence<int, N>{}, f);
+}
+
+// 16 bytes to shared memory, `bytes` of them (16 or 0) from src and zeros for the rest
+template <int OFF = 0>
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0+%3], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(OFF) : "memory");
 }
 // The same for the wide rows: a row's next 128 bytes, the next stage's, come to L2 along with these.
-__device__ __forceinline__ void cp_async16_ahead(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+template <int OFF = 0>
+__device__ __forceinline__ void cp_async16_ahead(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0+%3], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(OFF) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -199,23 +238,17 @@ __device__ __forceinline__ void st8(T* row, int k, int K, const uint4 v) {
 }
 
 // 16 bytes of a row into shared memory: asynchronous where alignment allows.
-template <class T, bool VEC>
-__device__ __forceinline__ void stage8(void* dst, const T* row, int k, int K, bool in, const T* any) {
-  if constexpr (VEC)
-    cp_async16(smem_u32(dst), in && k < K ? row + k : any, in && k < K);
-  else
-    *reinterpret_cast<uint4*>(dst) = in ? ld8<T, false>(row, k, K) : make_uint4(0, 0, 0, 0);
-}
-
-// The same from a pointer to the piece itself; `left`: values of the row from there on.
-template <class T, bool VEC, bool WIDE_ROW = false>
-__device__ __forceinline__ void stage16(void* dst, const T* piece, int left, bool in, const T* any) {
-  if constexpr (VEC && WIDE_ROW)
-    cp_async16_ahead(smem_u32(dst), in && left > 0 ? piece : any, in && left > 0);
-  else if constexpr (VEC)
-    cp_async16(smem_u32(dst), in && left > 0 ? piece : any, in && left > 0);
-  else
-    *reinterpret_cast<uint4*>(dst) = in ? ld8<T, false>(piece, 0, left) : make_uint4(0, 0, 0, 0);
+// `left`: values of the row from the piece on; `any`: an address that may be read.
+template <class T, bool VEC, bool WIDE_ROW = false, int OFF = 0>
+__device__ __forceinline__ void stage16(uint32_t dst, const T* piece, int left, bool in, const T* any) {
+  if constexpr (VEC && WIDE_ROW) {
+    cp_async16_ahead<OFF>(dst, in && left > 0 ? piece : any, in && left > 0 ? 16 : 0);
+  } else if constexpr (VEC) {
+    cp_async16<OFF>(dst, in && left > 0 ? piece : any, in && left > 0 ? 16 : 0);
+  } else {
+    const uint4 v = in ? ld8<T, false>(piece, 0, left) : make_uint4(0, 0, 0, 0);
+    asm volatile("st.shared.v4.u32 [%0+%5], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "n"(OFF) : "memory");
+  }
 }
 
 // base + fac * c for the 8 consecutive columns of one row: c[p][h], c[p][h + 1] are columns 2p, 2p + 1

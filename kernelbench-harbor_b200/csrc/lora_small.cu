@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(THREADS) lora_small_kernel(const Args a) {
       for (int i = 0; i < RP / 8; ++i) {
         const int idx = lane + 32 * i, k = idx / (RP / 8), pc = idx % (RP / 8);
         const int kk = 32 * c + k;
-        stage8<T, VEC>(ring + s * 32 * C::PITCH + row32(k) * C::PITCH + pc * 16, P + (size_t)kk * r, pc * 8, r, kk < D, P);
+        stage16<T, VEC>(smem_u32(ring + s * 32 * C::PITCH + row32(k) * C::PITCH + pc * 16), P + (size_t)kk * r + pc * 8,
+                        r - pc * 8, kk < D, P);
       }
     }
   };

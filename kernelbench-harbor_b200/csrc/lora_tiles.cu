@@ -71,39 +71,50 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_shrink_tile_ke
 
   // this thread's pieces of a stage: 16 bytes of rows tid / 8 + 32 i, and of P; pointers advance by a stage
   const int pc = tid & 7, prow = tid >> 3;
-  const int active = (count + 31) / 32;  // 32-row blocks that hold rows
   const T* src[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool in = prow + 32 * i < count;
-    src[i] = in ? x + (size_t)rows[prow + 32 * i] * D + s0 * SK + pc * 8 : nullptr;
-  }
-  constexpr int PIECES = SK * RP / 8, PSTEP = TR ? THREADS / 8 : THREADS / (RP / 8);  // rows of P between a thread's pieces
+  for (int i = 0; i < 4; ++i)
+    src[i] = x + (size_t)rows[prow + 32 * i < count ? prow + 32 * i : 0] * D + s0 * SK + pc * 8;
+  constexpr int PIECES = SK * RP / 8, NP = (PIECES + THREADS - 1) / THREADS;
+  constexpr int PSTEP = TR ? THREADS / 8 : THREADS / (RP / 8);  // rows of P between a thread's pieces
+  static_assert(PSTEP % 32 == 0, "row32(row + PSTEP) = row32(row) + PSTEP, and swz(row + PSTEP) = swz(row)");
   const int q = TR ? tid & 7 : tid % (RP / 8), prk = TR ? tid >> 3 : tid / (RP / 8);
-  const T* psrc = TR ? P + (size_t)prk * D + s0 * SK + q * 8 : P + (size_t)(s0 * SK + prk) * r + q * 8;
-  const uint32_t wdst = prow * ROWB + ((pc ^ swz(prow)) << 4);
-  int kst = s0 * SK, slot_in = 0;  // first column and ring slot of the stage that is requested next
+  const bool has_p = PIECES % THREADS == 0 || tid < PIECES;
+  const T* psrc[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+    psrc[i] = TR ? P + (size_t)(prk + i * PSTEP) * D + s0 * SK + q * 8 : P + (size_t)(s0 * SK + prk + i * PSTEP) * r + q * 8;
+  const uint32_t smem = smem_u32(sm), wdst = prow * ROWB + ((pc ^ swz(prow)) << 4);
+  const uint32_t pdst = WIDE + (TR ? prk * ROWB + ((q ^ swz(prk)) << 4) : row32(prk) * C::PITCH + q * 16);
+  int kst = s0 * SK;     // first column of the stage that is requested next
+  uint32_t in = smem;    // and its ring slot
   auto stage = [&]() {
-    uint8_t* buf = sm + slot_in * C::STAGE;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < active) {
-        stage16<T, VEC, true>(buf + wdst + 32 * i * ROWB, src[i], D - kst - pc * 8, src[i] != nullptr, x);
-        if (src[i]) src[i] += SK;
-      }
-    uint8_t* thin = buf + WIDE;
-#pragma unroll
-    for (int i = 0; i < (PIECES + THREADS - 1) / THREADS; ++i) {
-      const int row = prk + i * PSTEP;
-      if (PIECES % THREADS && row >= (TR ? RP : SK)) break;
-      if constexpr (!TR)
-        stage16<T, VEC>(thin + row32(row) * C::PITCH + q * 16, psrc + (size_t)(i * PSTEP) * r, r - q * 8, kst + row < D, P);
-      else
-        stage16<T, VEC>(thin + row * ROWB + ((q ^ swz(row)) << 4), psrc + (size_t)(i * PSTEP) * D, D - kst - q * 8, row < r, P);
+    if (VEC && kst + SK <= D) {  // a whole stage: no column to check
+      static_for<4>([&](auto i) {
+        cp_async16_ahead<32 * i * ROWB>(in + wdst, src[i], prow + 32 * i < count ? 16 : 0);
+      });
+      if (has_p)
+        static_for<NP>([&](auto i) {
+          cp_async16<i * PSTEP*(TR ? ROWB : C::PITCH)>(in + pdst, psrc[i], (TR ? prk + i * PSTEP < r : q * 8 < r) ? 16 : 0);
+        });
+    } else {
+      static_for<4>([&](auto i) {
+        stage16<T, VEC, true, 32 * i * ROWB>(in + wdst, src[i], D - kst - pc * 8, prow + 32 * i < count, x);
+      });
+      if (has_p)
+        static_for<NP>([&](auto i) {
+          if constexpr (!TR)
+            stage16<T, VEC, false, i * PSTEP * C::PITCH>(in + pdst, psrc[i], r - q * 8, kst + prk + i * PSTEP < D, P);
+          else
+            stage16<T, VEC, false, i * PSTEP * ROWB>(in + pdst, psrc[i], D - kst - q * 8, prk + i * PSTEP < r, P);
+        });
     }
-    psrc += TR ? SK : (size_t)SK * r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) src[i] += SK;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) psrc[i] += TR ? SK : SK * r;
     kst += SK;
-    slot_in = slot_in + 1 == STG ? 0 : slot_in + 1;
+    in = in == smem + (STG - 1) * C::STAGE ? smem : in + C::STAGE;
   };
   float acc[NM][RP / 8][4] = {};
 #pragma unroll
@@ -111,51 +122,55 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_shrink_tile_ke
     if (s0 + i < s1) stage();
     cp_async_commit();
   }
-  int slot = 0;
+  // where this lane reads a stage: its rows' pieces of either half, and P's
+  const uint32_t xrow = (16 * NM * mg + g) * ROWB;
+  uint32_t xoff[NH], poff[NH];
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+    const uint32_t piece = ((4 * (half + h) + t) ^ swz(g)) << 4;
+    xoff[h] = xrow + piece;
+    poff[h] = WIDE + (TR ? g * ROWB + piece : (32 * (half + h) + lane) * C::PITCH);
+  }
+  uint32_t slot = smem;
   for (int st = s0; st < s1; ++st) {
     cp_async_wait<STG - 2>();
     __syncthreads();  // stage st has landed for every thread; the slot filled next was read before
     if (st + STG - 1 < s1) stage();
     cp_async_commit();
-    const uint8_t* buf = sm + slot * C::STAGE;
-    slot = slot + 1 == STG ? 0 : slot + 1;
     if (16 * NM * mg < count) {
 #pragma unroll
-      for (int h = half; h < half + NH; ++h) {
+      for (int h = 0; h < NH; ++h) {
         uint4 xv[NM][2];
-#pragma unroll
-        for (int m = 0; m < NM; ++m)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            xv[m][e] = *reinterpret_cast<const uint4*>(buf + (16 * (NM * mg + m) + 8 * e + g) * ROWB + (((4 * h + t) ^ swz(g)) << 4));
-        const uint32_t row = smem_u32(buf + WIDE + (32 * h + lane) * C::PITCH);
+        static_for<NM>([&](auto m) {
+          xv[m][0] = lds16<16 * m * ROWB>(slot + xoff[h]);
+          xv[m][1] = lds16<(16 * m + 8) * ROWB>(slot + xoff[h]);
+        });
         // fragments of 4 column tiles at a time, then their products: none waits for the one before
         constexpr int JB = RP / 8 < 4 ? RP / 8 : 4;
-#pragma unroll
-        for (int j0 = 0; j0 < RP / 8; j0 += JB) {
+        static_for<RP / 8 / JB>([&](auto j0) {
           uint32_t b[JB][4];
-#pragma unroll
-          for (int j = 0; j < JB; ++j) {
+          static_for<JB>([&](auto j) {
             if constexpr (!TR) {
-              ldmatrix_x4_trans(b[j], row + (j0 + j) * 16);
+              ldmatrix_x4_trans<(j0 * JB + j) * 16>(b[j], slot + poff[h]);
             } else {
-              const uint4 w = *reinterpret_cast<const uint4*>(buf + WIDE + (8 * (j0 + j) + g) * ROWB + (((4 * h + t) ^ swz(g)) << 4));
+              const uint4 w = lds16<(j0 * JB + j) * 8 * ROWB>(slot + poff[h]);
               b[j][0] = w.x, b[j][1] = w.y, b[j][2] = w.z, b[j][3] = w.w;
             }
-          }
+          });
 #pragma unroll
           for (int m = 0; m < NM; ++m)
 #pragma unroll
             for (int j = 0; j < JB; ++j)
-              mma16816<T>(acc[m][j0 + j], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, b[j][0], b[j][1]);
+              mma16816<T>(acc[m][j0 * JB + j], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, b[j][0], b[j][1]);
 #pragma unroll
           for (int m = 0; m < NM; ++m)
 #pragma unroll
             for (int j = 0; j < JB; ++j)
-              mma16816<T>(acc[m][j0 + j], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, b[j][2], b[j][3]);
-        }
+              mma16816<T>(acc[m][j0 * JB + j], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, b[j][2], b[j][3]);
+        });
       }
     }
+    slot = slot == smem + (STG - 1) * C::STAGE ? smem : slot + C::STAGE;
   }
   pdl_launch_next();
   cp_async_wait<0>();
@@ -246,64 +261,74 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const T* Q = reinterpret_cast<const T*>(a.Q) + (size_t)tl.x * r * N;
   const int pc = tid & 7, prow = tid >> 3;
-  const int active = (count + 31) / 32;
   const T* src[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool in = base && prow + 32 * i < count;
-    src[i] = in ? base + (size_t)rows[prow + 32 * i] * N + n0 + pc * 8 : nullptr;
-  }
+  for (int i = 0; i < 4; ++i)
+    src[i] = base ? base + (size_t)rows[prow + 32 * i < count ? prow + 32 * i : 0] * N + n0 + pc * 8 : nullptr;
   constexpr int PIECES = SK * RP / 8, NP = (PIECES + THREADS - 1) / THREADS;
   constexpr int PSTEP = TR ? THREADS / (RP / 8) : THREADS / 8;  // rows of Q between a thread's pieces
+  static_assert(PSTEP % 32 == 0, "the row orders repeat every 32");
   const int q = TR ? tid % (RP / 8) : tid & 7, qrow = TR ? tid / (RP / 8) : tid >> 3;
-  const uint32_t wdst = prow * ROWB + ((pc ^ swz(prow)) << 4);
-  int cst = n0, slot_in = 0;
+  const bool has_q = PIECES % THREADS == 0 || tid < PIECES;
+  const T* qsrc[NP];
+  int qin[NP];  // TR: bytes of the piece inside the rank; !TR: whether the rank row exists
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int row = qrow + i * PSTEP, k = k_of_row16(row);  // !TR: rank rows in fragment order
+    qsrc[i] = TR ? Q + (size_t)(n0 + row) * r + q * 8 : Q + (size_t)(k < r ? k : 0) * N + n0 + q * 8;
+    qin[i] = TR ? (q * 8 < r ? 16 : 0) : k < r;
+  }
+  // TR: column 32 w + 8 a + 2 p + b is row 32 w + 8 p + 2 a + b: a fragment's columns together
+  const uint32_t smem = smem_u32(sm), wdst = prow * ROWB + ((pc ^ swz(prow)) << 4);
+  const uint32_t qdst = WIDE + (TR ? ((qrow & ~31) | (((qrow >> 1) & 3) << 3) | (((qrow >> 3) & 3) << 1) | (qrow & 1)) * C::PITCH + q * 16
+                                   : qrow * C::PITCH + (q >> 2) * 64 + (q & 3) * 4);
+  int cst = n0;
+  uint32_t in = smem;
   // base (and, TR, A's rows) by asynchronous copies
   auto stage = [&]() {
-    uint8_t* buf = sm + slot_in * C::STAGE;
-    if (base) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < active) {
-          stage16<T, VEC, true>(buf + wdst + 32 * i * ROWB, src[i], N - cst - pc * 8, src[i] != nullptr, base);
-          if (src[i]) src[i] += SK;
-        }
+    if (VEC && cst + SK <= N) {
+      if (base)
+        static_for<4>([&](auto i) {
+          cp_async16_ahead<32 * i * ROWB>(in + wdst, src[i], prow + 32 * i < count ? 16 : 0);
+        });
+      if (TR && has_q) static_for<NP>([&](auto i) { cp_async16<i * PSTEP * C::PITCH>(in + qdst, qsrc[i], qin[i]); });
+    } else {
+      if (base)
+        static_for<4>([&](auto i) {
+          stage16<T, VEC, true, 32 * i * ROWB>(in + wdst, src[i], N - cst - pc * 8, prow + 32 * i < count, base);
+        });
+      if (TR && has_q)
+        static_for<NP>([&](auto i) {
+          stage16<T, VEC, false, i * PSTEP * C::PITCH>(in + qdst, qsrc[i], r - q * 8, cst + qrow + i * PSTEP < N, Q);
+        });
     }
-    if constexpr (TR) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int c = qrow + i * PSTEP;
-        if (PIECES % THREADS && c >= SK) break;
-        // column 32 w + 8 a + 2 p + b is row 32 w + 8 p + 2 a + b: a fragment's columns together
-        const int row = (c & 32) | (((c >> 1) & 3) << 3) | (((c >> 3) & 3) << 1) | (c & 1);
-        stage16<T, VEC>(buf + WIDE + row * C::PITCH + q * 16, Q + (size_t)(cst + c) * r + q * 8, r - q * 8, cst + c < N, Q);
-      }
+    for (int i = 0; i < 4; ++i) src[i] += SK;
+    if (TR) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) qsrc[i] += SK * r;
     }
     cst += SK;
-    slot_in = slot_in + 1 == STG ? 0 : slot_in + 1;
+    in = in == smem + (STG - 1) * C::STAGE ? smem : in + C::STAGE;
   };
   // !TR: Q through registers, since its words change places: word p of the 8
-  // columns of lane t goes to tile p, place t; rank rows in fragment order
+  // columns of lane t goes to tile p, place t
   uint4 qv[TR ? 1 : NP];
   auto load_q = [&](int st) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int p = qrow + i * PSTEP, k = k_of_row16(p);
-      qv[i] = p < RP && k < r ? ld8<T, VEC>(Q + (size_t)k * N, n0 + st * SK + q * 8, N) : make_uint4(0, 0, 0, 0);
+      qv[i] = has_q && qin[i] ? ld8<T, VEC>(qsrc[i], 0, N - n0 - st * SK - q * 8) : make_uint4(0, 0, 0, 0);
+      qsrc[i] += SK;
     }
   };
-  auto put_q = [&](int slot) {
-    uint32_t* thin = reinterpret_cast<uint32_t*>(sm + slot * C::STAGE + WIDE);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int p = qrow + i * PSTEP;
-      if (PIECES % THREADS && p >= RP) break;
-      uint32_t* dst = thin + p * (C::PITCH / 4) + (q >> 2) * 16 + (q & 3);
-      dst[0] = qv[i].x;
-      dst[4] = qv[i].y;
-      dst[8] = qv[i].z;
-      dst[12] = qv[i].w;
-    }
+  auto put_q = [&](uint32_t to) {
+    if (has_q)
+      static_for<NP>([&](auto i) {
+        asm volatile("st.shared.u32 [%0+%5], %1;\n\tst.shared.u32 [%0+%5+16], %2;\n\tst.shared.u32 [%0+%5+32], %3;\n\t"
+                     "st.shared.u32 [%0+%5+48], %4;" ::"r"(to + qdst), "r"(qv[i].x), "r"(qv[i].y), "r"(qv[i].z), "r"(qv[i].w),
+                     "n"(i * PSTEP * C::PITCH)
+                     : "memory");
+      });
   };
 #pragma unroll
   for (int i = 0; i < STG - 1; ++i) {
@@ -349,7 +374,12 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
   }
   T* ya = y + (ra >= 0 ? ra : 0) * N + n0 + 8 * t;
   T* yb = y + (rb >= 0 ? rb : 0) * N + n0 + 8 * t;
-  int slot = 0;
+  int left = N - n0 - 8 * t;  // columns of the row from this lane's on
+  // where this lane reads a stage: base's pieces of either 32 columns, and Q's fragments
+  const uint32_t boff[2] = {(uint32_t)(m * ROWB + ((t ^ swz(g)) << 4)), (uint32_t)(m * ROWB + (((4 + t) ^ swz(g)) << 4))};
+  const uint32_t foff = WIDE + (TR ? g * C::PITCH + 8 * t
+                                   : (8 * ((lane >> 3) & 1) + (lane & 7)) * C::PITCH + (lane >> 4) * 16);
+  uint32_t slot = smem;
   for (int st = 0; st < nst; ++st) {
     if constexpr (!TR) put_q(slot);  // this slot's last readers are two barriers back
     cp_async_wait<STG - 2>();
@@ -359,27 +389,20 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
     if constexpr (!TR) {
       if (st + 1 < nst) load_q(st + 1);
     }
-    const uint8_t* buf = sm + slot * C::STAGE;
-    slot = slot + 1 == STG ? 0 : slot + 1;
     if (16 * warp < count) {
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {  // 32 columns each
+      static_for<2>([&](auto w) {  // 32 columns each
         float c[4][4] = {};
-#pragma unroll
-        for (int k = 0; k < RP / 16; ++k) {
+        static_for<RP / 16>([&](auto k) {
           uint32_t b[8];
           if constexpr (!TR) {
-            const uint32_t addr = smem_u32(buf + WIDE + (16 * k + 8 * ((lane >> 3) & 1) + (lane & 7)) * C::PITCH +
-                                           w * 64 + (lane >> 4) * 16);
-            ldmatrix_x4_trans(b, addr);
-            ldmatrix_x4_trans(b + 4, addr + 32);
+            ldmatrix_x4_trans<16 * k * C::PITCH + w * 64>(b, slot + foff);
+            ldmatrix_x4_trans<16 * k * C::PITCH + w * 64 + 32>(b + 4, slot + foff);
           } else {
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-              const uint2 u = *reinterpret_cast<const uint2*>(buf + WIDE + (32 * w + 8 * p + g) * C::PITCH + (16 * k + 4 * t) * 2);
+            static_for<4>([&](auto p) {
+              const uint2 u = lds8<(32 * w + 8 * p) * C::PITCH + 32 * k>(slot + foff);
               b[2 * p] = u.x;
               b[2 * p + 1] = u.y;
-            }
+            });
           }
 #pragma unroll
           for (int p = 0; p < 4; ++p)
@@ -387,18 +410,20 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
 #pragma unroll
           for (int p = 0; p < 4; ++p)
             mma16816<T>(c[p], la[k][0].x, la[k][1].x, la[k][0].y, la[k][1].y, b[2 * p], b[2 * p + 1]);
-        }
-        const int left = N - n0 - st * SK - 32 * w - 8 * t;  // columns of the row from this lane's on
+        });
         uint4 ua = make_uint4(0, 0, 0, 0), ub = ua;
         if (base) {
-          const uint32_t piece = ((4 * w + t) ^ swz(g)) << 4;
-          ua = *reinterpret_cast<const uint4*>(buf + m * ROWB + piece);
-          ub = *reinterpret_cast<const uint4*>(buf + (m + 8) * ROWB + piece);
+          ua = lds16<0>(slot + boff[w]);
+          ub = lds16<8 * ROWB>(slot + boff[w]);
         }
-        if (ra >= 0) st8<T, VEC>(ya + st * SK + 32 * w, 0, left, add8<T>(ua, c, 0, fac[0]));
-        if (rb >= 0) st8<T, VEC>(yb + st * SK + 32 * w, 0, left, add8<T>(ub, c, 2, fac[1]));
-      }
+        if (ra >= 0) st8<T, VEC>(ya + 32 * w, 0, left - 32 * w, add8<T>(ua, c, 0, fac[0]));
+        if (rb >= 0) st8<T, VEC>(yb + 32 * w, 0, left - 32 * w, add8<T>(ub, c, 2, fac[1]));
+      });
     }
+    ya += SK;
+    yb += SK;
+    left -= SK;
+    slot = slot == smem + (STG - 1) * C::STAGE ? smem : slot + C::STAGE;
   }
 }
 
