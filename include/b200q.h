@@ -272,20 +272,24 @@ size_t b200q_lora_plan_bytes(int64_t T, int64_t L);
 int b200q_lora_plan(const int64_t* lora_ids, int64_t T, int64_t L, int32_t* plan, size_t plan_bytes, void* workspace,
                     void* stream);
 
-/* y from x (transposed = 0) or dx from dy (transposed = 1: x is dy [T, N] and
- * y is dx [T, D]).  base: NULL for zeros; may be y itself; a token without an
- * adapter gets base.  y: NULL to compute mid alone.  mid: lo (or dlo), fp32,
- * b200q_lora_mid_bytes(T, r) of it, any contents; rows of tokens without an
- * adapter are left as they were; NULL is enough for y alone at T <= 256. */
+/* y.  base: NULL for zeros; may be y itself; a token without an adapter gets
+ * base.  lo: the row between the two products, for the backward pass:
+ * b200q_lora_mid_bytes(T, r) bytes, any contents; rows of tokens without an
+ * adapter are left as they were.  NULL where T <= 256 and no backward pass
+ * follows. */
 size_t b200q_lora_mid_bytes(int64_t T, int64_t r);
 int b200q_lora_apply(const void* x, const void* base, const void* A, const void* B, const float* scaling,
-                     const int32_t* plan, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype,
-                     int transposed, void* y, float* mid, void* stream);
+                     const int32_t* plan, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype, void* y,
+                     float* lo, void* stream);
 
-/* dA (from x and dlo) and dB (from lo and dy), either NULL to leave it out; an
- * adapter without tokens gets zeros. */
-int b200q_lora_grads(const void* x, const void* dy, const float* lo, const float* dlo, const int32_t* plan, int64_t T,
-                     int64_t D, int64_t N, int64_t r, int64_t L, int dtype, void* dA, void* dB, void* stream);
+/* The gradients of that call: dx (base: added to it, NULL for zeros, may be dx
+ * itself), dA and dB, each NULL to leave it out; an adapter without tokens gets
+ * zeros.  lo as b200q_lora_apply left it; dlo: b200q_lora_mid_bytes(T, r) bytes
+ * of scratch, needed for dx and dA.  The gradient of b200q_lora_apply's base is
+ * dy. */
+int b200q_lora_backward(const void* x, const void* dy, const void* base, const void* A, const void* B,
+                        const float* scaling, const int32_t* plan, const float* lo, int64_t T, int64_t D, int64_t N,
+                        int64_t r, int64_t L, int dtype, float* dlo, void* dx, void* dA, void* dB, void* stream);
 
 /* Grouped W4A16 GEMM over the experts of a MoE layer, one launch for all
  * experts.  x [rows, K] holds every expert's rows contiguously, expert e's at

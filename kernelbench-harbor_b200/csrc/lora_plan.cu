@@ -130,6 +130,10 @@ int launch_grads(const void* x, const void* dy, const float* lo, const float* dl
 // tiled pair.
 constexpr int64_t SMALL_MAX_T = 256;
 
+static int launch(const Args& a, int dtype, bool tr, cudaStream_t st) {
+  return a.T <= SMALL_MAX_T ? launch_small(a, dtype, tr, st) : launch_tiles(a, dtype, tr, st);
+}
+
 static int check_sizes(const char* what, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype) {
   const std::string w(what);
   if (dtype != B200Q_DTYPE_FP16 && dtype != B200Q_DTYPE_BF16)
@@ -183,46 +187,38 @@ size_t b200q_lora_mid_bytes(int64_t T, int64_t r) {
 }
 
 int b200q_lora_apply(const void* x, const void* base, const void* A, const void* B, const float* scaling,
-                     const int32_t* plan, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype,
-                     int transposed, void* y, float* mid, void* stream) {
+                     const int32_t* plan, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype, void* y,
+                     float* lo, void* stream) {
   using namespace b200q;
   using namespace b200q::lora;
   int rc = check_sizes("lora_apply", T, D, N, r, L, dtype);
   if (rc) return rc;
   if (T == 0) return B200Q_OK;
-  if (!x || !A || !B || !plan || (!y && !mid) || (!mid && T > SMALL_MAX_T)) return fail(B200Q_ERR_SHAPE, "lora_apply: null pointer argument");
-  if (misaligned({x, base, A, B, plan, y, mid})) return fail(B200Q_ERR_ALIGN, "lora_apply: pointers must be 16-byte aligned");
-  Args a;
-  a.x = x;
-  a.base = base;
-  a.P = transposed ? B : A;
-  a.Q = transposed ? A : B;
-  a.scaling = scaling;
-  a.plan = plan;
-  a.lay = plan_layout(T, L);
-  a.D = (int)(transposed ? N : D);
-  a.N = (int)(transposed ? D : N);
-  a.r = (int)r;
-  a.mp = mid_pitch(r);
-  a.y = y;
-  a.mid = mid;
-  a.T = T;
-  a.L = L;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return T <= SMALL_MAX_T ? launch_small(a, dtype, transposed != 0, st) : launch_tiles(a, dtype, transposed != 0, st);
+  if (!x || !A || !B || !plan || !y || (!lo && T > SMALL_MAX_T))
+    return fail(B200Q_ERR_SHAPE, "lora_apply: null pointer argument");
+  if (misaligned({x, base, A, B, plan, y, lo})) return fail(B200Q_ERR_ALIGN, "lora_apply: pointers must be 16-byte aligned");
+  const Args a = {x, base, A, B, scaling, plan, plan_layout(T, L), (int)D, (int)N, (int)r, mid_pitch(r), y, lo, T, L};
+  return launch(a, dtype, false, reinterpret_cast<cudaStream_t>(stream));
 }
 
-int b200q_lora_grads(const void* x, const void* dy, const float* lo, const float* dlo, const int32_t* plan, int64_t T,
-                     int64_t D, int64_t N, int64_t r, int64_t L, int dtype, void* dA, void* dB, void* stream) {
+int b200q_lora_backward(const void* x, const void* dy, const void* base, const void* A, const void* B,
+                        const float* scaling, const int32_t* plan, const float* lo, int64_t T, int64_t D, int64_t N,
+                        int64_t r, int64_t L, int dtype, float* dlo, void* dx, void* dA, void* dB, void* stream) {
   using namespace b200q;
   using namespace b200q::lora;
-  int rc = check_sizes("lora_grads", T, D, N, r, L, dtype);
+  int rc = check_sizes("lora_backward", T, D, N, r, L, dtype);
   if (rc) return rc;
-  if ((!dA && !dB) || (T > 0 && (!plan || (dA && (!x || !dlo)) || (dB && (!dy || !lo)))))
-    return fail(B200Q_ERR_SHAPE, "lora_grads: null pointer argument");
-  if (misaligned({x, dy, lo, dlo, plan, dA, dB})) return fail(B200Q_ERR_ALIGN, "lora_grads: pointers must be 16-byte aligned");
-  return launch_grads(x, dy, lo, dlo, plan, plan_layout(T, L), T, D, N, r, L, dtype, dA, dB,
-                      reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool need_dlo = dx || dA;
+  if (T > 0 && (!plan || !dy || (need_dlo && (!A || !B || !dlo)) || (dA && !x) || (dB && !lo)))
+    return fail(B200Q_ERR_SHAPE, "lora_backward: null pointer argument");
+  if (misaligned({x, dy, base, A, B, plan, lo, dlo, dx, dA, dB}))
+    return fail(B200Q_ERR_ALIGN, "lora_backward: pointers must be 16-byte aligned");
+  if (T > 0 && need_dlo) {
+    const Args a = {dy, base, B, A, scaling, plan, plan_layout(T, L), (int)N, (int)D, (int)r, mid_pitch(r), dx, dlo, T, L};
+    if ((rc = launch(a, dtype, true, st))) return rc;
+  }
+  return dA || dB ? launch_grads(x, dy, lo, dlo, plan, plan_layout(T, L), T, D, N, r, L, dtype, dA, dB, st) : B200Q_OK;
 }
 
 }  // extern "C"

@@ -86,6 +86,12 @@ def _once(backward, ctx, *grads):
     return backward(ctx, *grads)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    return pa < pb + b.numel() * b.element_size() and pb < pa + a.numel() * a.element_size()
+
+
 def _same_device(op: str, first: torch.Tensor, *rest: Optional[torch.Tensor]) -> None:
     for t in rest:
         if t is not None and t.device != first.device:
@@ -167,13 +173,13 @@ def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, z
 
 def _w4a16_setup(ctx, inputs, output):
     x, qweight, scales, zeros, group = inputs
-    if scales.requires_grad or zeros.requires_grad:
-        raise ValueError("w4a16_gemm: the quantised weight is frozen, scales and zeros have no gradient")
     ctx.save_for_backward(qweight, scales, zeros)
     ctx.group = group
 
 
 def _w4a16_backward(ctx, dy):
+    if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+        raise RuntimeError("w4a16_gemm: the quantised weight is frozen, scales and zeros have no gradient")
     qweight, scales, zeros = ctx.saved_tensors
     dx = w4a16_dgrad(dy, qweight, scales, zeros, ctx.group) if ctx.needs_input_grad[0] else None
     return dx, None, None, None, None
@@ -409,6 +415,8 @@ def moe_balance_loss(router_logits: torch.Tensor, topi: torch.Tensor,
         if token_mask.dtype != torch.bool or tuple(token_mask.shape) != (router_logits.shape[0],):
             raise ValueError("token_mask must be bool [T]")
         token_mask = token_mask.contiguous()
+    if topi.dtype == torch.int64:  # what 32 bits do not hold stays out of range
+        topi = topi.clamp(-2, router_logits.shape[1])
     topi = topi.to(torch.int32).contiguous()
     if torch.is_grad_enabled() and router_logits.requires_grad:
         return _BalanceLoss.apply(router_logits, topi, token_mask)
@@ -563,7 +571,7 @@ def lora_expand_add(base: torch.Tensor, lo: torch.Tensor, B: torch.Tensor, lora_
     return y
 
 
-_LORA_SMALL = 256  # tokens up to which b200q_lora_apply takes mid = NULL
+_LORA_SMALL = 256  # tokens up to which b200q_lora_apply takes lo = NULL
 
 
 class LoraPlan:
@@ -597,15 +605,14 @@ def lora_plan(lora_ids: torch.Tensor, n_adapters: int) -> LoraPlan:
     return LoraPlan(data, T, n_adapters)
 
 
-def _lora_run(x, base, A, B, scaling, plan, transposed, out, mid):
-    """One lora_apply call on contiguous, aligned tensors (see include/b200q.h)."""
+def _lora_run(x, base, A, B, scaling, plan, out, lo):
+    """One b200q_lora_apply call on contiguous, aligned tensors."""
     n_adapters, D, r = A.shape
     dev = x.device
     with _device(dev):
         _lib.check(_lib.lib().b200q_lora_apply(x.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling),
                                                plan.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters,
-                                               _dtype_code(x.dtype), transposed, _ptr(out), _ptr(mid),
-                                               _stream_ptr(dev)))
+                                               _dtype_code(x.dtype), out.data_ptr(), _ptr(lo), _stream_ptr(dev)))
 
 
 def _lora_mid(x: torch.Tensor, r: int) -> torch.Tensor:
@@ -617,8 +624,9 @@ class _LoraApply(torch.autograd.Function):
     def forward(ctx, base, x, A, B, scaling, plan):
         base, x, A, B = _aligned(base), _aligned(x), _aligned(A), _aligned(B)
         y, lo = torch.empty_like(base), _lora_mid(x, A.shape[2])
-        _lora_run(x, base, A, B, scaling, plan, 0, y, lo)
-        ctx.save_for_backward(x, A, B, scaling, plan, lo)
+        _lora_run(x, base, A, B, scaling, plan.data, y, lo)
+        ctx.save_for_backward(x, A, B, scaling)
+        ctx.lo, ctx.plan = lo, plan.data  # seen by nobody else
         return y
 
     @staticmethod
@@ -627,22 +635,23 @@ class _LoraApply(torch.autograd.Function):
 
 
 def _lora_backward(ctx, dy):
-    x, A, B, scaling, plan, lo = ctx.saved_tensors
-    need = ctx.needs_input_grad
+    x, A, B, scaling = ctx.saved_tensors
+    lo = ctx.lo
+    need_base, need_x, need_A, need_B = ctx.needs_input_grad[:4]
+    dev = x.device
     d = _aligned(dy)
-    dx = dlo = dA = dB = None
-    if need[1] or need[2]:
-        dx, dlo = torch.empty_like(x) if need[1] else None, torch.empty_like(lo)
-        _lora_run(d, None, A, B, scaling, plan, 1, dx, dlo)
-    if need[2] or need[3]:
-        dA = torch.empty_like(A) if need[2] else None
-        dB = torch.empty_like(B) if need[3] else None
+    dx = torch.empty_like(x) if need_x else None
+    dA = torch.empty_like(A) if need_A else None
+    dB = torch.empty_like(B) if need_B else None
+    dlo = torch.empty_like(lo) if need_x or need_A else None
+    if need_x or need_A or need_B:
         n_adapters, D, r = A.shape
-        with _device(x.device):
-            _lib.check(_lib.lib().b200q_lora_grads(x.data_ptr(), d.data_ptr(), lo.data_ptr(), _ptr(dlo),
-                                                   plan.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters,
-                                                   _dtype_code(x.dtype), _ptr(dA), _ptr(dB), _stream_ptr(x.device)))
-    return dy if need[0] else None, dx, dA, dB, None, None
+        with _device(dev):
+            _lib.check(_lib.lib().b200q_lora_backward(
+                x.data_ptr(), d.data_ptr(), None, A.data_ptr(), B.data_ptr(), _ptr(scaling), ctx.plan.data_ptr(),
+                lo.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters, _dtype_code(x.dtype), _ptr(dlo), _ptr(dx),
+                _ptr(dA), _ptr(dB), _stream_ptr(dev)))
+    return dy if need_base else None, dx, dA, dB, None, None
 
 
 def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
@@ -691,8 +700,9 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     if torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad or base.requires_grad):
         if out is not None:
             raise ValueError("lora_apply: out cannot be given where a gradient is wanted")
-        return _LoraApply.apply(base, x, A, B, scaling, plan.data)
-    if out is None:
+        return _LoraApply.apply(base, x, A, B, scaling, plan)
+    out_given = out is not None
+    if not out_given:
         base = _aligned(base)
         out = torch.empty_like(base)
     else:
@@ -700,10 +710,12 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
             raise ValueError("lora_apply: out must be a contiguous, 16-byte aligned [T, N] tensor of x's dtype")
         if out is not base:
             base = _aligned(base)
-    x = _aligned(x)
+    x, A, B = _aligned(x), _aligned(A), _aligned(B)
+    if out_given and (any(_overlap(out, t) for t in (x, A, B)) or (out.data_ptr() != base.data_ptr() and _overlap(out, base))):
+        raise ValueError("lora_apply: out shares memory with an input (it may be base itself)")
     # the one-launch kernel needs no room for the row between
-    mid = None if T <= _LORA_SMALL else _lora_mid(x, r)
-    _lora_run(x, base, _aligned(A), _aligned(B), scaling, plan.data, 0, out, mid)
+    lo = None if T <= _LORA_SMALL else _lora_mid(x, r)
+    _lora_run(x, base, A, B, scaling, plan.data, out, lo)
     return out
 
 

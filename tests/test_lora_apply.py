@@ -148,7 +148,7 @@ def test_ids_out_of_range_count_as_none():
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("T,D,N,r,L,kind", [
-    (1, 64, 64, 8, 1, "one"), (1, 4096, 4096, 16, 8, "one"), (1, 128, 256, 64, 2, "none"), (3, 32, 8, 1, 2, "mixed"),
+    (1, 64, 64, 8, 1, "one"), (5, 8, 8, 8, 2, "mixed"), (260, 8, 16, 8, 2, "runs"), (1, 4096, 4096, 16, 8, "one"), (1, 128, 256, 64, 2, "none"), (3, 32, 8, 1, 2, "mixed"),
     (16, 264, 40, 16, 1, "one"), (17, 4096, 1408, 16, 2, "one"), (64, 512, 768, 32, 64, "mixed"),
     (64, 4096, 4096, 16, 8, "mixed"), (100, 257, 129, 33, 3, "mixed"), (129, 1000, 264, 64, 2, "runs"),
     (256, 2048, 512, 24, 5, "runs"), (257, 128, 128, 16, 3, "runs"), (300, 4100, 64, 12, 2, "mixed"),
@@ -280,6 +280,16 @@ def test_gradients_one_at_a_time():
         kw = {**c, name: leaf}
         (g,) = torch.autograd.grad(ops.lora_apply(kw["base"], kw["x"], kw["A"], kw["B"], c["ids"], c["scaling"]), leaf, c["dy"])
         assert torch.equal(g, want)
+
+
+@pytest.mark.gpu
+def test_once_differentiable():
+    c = inputs(40, 64, 64, 8, 2, "bf16", "runs")
+    A = c["A"].float().requires_grad_()
+    y = ops.lora_apply(c["base"], c["x"], A, c["B"], c["ids"], c["scaling"])
+    (g,) = torch.autograd.grad(y.float().square().sum(), A, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.square().sum().backward()
 
 
 @pytest.mark.gpu
@@ -433,20 +443,22 @@ def test_refusals_without_gpu():
     assert L.b200q_lora_plan(p, 64, 8, 20, n, None, None) == _lib.ERR_ALIGN
     assert L.b200q_lora_plan(p, 64, 0, p, n, None, None) == L.b200q_lora_plan(p, (1 << 24) + 1, 8, p, n, None, None) == _lib.ERR_SHAPE
 
-    def call(T=64, D=64, N=64, r=8, nl=4, dtype=0, x=p, y=p, mid=p):
-        return L.b200q_lora_apply(x, p, p, p, None, p, T, D, N, r, nl, dtype, 0, y, mid, None)
+    def call(T=64, D=64, N=64, r=8, nl=4, dtype=0, x=p, y=p, lo=p):
+        return L.b200q_lora_apply(x, p, p, p, None, p, T, D, N, r, nl, dtype, y, lo, None)
 
     assert call(r=65) == call(r=0) == call(D=0) == call(N=1 << 23) == call(nl=1024) == call(T=-1) == _lib.ERR_SHAPE
-    assert call(x=None) == call(mid=None, T=257) == call(mid=None, y=None) == _lib.ERR_SHAPE
+    assert call(x=None) == call(lo=None, T=257) == call(y=None) == _lib.ERR_SHAPE
     assert call(y=24) == call(x=8) == _lib.ERR_ALIGN
     assert call(dtype=2) == _lib.ERR_UNSUPPORTED
     assert call(T=0) == _lib.OK
 
-    def grads(T=64, r=8, x=p, dA=p, dB=p, lo=p, dlo=p):
-        return L.b200q_lora_grads(x, p, lo, dlo, p, T, 64, 64, r, 4, 0, dA, dB, None)
+    def back(T=64, r=8, x=p, dy=p, A=p, dx=p, dA=p, dB=p, lo=p, dlo=p):
+        return L.b200q_lora_backward(x, dy, None, A, p, None, p, lo, T, 64, 64, r, 4, 0, dlo, dx, dA, dB, None)
 
-    assert grads(dA=None, dB=None) == grads(x=None) == grads(lo=None) == grads(dlo=None) == grads(r=65) == _lib.ERR_SHAPE
-    assert grads(dB=8) == _lib.ERR_ALIGN
+    assert back(x=None) == back(dy=None) == back(A=None) == back(lo=None) == back(r=65) == _lib.ERR_SHAPE
+    assert back(dlo=None) == back(dlo=None, dA=None, dB=None) == _lib.ERR_SHAPE
+    assert back(dB=8) == back(dx=4) == _lib.ERR_ALIGN
+    assert back(dx=None, dA=None, dB=None) == back(T=0, dA=None, dB=None) == _lib.OK
 
 
 @pytest.mark.gpu
@@ -454,6 +466,7 @@ def test_refusals():
     c = inputs(10, 64, 32, 8, 2, "fp16", "mixed")
     base, x, A, B, ids, s = (c[k] for k in ("base", "x", "A", "B", "ids", "scaling"))
     plan = ops.lora_plan(ids, 2)
+    big = torch.zeros(400, dtype=torch.float16, device="cuda")
     for args, err in [((base, x[:, :32], A, B, plan), ValueError), ((base[:5], x, A, B, plan), ValueError),
                       ((base, x, A, B[:1], plan), ValueError), ((base, x, A, B[:, :4], plan), ValueError),
                       ((base.bfloat16(), x, A, B, plan), TypeError), ((base.float(), x.float(), A, B, plan), TypeError),
@@ -463,6 +476,8 @@ def test_refusals():
                       ((base, x, A, B, plan, s.clone().requires_grad_()), ValueError),
                       ((base, x, A, B, plan, s, base[:, :16]), ValueError), ((base, x, A, B, plan, s, base.t()), ValueError),
                       ((base, x, A.clone().requires_grad_(), B, plan, s, base), ValueError),
+                      ((base, x, A, B, plan, s, x.view(-1)[:320].view(10, 32)), ValueError),
+                      ((big[:320].view(10, 32), x, A, B, plan, s, big[32:352].view(10, 32)), ValueError),
                       ((base, x[0], A, B, plan), ValueError)]:
         with pytest.raises(err):
             ops.lora_apply(*args)

@@ -143,6 +143,25 @@ def test_index_out_of_range_sets_the_status():
     check(logits, topi, None)
     assert ops.device_status() & 2
     assert ops.device_status() == 0
+    wide = topi.long()
+    wide[4, 0] = 2 ** 32 + 1  # not expert 1
+    wide[5, 1] = -2 ** 40
+    _, counts = ops.moe_balance_loss(logits, wide)
+    assert torch.equal(counts.long(), definition(logits, wide, None)[1])
+    assert ops.device_status() & 2
+
+
+@pytest.mark.gpu
+def test_gradient_twice_and_once_differentiable():
+    """A retained graph gives the same gradient again; the gradient itself has none."""
+    logits, topi, mask = inputs(50, 8, 2, "fp32", seed=21, masked=0.2)
+    lg = logits.requires_grad_()
+    loss, _ = ops.moe_balance_loss(lg, topi, mask)
+    (d1,) = torch.autograd.grad(loss, lg, retain_graph=True)
+    (d2,) = torch.autograd.grad(3 * loss, lg, create_graph=True)
+    torch.testing.assert_close(d2, 3 * d1, rtol=2 ** -22, atol=0)
+    with pytest.raises(RuntimeError):
+        d2.square().sum().backward()
 
 
 @pytest.mark.gpu

@@ -154,5 +154,7 @@ def test_refusals():
         with pytest.raises(err):
             ops.w4a16_dgrad(*args)
     x = torch.zeros(4, 128, dtype=torch.float16, device="cuda", requires_grad=True)
-    with pytest.raises(ValueError, match="frozen"):
-        ops.w4a16_gemm(x, q, s.clone().requires_grad_(), z, 128)
+    # scales that ask for a gradient run forward, as before, and have none
+    y = ops.w4a16_gemm(x, q, s.clone().requires_grad_(), z, 128)
+    with pytest.raises(RuntimeError, match="frozen"):
+        y.sum().backward()
