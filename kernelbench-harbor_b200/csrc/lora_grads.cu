@@ -44,11 +44,12 @@ struct GradArgs {
   const int32_t* plan;
   PlanLayout lay;
   int D, N, r, mp, nbd;
+  int64_t T;
   void *dA, *dB;
 };
 
 template <class T, int RP, bool VEC>
-__global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 1) lora_grads_kernel(const GradArgs a, int S) {
+__global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 2) lora_grads_kernel(const GradArgs a, int S) {
   using C = GradCfg<RP>;
   constexpr int GSTG = C::GSTG;
   constexpr bool F16 = std::is_same<T, __half>::value;
@@ -77,14 +78,24 @@ __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 1) lora_gra
   };
   const T* wcol = wide + w0 + (tid & 15) * 8;
   const int wleft = W - w0 - (tid & 15) * 8;
+  uint4 wv[VEC ? 1 : TK / 16];  // rows of any alignment: to registers a stage ahead, then to the ring
   auto stage_wide = [&](int st) {
     // this thread's 16 bytes of rows tid / 16 + 16 i
     const uint32_t dst = smem_u32(sm) + st % GSTG * (TK * WPITCH) + (tid >> 4) * WPITCH + (tid & 15) * 16;
     const int* toks = &s_tok[st % TOKS][tid >> 4];
     static_for<TK / 16>([&](auto i) {
       const int tok = toks[16 * i];
-      stage16<T, VEC, true, 16 * i * WPITCH>(dst, wcol + (size_t)max(tok, 0) * W, wleft, tok >= 0, wide);
+      if constexpr (VEC)
+        copy16<true, 16 * i * WPITCH>(dst, wcol + (size_t)max(tok, 0) * W, wleft, tok >= 0, wide);
+      else
+        wv[i] = tok >= 0 ? ld8_any<T>(wcol + (size_t)tok * W, wleft, wide + a.T * W) : make_uint4(0, 0, 0, 0);
     });
+  };
+  auto put_wide = [&](int st) {
+    if constexpr (!VEC) {
+      const uint32_t dst = smem_u32(sm) + st % GSTG * (TK * WPITCH) + (tid >> 4) * WPITCH + (tid & 15) * 16;
+      static_for<TK / 16>([&](auto i) { sts16<16 * i * WPITCH>(dst, wv[i]); });
+    }
   };
   float4 tv[C::VPT];
   auto load_thin = [&](int st) {
@@ -92,8 +103,8 @@ __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 1) lora_gra
     for (int i = 0; i < C::VPT; ++i) {
       const int idx = tid + i * THREADS, row = idx / (RP / 4), col = idx % (RP / 4) * 4;
       const int tok = s_tok[st % TOKS][row];
-      tv[i] = tok >= 0 && (VEC || col < a.mp) ? *reinterpret_cast<const float4*>(thin + (size_t)tok * a.mp + col)
-                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+      tv[i] = tok >= 0 ? *reinterpret_cast<const float4*>(thin + (size_t)tok * a.mp + col)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
   auto note_max = [&](int st) {  // fp16: the largest exponent of the finite values in tv
@@ -151,10 +162,16 @@ __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 1) lora_gra
   float rescale = 1.f;
   if (nst > 0) {
     load_thin(0);
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < GSTG - 1; ++i) {
-      if (i < nst) stage_wide(i);
-      cp_async_commit();
+      for (int i = 0; i < GSTG - 1; ++i) {
+        if (i < nst) stage_wide(i);
+        cp_async_commit();
+      }
+    } else {
+      stage_wide(0);
+      put_wide(0);
+      if (nst > 1) stage_wide(1);
     }
     if (F16) {
       note_max(0);
@@ -170,8 +187,13 @@ __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 1) lora_gra
     rescale = 1.f;
     if (st + 1 < nst) rescale = put_thin(st + 1);
     if (F16 && tid == 0) s_max[(st + 3) & 3] = 0;  // next used by note_max(st + 3), a barrier from here
-    if (st + GSTG - 1 < nst) stage_wide(st + GSTG - 1);
-    cp_async_commit();
+    if constexpr (VEC) {
+      if (st + GSTG - 1 < nst) stage_wide(st + GSTG - 1);
+      cp_async_commit();
+    } else {
+      if (st + 1 < nst) put_wide(st + 1);
+      if (st + 2 < nst) stage_wide(st + 2);
+    }
     if (st + 2 < nst) load_thin(st + 2);
     if (tid < TK) load_tokens(st + GSTG + 1);
     // A: thin^T (rank rows), B: wide (this warp's 32 columns), k: this warp's half of the tokens
@@ -260,11 +282,11 @@ int launch_grads(const void* x, const void* dy, const float* lo, const float* dl
   }
   GradArgs a;
   a.x = x, a.dy = dy, a.lo = lo, a.dlo = dlo, a.plan = plan, a.lay = lay;
-  a.D = (int)D, a.N = (int)N, a.r = (int)r, a.mp = mid_pitch(r);
+  a.D = (int)D, a.N = (int)N, a.r = (int)r, a.mp = mid_pitch(r), a.T = T_;
   a.nbd = dA ? (int)((D + CT - 1) / CT) : 0;
   const int nbn = dB ? (int)((N + CT - 1) / CT) : 0;
   a.dA = dA, a.dB = dB;
-  const bool vec = D % 8 == 0 && N % 8 == 0 && r % 8 == 0;
+  const bool vec = aligned_widths(D, N, r);
   return by_type(dtype, r, vec, [&](auto tc, auto rc, auto vc) -> int {
     using T = decltype(tc);
     constexpr int RP = decltype(rc)::value;

@@ -184,6 +184,10 @@ template <int OFF = 0>
 __device__ __forceinline__ void cp_async16_ahead(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0+%3], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(OFF) : "memory");
 }
+template <int OFF = 0>
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0+%3], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(OFF) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -191,22 +195,57 @@ __device__ __forceinline__ void cp_async_wait() {
 }
 
 // ------------------------------------------------------------------ rows of any width
-// Values [k, k + 8) of a row of K, zeros past its end.  VEC: K % 8 == 0 and
-// 16-byte aligned rows, k a multiple of 8: all in or all out.
-template <class T, bool VEC>
-__device__ __forceinline__ uint4 ld8(const T* row, int k, int K) {
-  if constexpr (VEC) {
-    return k < K ? __ldg(reinterpret_cast<const uint4*>(row + k)) : make_uint4(0, 0, 0, 0);
-  } else {
-    uint32_t w[4];
+// VEC: widths and pointers let every piece of a wide row be one aligned 16-byte
+// access (D % 8 == 0, N % 8 == 0, and r % 4 == 0, so that A's rows come in
+// 8-byte pieces at least).  Otherwise a row may start at any value: 8 values are
+// cut out of the one or two aligned 16-byte blocks that hold them, or read one
+// by one where such a block would reach past the tensor's end.
+
+// Up to 8 values from p on, zeros past `left`; `end`: the tensor's end.
+template <class T>
+__device__ __forceinline__ uint4 ld8_any(const T* p, int left, const T* end) {
+  if (left <= 0) return make_uint4(0, 0, 0, 0);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p), lo = at & ~(uintptr_t)15;
+  const int shift = (int)(at & 15);
+  const bool two = shift && 2 * min(left, 8) > 16 - shift;
+  uint32_t w[8];
+  if (lo + (two ? 32 : 16) <= reinterpret_cast<uintptr_t>(end)) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(lo));
+    const uint4 b = two ? __ldg(reinterpret_cast<const uint4*>(lo) + 1) : make_uint4(0, 0, 0, 0);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    if (shift & 8) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (shift & 4) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    if (shift & 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t a = k + 2 * i < K ? reinterpret_cast<const uint16_t*>(row)[k + 2 * i] : 0;
-      const uint32_t b = k + 2 * i + 1 < K ? reinterpret_cast<const uint16_t*>(row)[k + 2 * i + 1] : 0;
-      w[i] = a | (b << 16);
+      if (left <= 2 * i) w[i] = 0;
+      if (left == 2 * i + 1) w[i] &= 0xffffu;
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = (2 * i < left ? (uint32_t)h[2 * i] : 0) | (2 * i + 1 < left ? (uint32_t)h[2 * i + 1] << 16 : 0);
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Values [k, k + 8) of a row of K, zeros past its end (VEC: k a multiple of 8, all in or all out).
+template <class T, bool VEC>
+__device__ __forceinline__ uint4 ld8(const T* row, int k, int K, const T* end) {
+  if constexpr (VEC)
+    return k < K ? __ldg(reinterpret_cast<const uint4*>(row + k)) : make_uint4(0, 0, 0, 0);
+  else
+    return ld8_any<T>(row + k, K - k, end);
 }
 
 template <class T, bool VEC>
@@ -225,29 +264,51 @@ __device__ __forceinline__ uint2 ld4(const T* row, int k, int K) {
   }
 }
 
+// 8 values to p, as many of them as are `left` in the row; otherwise in aligned pairs.
 template <class T, bool VEC>
-__device__ __forceinline__ void st8(T* row, int k, int K, const uint4 v) {
+__device__ __forceinline__ void st8(T* p, int left, const uint4 v) {
   if constexpr (VEC) {
-    if (k < K) *reinterpret_cast<uint4*>(row + k) = v;
+    if (left > 0) *reinterpret_cast<uint4*>(p) = v;
   } else {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint16_t* h = reinterpret_cast<uint16_t*>(p);
+    if (left >= 8) {
+      if (reinterpret_cast<uintptr_t>(p) & 2) {
+        h[0] = (uint16_t)w[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (k + i < K) reinterpret_cast<uint16_t*>(row)[k + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        for (int i = 0; i < 3; ++i) *reinterpret_cast<uint32_t*>(h + 1 + 2 * i) = __funnelshift_r(w[i], w[i + 1], 16);
+        h[7] = (uint16_t)(w[3] >> 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(h + 2 * i) = w[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) h[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
   }
 }
 
-// 16 bytes of a row into shared memory: asynchronous where alignment allows.
-// `left`: values of the row from the piece on; `any`: an address that may be read.
-template <class T, bool VEC, bool WIDE_ROW = false, int OFF = 0>
-__device__ __forceinline__ void stage16(uint32_t dst, const T* piece, int left, bool in, const T* any) {
-  if constexpr (VEC && WIDE_ROW) {
-    cp_async16_ahead<OFF>(dst, in && left > 0 ? piece : any, in && left > 0 ? 16 : 0);
-  } else if constexpr (VEC) {
-    cp_async16<OFF>(dst, in && left > 0 ? piece : any, in && left > 0 ? 16 : 0);
+template <int OFF = 0>
+__device__ __forceinline__ void sts16(uint32_t dst, const uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0+%5], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "n"(OFF) : "memory");
+}
+
+// Up to 16 aligned bytes of a row to shared memory, asynchronously, zeros for the
+// rest (VEC).  `left`: values of the row from the piece on; `any`: an address
+// that may be read.  halves: the row is 8-byte aligned only (A where r % 8 == 4).
+template <bool WIDE_ROW, int OFF, class T>
+__device__ __forceinline__ void copy16(uint32_t dst, const T* piece, int left, bool in, const T* any, bool halves = false) {
+  const bool a = in && left > 0;
+  if (WIDE_ROW) {
+    cp_async16_ahead<OFF>(dst, a ? piece : any, a ? 16 : 0);
+  } else if (!halves) {
+    cp_async16<OFF>(dst, a ? piece : any, a ? 16 : 0);
   } else {
-    const uint4 v = in ? ld8<T, false>(piece, 0, left) : make_uint4(0, 0, 0, 0);
-    asm volatile("st.shared.v4.u32 [%0+%5], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "n"(OFF) : "memory");
+    const bool b = in && left > 4;
+    cp_async8<OFF>(dst, a ? piece : any, a ? 8 : 0);
+    cp_async8<OFF + 8>(dst, b ? piece + 4 : any, b ? 8 : 0);
   }
 }
 
@@ -273,13 +334,14 @@ __device__ __forceinline__ int k_of_row16(int p) { return (p & ~15) | (((p >> 1)
 
 // Rows [0, count) of a tile without an adapter: y = base (zeros without one), columns [n0, n1).
 template <class T, bool VEC>
-__device__ __forceinline__ void copy_rows(const T* base, T* y, const int32_t* rows, int count, int N, int n0, int n1) {
+__device__ __forceinline__ void copy_rows(const T* base, T* y, const int32_t* rows, int count, int N, int n0, int n1,
+                                          const T* end) {
   if (base == y) return;
   const int g8 = (n1 - n0 + 7) / 8;
   for (int i = threadIdx.x; i < count * g8; i += THREADS) {
     const size_t off = (size_t)rows[i / g8] * N;
     const int n = n0 + i % g8 * 8;
-    st8<T, VEC>(y + off, n, n1, base ? ld8<T, VEC>(base + off, n, N) : make_uint4(0, 0, 0, 0));
+    st8<T, VEC>(y + off + n, n1 - n, base ? ld8<T, VEC>(base + off, n, N, end) : make_uint4(0, 0, 0, 0));
   }
 }
 
@@ -297,15 +359,16 @@ struct Args {
 int launch_small(const Args& a, int dtype, bool tr, cudaStream_t st);
 int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st);
 
-// Calls f(type, rank, aligned) with compile-time values; widths or ranks that
-// are not multiples of 8 take the general variant, built for the largest rank only.
+inline bool aligned_widths(int64_t D, int64_t N, int64_t r) { return D % 8 == 0 && N % 8 == 0 && r % 4 == 0; }
+
+// Calls f(type, rank, aligned) with compile-time values.
 template <class F>
 int by_type(int dtype, int64_t r, bool vec, F f) {
   auto rank = [&](auto t) {
-    if (!vec) return f(t, std::integral_constant<int, 64>{}, std::false_type{});
-    if (r <= 16) return f(t, std::integral_constant<int, 16>{}, std::true_type{});
-    if (r <= 32) return f(t, std::integral_constant<int, 32>{}, std::true_type{});
-    return f(t, std::integral_constant<int, 64>{}, std::true_type{});
+    auto width = [&](auto rc) { return vec ? f(t, rc, std::true_type{}) : f(t, rc, std::false_type{}); };
+    if (r <= 16) return width(std::integral_constant<int, 16>{});
+    if (r <= 32) return width(std::integral_constant<int, 32>{});
+    return width(std::integral_constant<int, 64>{});
   };
   return dtype == B200Q_DTYPE_FP16 ? rank(__half{}) : rank(__nv_bfloat16{});
 }

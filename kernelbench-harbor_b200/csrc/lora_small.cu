@@ -49,26 +49,28 @@ __global__ void __launch_bounds__(THREADS) lora_small_kernel(const Args a) {
   const int ng = (N + 31) / 32;  // 32-column groups; this CTA's are [g0, g1)
   const int g0 = rank * ng / CL, g1 = (rank + 1) * ng / CL;
   if (tl.x < 0) {
-    if (y) copy_rows<T, VEC>(base, y, rows, count, N, g0 * 32, min(g1 * 32, N));
+    if (y) copy_rows<T, VEC>(base, y, rows, count, N, g0 * 32, min(g1 * 32, N), base + a.T * N);
     return;
   }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int64_t ra = g < count ? rows[g] : -1, rb = g + 8 < count ? rows[g + 8] : -1;
   const T* P = reinterpret_cast<const T*>(a.P) + (size_t)tl.x * D * r;
   const T* Q = reinterpret_cast<const T*>(a.Q) + (size_t)tl.x * r * N;
+  const T* const p_end = reinterpret_cast<const T*>(a.P) + a.L * D * r;
+  const T* const q_end = reinterpret_cast<const T*>(a.Q) + a.L * N * r;
 
   // ---------------------------------------------------------------- first expand group: loads in flight early
   uint4 bv[2], qv[TR ? 1 : RP / 8];
   uint2 qt[TR ? RP / 16 : 1][4];
   auto load_group = [&](int q) {
     const int n = q * 32 + 8 * t;
-    bv[0] = base && ra >= 0 ? ld8<T, VEC>(base + ra * N, n, N) : make_uint4(0, 0, 0, 0);
-    bv[1] = base && rb >= 0 ? ld8<T, VEC>(base + rb * N, n, N) : make_uint4(0, 0, 0, 0);
+    bv[0] = base && ra >= 0 ? ld8<T, VEC>(base + ra * N, n, N, base + a.T * N) : make_uint4(0, 0, 0, 0);
+    bv[1] = base && rb >= 0 ? ld8<T, VEC>(base + rb * N, n, N, base + a.T * N) : make_uint4(0, 0, 0, 0);
     if constexpr (!TR) {
 #pragma unroll
       for (int i = 0; i < RP / 8; ++i) {  // rank rows in fragment order, 4 lanes per row
         const int k = k_of_row16(i * 8 + g);
-        qv[i] = k < r ? ld8<T, VEC>(Q + (size_t)k * N, n, N) : make_uint4(0, 0, 0, 0);
+        qv[i] = k < r ? ld8<T, VEC>(Q + (size_t)k * N, n, N, q_end) : make_uint4(0, 0, 0, 0);
       }
     } else {
 #pragma unroll
@@ -91,28 +93,43 @@ __global__ void __launch_bounds__(THREADS) lora_small_kernel(const Args a) {
   uint4 xv[2], pv[TR ? RP / 8 : 1];
   auto load_x = [&](int c) {
     const int k = 32 * c + 8 * t;
-    xv[0] = ra >= 0 ? ld8<T, VEC>(x + ra * D, k, D) : make_uint4(0, 0, 0, 0);
-    xv[1] = rb >= 0 ? ld8<T, VEC>(x + rb * D, k, D) : make_uint4(0, 0, 0, 0);
+    xv[0] = ra >= 0 ? ld8<T, VEC>(x + ra * D, k, D, x + a.T * D) : make_uint4(0, 0, 0, 0);
+    xv[1] = rb >= 0 ? ld8<T, VEC>(x + rb * D, k, D, x + a.T * D) : make_uint4(0, 0, 0, 0);
     if (TR) {
 #pragma unroll
       for (int j = 0; j < RP / 8; ++j)
-        pv[j] = 8 * j + g < r ? ld8<T, VEC>(P + (size_t)(8 * j + g) * D, k, D) : make_uint4(0, 0, 0, 0);
+        pv[j] = 8 * j + g < r ? ld8<T, VEC>(P + (size_t)(8 * j + g) * D, k, D, p_end) : make_uint4(0, 0, 0, 0);
     }
   };
-  auto stage_p = [&](int c, int s) {  // 32 contraction rows of P
+  // 32 contraction rows of P: to the ring by asynchronous copies (VEC), else to registers and from there
+  uint4 pq[TR || VEC ? 1 : RP / 8];
+  auto stage_p = [&](int c, int s) {
     if constexpr (!TR) {
 #pragma unroll
       for (int i = 0; i < RP / 8; ++i) {
+        const int idx = lane + 32 * i, k = idx / (RP / 8), pc = idx % (RP / 8), kk = 32 * c + k;
+        const T* piece = P + (size_t)kk * r + pc * 8;
+        if constexpr (VEC)
+          copy16<false, 0>(smem_u32(ring + s * 32 * C::PITCH + row32(k) * C::PITCH + pc * 16), piece, r - pc * 8, kk < D, P,
+                           r % 8 != 0);
+        else
+          pq[i] = kk < D ? ld8_any<T>(piece, r - pc * 8, p_end) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  auto put_p = [&](int s) {
+    if constexpr (!TR && !VEC) {
+#pragma unroll
+      for (int i = 0; i < RP / 8; ++i) {
         const int idx = lane + 32 * i, k = idx / (RP / 8), pc = idx % (RP / 8);
-        const int kk = 32 * c + k;
-        stage16<T, VEC>(smem_u32(ring + s * 32 * C::PITCH + row32(k) * C::PITCH + pc * 16), P + (size_t)kk * r + pc * 8,
-                        r - pc * 8, kk < D, P);
+        sts16(smem_u32(ring + s * 32 * C::PITCH + row32(k) * C::PITCH + pc * 16), pq[i]);
       }
     }
   };
   const int c0 = rank * nch / CL + warp;
+  constexpr int AHEAD = VEC ? STAGES - 1 : 1;  // chunks of P requested before they are used
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
+  for (int s = 0; s < AHEAD; ++s) {
     if (c0 + s * WARPS < c1) stage_p(c0 + s * WARPS, s);
     cp_async_commit();
   }
@@ -125,10 +142,16 @@ __global__ void __launch_bounds__(THREADS) lora_small_kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < RP / 8; ++j) pc_[j] = pv[j];
     }
-    if (c + WARPS < c1) load_x(c + WARPS);
     if (!TR) {
-      cp_async_wait<STAGES - 2>();
+      if (VEC)
+        cp_async_wait<STAGES - 2>();
+      else
+        put_p(s);
       __syncwarp();
+    }
+    if (c + WARPS < c1) {
+      load_x(c + WARPS);
+      if (!VEC) stage_p(c + WARPS, 0);
     }
     const uint32_t row = smem_u32(ring + s * 32 * C::PITCH + lane * C::PITCH);
 #pragma unroll
@@ -144,9 +167,11 @@ __global__ void __launch_bounds__(THREADS) lora_small_kernel(const Args a) {
     }
     if (!TR) {
       __syncwarp();  // every lane has read the slot that is filled next
-      const int cn = c + (STAGES - 1) * WARPS;
-      if (cn < c1) stage_p(cn, s == 0 ? STAGES - 1 : s - 1);
-      cp_async_commit();
+      if (VEC) {
+        const int cn = c + (STAGES - 1) * WARPS;
+        if (cn < c1) stage_p(cn, s == 0 ? STAGES - 1 : s - 1);
+        cp_async_commit();
+      }
       s = s + 1 == STAGES ? 0 : s + 1;
     }
   }
@@ -199,8 +224,7 @@ __global__ void __launch_bounds__(THREADS) lora_small_kernel(const Args a) {
   if (a.mid && rank == 0 && mrow < count) {
     float* mid = a.mid + (size_t)rows[mrow] * a.mp;
 #pragma unroll
-    for (int e = 0; e < EPT; ++e)
-      if (VEC || mcol + e < a.mp) mid[mcol + e] = v[e];
+    for (int e = 0; e < EPT; ++e) mid[mcol + e] = v[e];
   }
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -276,14 +300,14 @@ __global__ void __launch_bounds__(THREADS) lora_small_kernel(const Args a) {
         }
     }
     const int n = q * 32 + 8 * t;
-    if (ra >= 0) st8<T, VEC>(y + ra * N, n, N, add8<T>(b0, c, 0, fa));
-    if (rb >= 0) st8<T, VEC>(y + rb * N, n, N, add8<T>(b1, c, 2, fb));
+    if (ra >= 0) st8<T, VEC>(y + ra * N + n, N - n, add8<T>(b0, c, 0, fa));
+    if (rb >= 0) st8<T, VEC>(y + rb * N + n, N - n, add8<T>(b1, c, 2, fb));
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 int launch_small(const Args& a, int dtype, bool tr, cudaStream_t st) {
-  const bool vec = a.D % 8 == 0 && a.N % 8 == 0 && a.r % 8 == 0;
+  const bool vec = aligned_widths(a.D, a.N, a.r);
   return by_type(dtype, a.r, vec, [&](auto tc, auto rc, auto vc) -> int {
     using T = decltype(tc);
     constexpr int RP = decltype(rc)::value;

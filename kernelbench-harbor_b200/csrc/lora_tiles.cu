@@ -27,10 +27,10 @@ constexpr int ROWB = SK * 2;               // bytes of a stage's wide row; 16-by
 constexpr int WIDE = ROWS_L * ROWB;        // bytes of a stage's wide rows
 constexpr int MAX_SPLIT = 8;
 
-// Stages of the ring and CTAs per SM: 2 x 4 at rank 64, else 3 x 3 -- as many
+// Stages of the ring and CTAs per SM: 3 x 3 up to rank 16, else 2 x 4 -- as many
 // bytes in flight, and half as many warps again to hide each other's latencies.
-__host__ __device__ constexpr int stages_of(int rp) { return rp == 64 ? 4 : 3; }
-__host__ __device__ constexpr int ctas_of(int rp, bool vec) { return !vec ? 1 : rp == 64 ? 2 : 3; }
+__host__ __device__ constexpr int stages_of(int rp) { return rp >= 32 ? 4 : 3; }
+__host__ __device__ constexpr int ctas_of(int rp, bool vec) { return !vec || rp >= 32 ? 2 : 3; }
 
 // Swizzle of a row's 16-byte pieces: 8 rows x 1 piece (a fragment's words) and
 // 2 rows x 4 pieces (a quarter warp's 16-byte loads) both meet all banks once.
@@ -85,11 +85,20 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_shrink_tile_ke
   for (int i = 0; i < NP; ++i)
     psrc[i] = TR ? P + (size_t)(prk + i * PSTEP) * D + s0 * SK + q * 8 : P + (size_t)(s0 * SK + prk + i * PSTEP) * r + q * 8;
   const uint32_t smem = smem_u32(sm), wdst = prow * ROWB + ((pc ^ swz(prow)) << 4);
+  const bool halves = r % 8 != 0;  // A's rows are 8-byte aligned only
   const uint32_t pdst = WIDE + (TR ? prk * ROWB + ((q ^ swz(prk)) << 4) : row32(prk) * C::PITCH + q * 16);
   int kst = s0 * SK;     // first column of the stage that is requested next
   uint32_t in = smem;    // and its ring slot
-  auto stage = [&]() {
-    if (VEC && kst + SK <= D) {  // a whole stage: no column to check
+  auto advance = [&]() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) src[i] += SK;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) psrc[i] += TR ? SK : SK * r;
+    kst += SK;
+  };
+  auto next = [&](uint32_t slot) { return slot == smem + (STG - 1) * C::STAGE ? smem : slot + C::STAGE; };
+  auto stage = [&]() {  // VEC: asynchronous copies
+    if (kst + SK <= D && (TR || !halves)) {  // a whole stage: no column to check
       static_for<4>([&](auto i) {
         cp_async16_ahead<32 * i * ROWB>(in + wdst, src[i], prow + 32 * i < count ? 16 : 0);
       });
@@ -99,28 +108,53 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_shrink_tile_ke
         });
     } else {
       static_for<4>([&](auto i) {
-        stage16<T, VEC, true, 32 * i * ROWB>(in + wdst, src[i], D - kst - pc * 8, prow + 32 * i < count, x);
+        copy16<true, 32 * i * ROWB>(in + wdst, src[i], D - kst - pc * 8, prow + 32 * i < count, x);
       });
       if (has_p)
         static_for<NP>([&](auto i) {
           if constexpr (!TR)
-            stage16<T, VEC, false, i * PSTEP * C::PITCH>(in + pdst, psrc[i], r - q * 8, kst + prk + i * PSTEP < D, P);
+            copy16<false, i * PSTEP * C::PITCH>(in + pdst, psrc[i], r - q * 8, kst + prk + i * PSTEP < D, P, halves);
           else
-            stage16<T, VEC, false, i * PSTEP * ROWB>(in + pdst, psrc[i], D - kst - q * 8, prk + i * PSTEP < r, P);
+            copy16<false, i * PSTEP * ROWB>(in + pdst, psrc[i], D - kst - q * 8, prk + i * PSTEP < r, P);
         });
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) src[i] += SK;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) psrc[i] += TR ? SK : SK * r;
-    kst += SK;
-    in = in == smem + (STG - 1) * C::STAGE ? smem : in + C::STAGE;
+    advance();
+    in = next(in);
+  };
+  // otherwise: to registers a stage ahead, then to the ring
+  uint4 wv[VEC ? 1 : 4], pv[VEC ? 1 : NP];
+  auto request = [&]() {
+    if constexpr (!VEC) {
+      const T* const x_end = x + a.T * D;
+      const T* const p_end = reinterpret_cast<const T*>(a.P) + a.L * D * r;
+      static_for<4>([&](auto i) {
+        wv[i] = prow + 32 * i < count ? ld8_any<T>(src[i], D - kst - pc * 8, x_end) : make_uint4(0, 0, 0, 0);
+      });
+      static_for<NP>([&](auto i) {
+        const bool here = has_p && (TR ? prk + i * PSTEP < r : kst + prk + i * PSTEP < D);
+        pv[i] = here ? ld8_any<T>(psrc[i], TR ? D - kst - q * 8 : r - q * 8, p_end) : make_uint4(0, 0, 0, 0);
+      });
+      advance();
+    }
+  };
+  auto deposit = [&]() {
+    if constexpr (!VEC) {
+      static_for<4>([&](auto i) { sts16<32 * i * ROWB>(in + wdst, wv[i]); });
+      if (has_p) static_for<NP>([&](auto i) { sts16<i * PSTEP*(TR ? ROWB : C::PITCH)>(in + pdst, pv[i]); });
+      in = next(in);
+    }
   };
   float acc[NM][RP / 8][4] = {};
+  if constexpr (VEC) {
 #pragma unroll
-  for (int i = 0; i < STG - 1; ++i) {
-    if (s0 + i < s1) stage();
-    cp_async_commit();
+    for (int i = 0; i < STG - 1; ++i) {
+      if (s0 + i < s1) stage();
+      cp_async_commit();
+    }
+  } else if (s0 < s1) {
+    request();
+    deposit();
+    if (s0 + 1 < s1) request();
   }
   // where this lane reads a stage: its rows' pieces of either half, and P's
   const uint32_t xrow = (16 * NM * mg + g) * ROWB;
@@ -135,8 +169,13 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_shrink_tile_ke
   for (int st = s0; st < s1; ++st) {
     cp_async_wait<STG - 2>();
     __syncthreads();  // stage st has landed for every thread; the slot filled next was read before
-    if (st + STG - 1 < s1) stage();
-    cp_async_commit();
+    if constexpr (VEC) {
+      if (st + STG - 1 < s1) stage();
+      cp_async_commit();
+    } else {
+      if (st + 1 < s1) deposit();
+      if (st + 2 < s1) request();
+    }
     if (16 * NM * mg < count) {
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
@@ -170,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_shrink_tile_ke
         });
       }
     }
-    slot = slot == smem + (STG - 1) * C::STAGE ? smem : slot + C::STAGE;
+    slot = next(slot);
   }
   pdl_launch_next();
   cp_async_wait<0>();
@@ -217,10 +256,9 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_shrink_tile_ke
       }
     }
     // past the rank: an exact 0, whatever x holds
-    if (VEC || col < a.mp)
-      *reinterpret_cast<float4*>(a.mid + (size_t)rows[row] * a.mp + col) =
-          make_float4(col < r ? s.x * scale : 0.f, col + 1 < r ? s.y * scale : 0.f, col + 2 < r ? s.z * scale : 0.f,
-                      col + 3 < r ? s.w * scale : 0.f);
+    *reinterpret_cast<float4*>(a.mid + (size_t)rows[row] * a.mp + col) =
+        make_float4(col < r ? s.x * scale : 0.f, col + 1 < r ? s.y * scale : 0.f, col + 2 < r ? s.z * scale : 0.f,
+                    col + 3 < r ? s.w * scale : 0.f);
   }
   if (S > 1) cluster_sync();  // the others have read this CTA's part
 }
@@ -254,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
   const T* base = reinterpret_cast<const T*>(a.base);
   T* y = reinterpret_cast<T*>(a.y);
   if (tl.x < 0) {
-    copy_rows<T, VEC>(base, y, rows, count, N, n0, min(n0 + steps * SK, N));
+    copy_rows<T, VEC>(base, y, rows, count, N, n0, min(n0 + steps * SK, N), base + a.T * N);
     pdl_wait_previous();
     return;
   }
@@ -284,9 +322,20 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
                                    : qrow * C::PITCH + (q >> 2) * 64 + (q & 3) * 4);
   int cst = n0;
   uint32_t in = smem;
-  // base (and, TR, A's rows) by asynchronous copies
+  auto advance = [&]() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) src[i] += SK;
+    if (TR) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) qsrc[i] += SK * r;
+    }
+    cst += SK;
+  };
+  auto next = [&](uint32_t slot) { return slot == smem + (STG - 1) * C::STAGE ? smem : slot + C::STAGE; };
+  const bool halves = r % 8 != 0;  // TR: A's rows are 8-byte aligned only
+  // VEC: base (and, TR, A's rows) by asynchronous copies
   auto stage = [&]() {
-    if (VEC && cst + SK <= N) {
+    if (cst + SK <= N && !(TR && halves)) {
       if (base)
         static_for<4>([&](auto i) {
           cp_async16_ahead<32 * i * ROWB>(in + wdst, src[i], prow + 32 * i < count ? 16 : 0);
@@ -295,21 +344,38 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
     } else {
       if (base)
         static_for<4>([&](auto i) {
-          stage16<T, VEC, true, 32 * i * ROWB>(in + wdst, src[i], N - cst - pc * 8, prow + 32 * i < count, base);
+          copy16<true, 32 * i * ROWB>(in + wdst, src[i], N - cst - pc * 8, prow + 32 * i < count, base);
         });
       if (TR && has_q)
         static_for<NP>([&](auto i) {
-          stage16<T, VEC, false, i * PSTEP * C::PITCH>(in + qdst, qsrc[i], r - q * 8, cst + qrow + i * PSTEP < N, Q);
+          copy16<false, i * PSTEP * C::PITCH>(in + qdst, qsrc[i], r - q * 8, cst + qrow + i * PSTEP < N, Q, halves);
         });
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) src[i] += SK;
-    if (TR) {
-#pragma unroll
-      for (int i = 0; i < NP; ++i) qsrc[i] += SK * r;
+    advance();
+    in = next(in);
+  };
+  // otherwise: to registers a stage ahead, then to the ring
+  const T* const q_end = reinterpret_cast<const T*>(a.Q) + a.L * N * r;
+  uint4 wv[VEC ? 1 : 4], av[VEC || !TR ? 1 : NP];
+  auto request = [&]() {
+    if constexpr (!VEC) {
+      static_for<4>([&](auto i) {
+        wv[i] = base && prow + 32 * i < count ? ld8_any<T>(src[i], N - cst - pc * 8, base + a.T * N) : make_uint4(0, 0, 0, 0);
+      });
+      if constexpr (TR)
+        static_for<NP>([&](auto i) {
+          av[i] = has_q && cst + qrow + i * PSTEP < N ? ld8_any<T>(qsrc[i], r - q * 8, q_end) : make_uint4(0, 0, 0, 0);
+        });
+      advance();
     }
-    cst += SK;
-    in = in == smem + (STG - 1) * C::STAGE ? smem : in + C::STAGE;
+  };
+  auto deposit = [&]() {
+    if constexpr (!VEC) {
+      if (base) static_for<4>([&](auto i) { sts16<32 * i * ROWB>(in + wdst, wv[i]); });
+      if constexpr (TR)
+        if (has_q) static_for<NP>([&](auto i) { sts16<i * PSTEP * C::PITCH>(in + qdst, av[i]); });
+      in = next(in);
+    }
   };
   // !TR: Q through registers, since its words change places: word p of the 8
   // columns of lane t goes to tile p, place t
@@ -317,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
   auto load_q = [&](int st) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      qv[i] = has_q && qin[i] ? ld8<T, VEC>(qsrc[i], 0, N - n0 - st * SK - q * 8) : make_uint4(0, 0, 0, 0);
+      qv[i] = has_q && qin[i] ? ld8<T, VEC>(qsrc[i], 0, N - n0 - st * SK - q * 8, q_end) : make_uint4(0, 0, 0, 0);
       qsrc[i] += SK;
     }
   };
@@ -330,10 +396,16 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
                      : "memory");
       });
   };
+  if constexpr (VEC) {
 #pragma unroll
-  for (int i = 0; i < STG - 1; ++i) {
-    if (i < nst) stage();
-    cp_async_commit();
+    for (int i = 0; i < STG - 1; ++i) {
+      if (i < nst) stage();
+      cp_async_commit();
+    }
+  } else {
+    request();
+    deposit();
+    if (nst > 1) request();
   }
   if constexpr (!TR) load_q(0);
   pdl_wait_previous();  // mid comes from the kernel before; all else was there when that one began
@@ -349,9 +421,8 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
     float mx = 0.f;
 #pragma unroll
     for (int k = 0; k < RP / 16; ++k) {
-      v[k] = row >= 0 && (VEC || 16 * k + 4 * t < a.mp)
-                 ? *reinterpret_cast<const float4*>(a.mid + row * a.mp + 16 * k + 4 * t)
-                 : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[k] = row >= 0 ? *reinterpret_cast<const float4*>(a.mid + row * a.mp + 16 * k + 4 * t)
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
       const float f[4] = {fabsf(v[k].x), fabsf(v[k].y), fabsf(v[k].z), fabsf(v[k].w)};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -384,8 +455,13 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
     if constexpr (!TR) put_q(slot);  // this slot's last readers are two barriers back
     cp_async_wait<STG - 2>();
     __syncthreads();
-    if (st + STG - 1 < nst) stage();
-    cp_async_commit();
+    if constexpr (VEC) {
+      if (st + STG - 1 < nst) stage();
+      cp_async_commit();
+    } else {
+      if (st + 1 < nst) deposit();
+      if (st + 2 < nst) request();
+    }
     if constexpr (!TR) {
       if (st + 1 < nst) load_q(st + 1);
     }
@@ -416,19 +492,19 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
           ua = lds16<0>(slot + boff[w]);
           ub = lds16<8 * ROWB>(slot + boff[w]);
         }
-        if (ra >= 0) st8<T, VEC>(ya + 32 * w, 0, left - 32 * w, add8<T>(ua, c, 0, fac[0]));
-        if (rb >= 0) st8<T, VEC>(yb + 32 * w, 0, left - 32 * w, add8<T>(ub, c, 2, fac[1]));
+        if (ra >= 0) st8<T, VEC>(ya + 32 * w, left - 32 * w, add8<T>(ua, c, 0, fac[0]));
+        if (rb >= 0) st8<T, VEC>(yb + 32 * w, left - 32 * w, add8<T>(ub, c, 2, fac[1]));
       });
     }
     ya += SK;
     yb += SK;
     left -= SK;
-    slot = slot == smem + (STG - 1) * C::STAGE ? smem : slot + C::STAGE;
+    slot = next(slot);
   }
 }
 
 int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
-  const bool vec = a.D % 8 == 0 && a.N % 8 == 0 && a.r % 8 == 0;
+  const bool vec = aligned_widths(a.D, a.N, a.r);
   return by_type(dtype, a.r, vec, [&](auto tc, auto rc, auto vc) -> int {
     using T = decltype(tc);
     constexpr int RP = decltype(rc)::value;
