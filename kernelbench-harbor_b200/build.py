@@ -20,7 +20,7 @@ LIB = os.path.join(PKG_DIR, "libb200q.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
-    "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
+    "-O3", "-lineinfo", "-std=c++17", "-shared", "--threads", "0", "-Xcompiler", "-fPIC",
     "-Xptxas", "-warn-spills",
 ]
 

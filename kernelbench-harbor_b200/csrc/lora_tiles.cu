@@ -27,10 +27,10 @@ constexpr int ROWB = SK * 2;               // bytes of a stage's wide row; 16-by
 constexpr int WIDE = ROWS_L * ROWB;        // bytes of a stage's wide rows
 constexpr int MAX_SPLIT = 8;
 
-// Stages of the ring and CTAs per SM: 3 x 3 up to rank 16, else 2 x 4 -- as many
+// Stages of the ring and CTAs per SM: 4 and 2 at rank 64, else 3 and 3 -- as many
 // bytes in flight, and half as many warps again to hide each other's latencies.
-__host__ __device__ constexpr int stages_of(int rp) { return rp >= 32 ? 4 : 3; }
-__host__ __device__ constexpr int ctas_of(int rp, bool vec) { return !vec || rp >= 32 ? 2 : 3; }
+__host__ __device__ constexpr int stages_of(int rp) { return rp == 64 ? 4 : 3; }
+__host__ __device__ constexpr int ctas_of(int rp, bool vec) { return !vec || rp == 64 ? 2 : 3; }
 
 // Swizzle of a row's 16-byte pieces: 8 rows x 1 piece (a fragment's words) and
 // 2 rows x 4 pieces (a quarter warp's 16-byte loads) both meet all banks once.
