@@ -276,11 +276,11 @@ int b200q_lora_plan(const int64_t* lora_ids, int64_t T, int64_t L, int32_t* plan
  * base.  lo: the row between the two products, for the backward pass:
  * b200q_lora_mid_bytes(T, r) bytes, any contents; rows of tokens without an
  * adapter are left as they were.  NULL where T <= 256 and no backward pass
- * follows. */
+ * follows.  workspace: a status word for waits that run out, or NULL. */
 size_t b200q_lora_mid_bytes(int64_t T, int64_t r);
 int b200q_lora_apply(const void* x, const void* base, const void* A, const void* B, const float* scaling,
                      const int32_t* plan, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype, void* y,
-                     float* lo, void* stream);
+                     float* lo, void* workspace, void* stream);
 
 /* The gradients of that call: dx (base: added to it, NULL for zeros, may be dx
  * itself), dA and dB, each NULL to leave it out; an adapter without tokens gets
@@ -289,7 +289,8 @@ int b200q_lora_apply(const void* x, const void* base, const void* A, const void*
  * dy. */
 int b200q_lora_backward(const void* x, const void* dy, const void* base, const void* A, const void* B,
                         const float* scaling, const int32_t* plan, const float* lo, int64_t T, int64_t D, int64_t N,
-                        int64_t r, int64_t L, int dtype, float* dlo, void* dx, void* dA, void* dB, void* stream);
+                        int64_t r, int64_t L, int dtype, float* dlo, void* dx, void* dA, void* dB, void* workspace,
+                        void* stream);
 
 /* Grouped W4A16 GEMM over the experts of a MoE layer, one launch for all
  * experts.  x [rows, K] holds every expert's rows contiguously, expert e's at

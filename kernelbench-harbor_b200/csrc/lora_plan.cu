@@ -188,7 +188,7 @@ size_t b200q_lora_mid_bytes(int64_t T, int64_t r) {
 
 int b200q_lora_apply(const void* x, const void* base, const void* A, const void* B, const float* scaling,
                      const int32_t* plan, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype, void* y,
-                     float* lo, void* stream) {
+                     float* lo, void* workspace, void* stream) {
   using namespace b200q;
   using namespace b200q::lora;
   int rc = check_sizes("lora_apply", T, D, N, r, L, dtype);
@@ -197,13 +197,15 @@ int b200q_lora_apply(const void* x, const void* base, const void* A, const void*
   if (!x || !A || !B || !plan || !y || (!lo && T > SMALL_MAX_T))
     return fail(B200Q_ERR_SHAPE, "lora_apply: null pointer argument");
   if (misaligned({x, base, A, B, plan, y, lo})) return fail(B200Q_ERR_ALIGN, "lora_apply: pointers must be 16-byte aligned");
-  const Args a = {x, base, A, B, scaling, plan, plan_layout(T, L), (int)D, (int)N, (int)r, mid_pitch(r), y, lo, T, L};
+  const Args a = {x, base, A, B, scaling, plan, plan_layout(T, L), (int)D, (int)N, (int)r, mid_pitch(r), y, lo, T, L,
+                  reinterpret_cast<int*>(workspace)};
   return launch(a, dtype, false, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int b200q_lora_backward(const void* x, const void* dy, const void* base, const void* A, const void* B,
                         const float* scaling, const int32_t* plan, const float* lo, int64_t T, int64_t D, int64_t N,
-                        int64_t r, int64_t L, int dtype, float* dlo, void* dx, void* dA, void* dB, void* stream) {
+                        int64_t r, int64_t L, int dtype, float* dlo, void* dx, void* dA, void* dB, void* workspace,
+                        void* stream) {
   using namespace b200q;
   using namespace b200q::lora;
   int rc = check_sizes("lora_backward", T, D, N, r, L, dtype);
@@ -215,7 +217,8 @@ int b200q_lora_backward(const void* x, const void* dy, const void* base, const v
   if (misaligned({x, dy, base, A, B, plan, lo, dlo, dx, dA, dB}))
     return fail(B200Q_ERR_ALIGN, "lora_backward: pointers must be 16-byte aligned");
   if (T > 0 && need_dlo) {
-    const Args a = {dy, base, B, A, scaling, plan, plan_layout(T, L), (int)N, (int)D, (int)r, mid_pitch(r), dx, dlo, T, L};
+    const Args a = {dy, base, B, A, scaling, plan, plan_layout(T, L), (int)N, (int)D, (int)r, mid_pitch(r), dx, dlo, T, L,
+                    reinterpret_cast<int*>(workspace)};
     if ((rc = launch(a, dtype, true, st))) return rc;
   }
   return dA || dB ? launch_grads(x, dy, lo, dlo, plan, plan_layout(T, L), T, D, N, r, L, dtype, dA, dB, st) : B200Q_OK;

@@ -354,10 +354,16 @@ struct Args {
   void* y;
   float* mid;
   int64_t T, L;
+  int* status;  // or NULL
 };
 
 int launch_small(const Args& a, int dtype, bool tr, cudaStream_t st);
 int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st);
+
+// lora_shrink_tc.cu: ranks 33 to 64, aligned rows
+using ShrinkFn = void (*)(const Args, int);
+constexpr int SHRINK_TC_THREADS = THREADS + 32, SHRINK_TC_SMEM = 4 * (128 * 128 + 64 * 128) + 1024;
+const void* shrink_tc_kernel(int dtype, bool tr);
 
 inline bool aligned_widths(int64_t D, int64_t N, int64_t r) { return D % 8 == 0 && N % 8 == 0 && r % 4 == 0; }
 

@@ -503,33 +503,49 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
   }
 }
 
+// Launches a shrink kernel (kern<<<tiles x S>>>(args, S)) with the split of the
+// contraction that has the shortest estimate: rounds of co-resident clusters x
+// (stages of a part + 5 for start, joining and ending), for about half a tile
+// more than T / 128 with each adapter that ends inside one.
+template <class Kern, class Fit>
+int launch_split(Kern kern, int threads, int smem, const Args& a, cudaStream_t st, Fit fit) {
+  const int64_t whole = (a.T + ROWS_L - 1) / ROWS_L, tiles = whole + std::min(a.L, whole) / 2, nst = (a.D + SK - 1) / SK;
+  int S = 1;
+  int64_t best = INT64_MAX;
+  for (int s = 1; s <= MAX_SPLIT && (s == 1 || nst >= 4 * s); ++s) {
+    const int64_t at_once = fit(s), cost = ((tiles + at_once - 1) / at_once) * ((nst + s - 1) / s + 5);
+    if (cost < best) best = cost, S = s;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.lay.max_large * S));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)S;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a, S), "lora shrink launch");
+}
+
 int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
   const bool vec = aligned_widths(a.D, a.N, a.r);
   return by_type(dtype, a.r, vec, [&](auto tc, auto rc, auto vc) -> int {
     using T = decltype(tc);
     constexpr int RP = decltype(rc)::value;
     constexpr bool VEC = decltype(vc)::value;
-    auto shrink = tr ? lora_shrink_tile_kernel<T, RP, true, VEC> : lora_shrink_tile_kernel<T, RP, false, VEC>;
     auto expand = tr ? lora_expand_tile_kernel<T, RP, true, VEC> : lora_expand_tile_kernel<T, RP, false, VEC>;
-    const int smem_s = tr ? ShrinkCfg<RP, true>::SMEM : ShrinkCfg<RP, false>::SMEM;
     const int smem_e = tr ? ExpandCfg<RP, true>::SMEM : ExpandCfg<RP, false>::SMEM;
-    int rc2 = allow_smem((const void*)shrink, smem_s, "cudaFuncSetAttribute(lora shrink)");
-    if (rc2 || (rc2 = allow_smem((const void*)expand, smem_e, "cudaFuncSetAttribute(lora expand)"))) return rc2;
-    // shrink: the split with the shortest estimate, rounds of co-resident
-    // clusters x (stages of a part + 5 for start, joining and ending)
-    // (about half a tile more than T / 128 for each adapter that ends inside one)
-    const int64_t full = (a.T + ROWS_L - 1) / ROWS_L, tiles = full + std::min(a.L, full) / 2, nst = (a.D + SK - 1) / SK;
-    int S = 1;
-    int64_t best = INT64_MAX;
-    for (int s = 1; s <= MAX_SPLIT && (s == 1 || nst >= 4 * s); ++s) {
-      const int64_t fit = resident_clusters((const void*)shrink, THREADS, smem_s, s);
-      const int64_t cost = ((tiles + fit - 1) / fit) * ((nst + s - 1) / s + 5);
-      if (cost < best) best = cost, S = s;
-    }
-    // expand: likewise the number of 64-column steps per CTA (start: 2 steps)
+    // expand: the number of 64-column steps per CTA with the shortest estimate (start: 2 steps)
+    int status = allow_smem((const void*)expand, smem_e, "cudaFuncSetAttribute(lora expand)");
+    if (status) return status;
+    const int64_t whole = (a.T + ROWS_L - 1) / ROWS_L, tiles = whole + std::min(a.L, whole) / 2;
     const int64_t nsteps = (a.N + SK - 1) / SK, slots = resident_clusters((const void*)expand, THREADS, smem_e, 1);
     int steps = 2;
-    best = INT64_MAX;
+    int64_t best = INT64_MAX;
     for (int s = 2; s <= 16; ++s) {
       const int64_t cost = ((tiles * ((nsteps + s - 1) / s) + slots - 1) / slots) * (s + 2);
       if (cost < best) best = cost, steps = s;
@@ -537,26 +553,35 @@ int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
     const int parts = (int)((nsteps + steps - 1) / steps);
     const int64_t blocks = a.lay.max_large * parts;
     if (blocks > (1ll << 31) - 1) return fail(B200Q_ERR_SHAPE, "lora_apply: size too large");
+    if constexpr (VEC && RP == 64) {
+      // tensor memory instead of register fragments from rank 33 on: D=14336,
+      // r=64, 4096 tokens 53 us with it and 61 us without (shrink and expand);
+      // D=4096 and N=14336, r=16, 8192 tokens, forward and backward 253 and 250
+      const void* kern = shrink_tc_kernel(dtype, tr);
+      if ((status = allow_smem(kern, SHRINK_TC_SMEM, "cudaFuncSetAttribute(lora shrink)"))) return status;
+      // the occupancy query counts a kernel with tensor memory once per SM; its 64 of 512 columns and its shared memory
+      // let two share one
+      status = launch_split(reinterpret_cast<ShrinkFn>(const_cast<void*>(kern)), SHRINK_TC_THREADS, SHRINK_TC_SMEM, a, st,
+                            [&](int s) { return 2 * resident_clusters(kern, SHRINK_TC_THREADS, SHRINK_TC_SMEM, s); });
+    } else {
+      auto shrink = tr ? lora_shrink_tile_kernel<T, RP, true, VEC> : lora_shrink_tile_kernel<T, RP, false, VEC>;
+      const int smem_s = tr ? ShrinkCfg<RP, true>::SMEM : ShrinkCfg<RP, false>::SMEM;
+      if ((status = allow_smem((const void*)shrink, smem_s, "cudaFuncSetAttribute(lora shrink)"))) return status;
+      status = launch_split(shrink, THREADS, smem_s, a, st,
+                            [&](int s) { return resident_clusters((const void*)shrink, THREADS, smem_s, s); });
+    }
+    if (status || !a.y) return status;  // no y: mid alone was asked for
+    // the expand kernel's start overlaps the shrink kernel's end
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.lay.max_large * S));
+    cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem_s;
+    cfg.dynamicSmemBytes = (size_t)smem_e;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)S;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, shrink, a, S);
-    if (e != cudaSuccess) return check_cuda(e, "lora shrink launch");
-    if (!a.y) return B200Q_OK;  // mid alone was asked for
-    // the expand kernel's start overlaps the shrink kernel's end
-    cfg.gridDim = dim3((unsigned)blocks);
-    cfg.dynamicSmemBytes = smem_e;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     return check_cuda(cudaLaunchKernelEx(&cfg, expand, a, parts, steps), "lora expand launch");
   });
 }

@@ -612,7 +612,8 @@ def _lora_run(x, base, A, B, scaling, plan, out, lo):
     with _device(dev):
         _lib.check(_lib.lib().b200q_lora_apply(x.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling),
                                                plan.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters,
-                                               _dtype_code(x.dtype), out.data_ptr(), _ptr(lo), _stream_ptr(dev)))
+                                               _dtype_code(x.dtype), out.data_ptr(), _ptr(lo),
+                                               workspace(dev, 256).data_ptr(), _stream_ptr(dev)))
 
 
 def _lora_mid(x: torch.Tensor, r: int) -> torch.Tensor:
@@ -650,7 +651,7 @@ def _lora_backward(ctx, dy):
             _lib.check(_lib.lib().b200q_lora_backward(
                 x.data_ptr(), d.data_ptr(), None, A.data_ptr(), B.data_ptr(), _ptr(scaling), ctx.plan.data_ptr(),
                 lo.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters, _dtype_code(x.dtype), _ptr(dlo), _ptr(dx),
-                _ptr(dA), _ptr(dB), _stream_ptr(dev)))
+                _ptr(dA), _ptr(dB), workspace(dev, 256).data_ptr(), _stream_ptr(dev)))
     return dy if need_base else None, dx, dA, dB, None, None
 
 

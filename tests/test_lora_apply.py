@@ -444,7 +444,7 @@ def test_refusals_without_gpu():
     assert L.b200q_lora_plan(p, 64, 0, p, n, None, None) == L.b200q_lora_plan(p, (1 << 24) + 1, 8, p, n, None, None) == _lib.ERR_SHAPE
 
     def call(T=64, D=64, N=64, r=8, nl=4, dtype=0, x=p, y=p, lo=p):
-        return L.b200q_lora_apply(x, p, p, p, None, p, T, D, N, r, nl, dtype, y, lo, None)
+        return L.b200q_lora_apply(x, p, p, p, None, p, T, D, N, r, nl, dtype, y, lo, None, None)
 
     assert call(r=65) == call(r=0) == call(D=0) == call(N=1 << 23) == call(nl=1024) == call(T=-1) == _lib.ERR_SHAPE
     assert call(x=None) == call(lo=None, T=257) == call(y=None) == _lib.ERR_SHAPE
@@ -453,7 +453,7 @@ def test_refusals_without_gpu():
     assert call(T=0) == _lib.OK
 
     def back(T=64, r=8, x=p, dy=p, A=p, dx=p, dA=p, dB=p, lo=p, dlo=p):
-        return L.b200q_lora_backward(x, dy, None, A, p, None, p, lo, T, 64, 64, r, 4, 0, dlo, dx, dA, dB, None)
+        return L.b200q_lora_backward(x, dy, None, A, p, None, p, lo, T, 64, 64, r, 4, 0, dlo, dx, dA, dB, None, None)
 
     assert back(x=None) == back(dy=None) == back(A=None) == back(lo=None) == back(r=65) == _lib.ERR_SHAPE
     assert back(dlo=None) == back(dlo=None, dA=None, dB=None) == _lib.ERR_SHAPE
