@@ -284,13 +284,15 @@ int b200q_lora_apply(const void* x, const void* base, const void* A, const void*
 
 /* The gradients of that call: dx (base: added to it, NULL for zeros, may be dx
  * itself), dA and dB, each NULL to leave it out; an adapter without tokens gets
- * zeros.  lo as b200q_lora_apply left it; dlo: b200q_lora_mid_bytes(T, r) bytes
- * of scratch, needed for dx and dA.  The gradient of b200q_lora_apply's base is
- * dy. */
+ * zeros.  lo as b200q_lora_apply left it.  scratch: any contents, overwritten,
+ * b200q_lora_backward_scratch_bytes of it (for the current device); it may be
+ * freed or reused once the call has run on the stream.  The gradient of
+ * b200q_lora_apply's base is dy. */
+size_t b200q_lora_backward_scratch_bytes(int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype);
 int b200q_lora_backward(const void* x, const void* dy, const void* base, const void* A, const void* B,
                         const float* scaling, const int32_t* plan, const float* lo, int64_t T, int64_t D, int64_t N,
-                        int64_t r, int64_t L, int dtype, float* dlo, void* dx, void* dA, void* dB, void* workspace,
-                        void* stream);
+                        int64_t r, int64_t L, int dtype, void* scratch, size_t scratch_bytes, void* dx, void* dA,
+                        void* dB, void* workspace, void* stream);
 
 /* Grouped W4A16 GEMM over the experts of a MoE layer, one launch for all
  * experts.  x [rows, K] holds every expert's rows contiguously, expert e's at

@@ -76,7 +76,8 @@ SIGNATURES = {
     "b200q_lora_plan": (ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_sz, _c_vp, _c_vp]),
     "b200q_lora_mid_bytes": (_c_sz, [_c_i64, _c_i64]),
     "b200q_lora_apply": (ctypes.c_int, [_c_vp] * 6 + [_c_i64] * 5 + [ctypes.c_int] + [_c_vp] * 4),
-    "b200q_lora_backward": (ctypes.c_int, [_c_vp] * 8 + [_c_i64] * 5 + [ctypes.c_int] + [_c_vp] * 6),
+    "b200q_lora_backward_scratch_bytes": (_c_sz, [_c_i64] * 5 + [ctypes.c_int]),
+    "b200q_lora_backward": (ctypes.c_int, [_c_vp] * 8 + [_c_i64] * 5 + [ctypes.c_int, _c_vp, _c_sz] + [_c_vp] * 5),
     "b200q_mxfp8_gemm_peers": (ctypes.c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_int, _c_i64, _c_i64,
                                               _c_vp, ctypes.c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_sz, _c_vp]),
     "b200q_peer_barrier": (ctypes.c_int, [_c_vp, ctypes.c_int, ctypes.c_int, _c_vp, _c_vp]),

@@ -9,8 +9,10 @@
 // ring of GSTG stages, the thin rows through registers, split into two halves
 // of the type one stage ahead (fp16: scaled by a power of two that follows the
 // largest value seen, the sums with it).  A warp takes 32 columns and one half
-// of the stage's tokens.  The two halves, and the S parts of a token range,
-// which form a cluster, are added in a fixed order: deterministic.
+// of the stage's tokens.  The two halves, and the S parts of a token range, which
+// a second launch joins, are added in a fixed order: deterministic.  (As a
+// cluster the parts would need no second launch, but clusters of 3 fill only
+// 142 x 3 of the SMs' 444 places: 144 column blocks took two rounds.)
 // Bound: HBM, x and dy once; at r = 64 the legacy tensor rate is as near (two
 // halves: 4 T r (D + N) flop).
 #include <type_traits>
@@ -46,7 +48,25 @@ struct GradArgs {
   int D, N, r, mp, nbd;
   int64_t T;
   void *dA, *dB;
+  float* part;  // S > 1: [S][L][blocks][RP][CT] sums
 };
+
+// Rounds a block's sums [rank][column] into dA [column][rank] or dB [rank][column].
+template <class T>
+__device__ __forceinline__ void write_block(const GradArgs& a, const float* out, int block, int seg) {
+  const bool da = block < a.nbd;
+  const int W = da ? a.D : a.N, r = a.r, w0 = (da ? block : block - a.nbd) * CT, nc = min(CT, W - w0);
+  T* dst = reinterpret_cast<T*>(da ? a.dA : a.dB) + (size_t)seg * W * r;
+  if (da) {
+    for (int i = threadIdx.x; i < nc * r; i += THREADS)  // nc * r consecutive values of dA
+      dst[(size_t)w0 * r + i] = ft<T>(out[i % r * OPITCH + i / r]);
+  } else {
+    for (int i = threadIdx.x; i < CT * r; i += THREADS) {
+      const int j = i / CT, c = i % CT;
+      if (c < nc) dst[(size_t)j * W + w0 + c] = ft<T>(out[j * OPITCH + c]);
+    }
+  }
+}
 
 template <class T, int RP, bool VEC>
 __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 2) lora_grads_kernel(const GradArgs a, int S) {
@@ -59,9 +79,9 @@ __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 2) lora_gra
   const bool da = (int)blockIdx.x < a.nbd;  // columns of x (dA) or of dy (dB)
   const T* wide = reinterpret_cast<const T*>(da ? a.x : a.dy);
   const float* thin = da ? a.dlo : a.lo;
-  const int W = da ? a.D : a.N, r = a.r;
+  const int W = da ? a.D : a.N;
   const int w0 = (da ? blockIdx.x : blockIdx.x - a.nbd) * CT;
-  const int seg = blockIdx.y, rank = S > 1 ? (int)cluster_ctarank() : 0;
+  const int seg = blockIdx.y, rank = blockIdx.z;
   const int b0 = a.plan[a.lay.seg + seg], b1 = a.plan[a.lay.seg + seg + 1];
   const int nst_all = (b1 - b0 + TK - 1) / TK;
   // whole stages per rank
@@ -245,49 +265,79 @@ __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 2) lora_gra
     }
     if (h) __syncthreads();
   }
-  if (S > 1)
-    cluster_sync();
-  else
-    __syncthreads();
-  // this rank's columns [q0, q1) of the block
-  const int q0 = rank * CT / S, q1 = min((rank + 1) * CT / S, W - w0), nq = max(q1 - q0, 0);
-  T* dst = reinterpret_cast<T*>(da ? a.dA : a.dB) + (size_t)seg * W * r;
-  for (int i = tid; i < nq * r; i += THREADS) {
-    const int j = da ? i % r : i / nq, c = q0 + (da ? i / r : i % nq);
-    float v;
-    if (S > 1) {
-      const uint32_t addr = smem_u32(out + j * OPITCH + c);
-      v = 0.f;
-      for (int k = 0; k < S; ++k) {
-        float u;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u) : "r"(map_shared_rank(addr, k)) : "memory");
-        v += u;
-      }
-    } else {
-      v = out[j * OPITCH + c];
-    }
-    dst[da ? (size_t)(w0 + c) * r + j : (size_t)j * W + w0 + c] = ft<T>(v);
+  pdl_launch_next();
+  __syncthreads();
+  if (S > 1) {
+    float* dst = a.part + (((size_t)rank * gridDim.y + seg) * gridDim.x + blockIdx.x) * (RP * CT);
+    for (int i = tid; i < RP * CT; i += THREADS) dst[i] = out[i / CT * OPITCH + i % CT];
+    return;
   }
-  if (S > 1) cluster_sync();  // the others have read this CTA's sums
+  write_block<T>(a, out, blockIdx.x, seg);
+}
+
+// The sums of the S parts of a block, in order.
+template <class T, int RP>
+__global__ void __launch_bounds__(THREADS) lora_grads_join_kernel(const GradArgs a, int S) {
+  __shared__ float out[RP * OPITCH];
+  pdl_wait_previous();
+  const size_t step = (size_t)gridDim.y * gridDim.x * (RP * CT);
+  const float* src = a.part + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * (RP * CT);
+  for (int i = threadIdx.x; i < RP * CT; i += THREADS) {
+    float v = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < S; ++s) v += src[s * step + i];
+    out[i / CT * OPITCH + i % CT] = v;
+  }
+  __syncthreads();
+  write_block<T>(a, out, blockIdx.x, blockIdx.y);
+}
+
+constexpr int MAX_PARTS = 8;
+
+// Parts of the tokens: the shortest estimate, for adapters of equal shares:
+// rounds of co-resident CTAs x (stages of a part + 5).  More than one part only
+// where the column blocks leave places free, so the parts' sums stay small.
+template <class T, int RP, bool VEC>
+int parts_of(int64_t T_, int64_t blocks, int64_t L) {
+  const int64_t fit = resident_clusters((const void*)lora_grads_kernel<T, RP, VEC>, THREADS, GradCfg<RP>::SMEM, 1);
+  const int64_t nst = (T_ + TK * L - 1) / (TK * L);
+  int S = 1;
+  int64_t best = INT64_MAX;
+  for (int s = 1; s <= MAX_PARTS && (s == 1 || (T_ >= 4 * TK * s && blocks * s <= 2 * fit)); ++s) {
+    const int64_t cost = (blocks * s + fit - 1) / fit * ((nst + s - 1) / s + 5);
+    if (cost < best) best = cost, S = s;
+  }
+  return S;
+}
+
+static int64_t column_blocks(int64_t W) { return (W + CT - 1) / CT; }
+
+size_t grads_part_bytes(int64_t T_, int64_t D, int64_t N, int64_t r, int64_t L, int dtype) {
+  size_t bytes = 0;
+  by_type(dtype, r, aligned_widths(D, N, r), [&](auto tc, auto rc, auto vc) -> int {
+    using T = decltype(tc);
+    constexpr int RP = decltype(rc)::value;
+    allow_smem((const void*)lora_grads_kernel<T, RP, decltype(vc)::value>, GradCfg<RP>::SMEM, "cudaFuncSetAttribute(lora grads)");
+    const int64_t blocks = (column_blocks(D) + column_blocks(N)) * L;
+    const int S = parts_of<T, RP, decltype(vc)::value>(T_, blocks, L);
+    bytes = S > 1 ? (size_t)S * blocks * (RP * CT) * 4 : 0;
+    return 0;
+  });
+  return bytes;
 }
 
 int launch_grads(const void* x, const void* dy, const float* lo, const float* dlo, const int32_t* plan,
-                 const PlanLayout& lay, int64_t T_, int64_t D, int64_t N, int64_t r, int64_t L, int dtype, void* dA,
-                 void* dB, cudaStream_t st) {
+                 const PlanLayout& lay, int64_t T_, int64_t D, int64_t N, int64_t r, int64_t L, int dtype, float* part,
+                 void* dA, void* dB, cudaStream_t st) {
   if (T_ == 0) {
     cudaError_t e = cudaSuccess;
     if (dA) e = cudaMemsetAsync(dA, 0, (size_t)L * D * r * 2, st);
     if (dB && e == cudaSuccess) e = cudaMemsetAsync(dB, 0, (size_t)L * N * r * 2, st);
     return check_cuda(e, "lora_grads memset");
   }
-  GradArgs a;
-  a.x = x, a.dy = dy, a.lo = lo, a.dlo = dlo, a.plan = plan, a.lay = lay;
-  a.D = (int)D, a.N = (int)N, a.r = (int)r, a.mp = mid_pitch(r), a.T = T_;
-  a.nbd = dA ? (int)((D + CT - 1) / CT) : 0;
-  const int nbn = dB ? (int)((N + CT - 1) / CT) : 0;
-  a.dA = dA, a.dB = dB;
-  const bool vec = aligned_widths(D, N, r);
-  return by_type(dtype, r, vec, [&](auto tc, auto rc, auto vc) -> int {
+  const int nbd = dA ? (int)column_blocks(D) : 0, nbn = dB ? (int)column_blocks(N) : 0;
+  const GradArgs a = {x, dy, lo, dlo, plan, lay, (int)D, (int)N, (int)r, mid_pitch(r), nbd, T_, dA, dB, part};
+  return by_type(dtype, r, aligned_widths(D, N, r), [&](auto tc, auto rc, auto vc) -> int {
     using T = decltype(tc);
     constexpr int RP = decltype(rc)::value;
     constexpr bool VEC = decltype(vc)::value;
@@ -295,29 +345,22 @@ int launch_grads(const void* x, const void* dy, const float* lo, const float* dl
     constexpr int smem = GradCfg<RP>::SMEM;
     const int rc2 = allow_smem((const void*)kern, smem, "cudaFuncSetAttribute(lora grads)");
     if (rc2) return rc2;
-    // the split of the tokens with the shortest estimate, for adapters of equal
-    // shares: rounds of co-resident clusters x (stages of a part + 5)
-    const int64_t blocks = (int64_t)(a.nbd + nbn) * L, nst = (T_ + TK * L - 1) / (TK * L);
-    int S = 1;
-    int64_t best = INT64_MAX;
-    for (int s = 1; s <= 8 && (s == 1 || T_ >= 4 * TK * s); ++s) {
-      const int64_t fit = resident_clusters((const void*)kern, THREADS, smem, s);
-      const int64_t cost = ((blocks + fit - 1) / fit) * ((nst + s - 1) / s + 5);
-      if (cost < best) best = cost, S = s;
+    // as in grads_part_bytes, whichever gradients are wanted
+    const int S = parts_of<T, RP, VEC>(T_, (column_blocks(D) + column_blocks(N)) * L, L);
+    kern<<<dim3((unsigned)(nbd + nbn), (unsigned)L, (unsigned)S), THREADS, smem, st>>>(a, S);
+    if (S > 1) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(nbd + nbn), (unsigned)L);
+      cfg.blockDim = dim3(THREADS);
+      cfg.stream = st;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[0].val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      cudaLaunchKernelEx(&cfg, lora_grads_join_kernel<T, RP>, a, S);
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.nbd + nbn), (unsigned)L, (unsigned)S);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = (unsigned)S;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&cfg, kern, a, S), "lora_grads launch");
+    return check_cuda(cudaGetLastError(), "lora_grads launch");
   });
 }
 

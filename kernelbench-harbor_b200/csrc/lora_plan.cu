@@ -123,8 +123,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int64_t* __res
 }
 
 int launch_grads(const void* x, const void* dy, const float* lo, const float* dlo, const int32_t* plan,
-                 const PlanLayout& lay, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype, void* dA,
-                 void* dB, cudaStream_t st);
+                 const PlanLayout& lay, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype, float* part,
+                 void* dA, void* dB, cudaStream_t st);
+size_t grads_part_bytes(int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype);
 
 // Up to this many tokens the one-launch cluster kernel runs, above it the
 // tiled pair.
@@ -202,26 +203,39 @@ int b200q_lora_apply(const void* x, const void* base, const void* A, const void*
   return launch(a, dtype, false, reinterpret_cast<cudaStream_t>(stream));
 }
 
+size_t b200q_lora_backward_scratch_bytes(int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype) {
+  using namespace b200q::lora;
+  if (check_sizes("lora_backward", T, D, N, r, L, dtype) || T == 0) return 0;
+  return b200q_lora_mid_bytes(T, r) + grads_part_bytes(T, D, N, r, L, dtype);
+}
+
 int b200q_lora_backward(const void* x, const void* dy, const void* base, const void* A, const void* B,
                         const float* scaling, const int32_t* plan, const float* lo, int64_t T, int64_t D, int64_t N,
-                        int64_t r, int64_t L, int dtype, float* dlo, void* dx, void* dA, void* dB, void* workspace,
-                        void* stream) {
+                        int64_t r, int64_t L, int dtype, void* scratch, size_t scratch_bytes, void* dx, void* dA,
+                        void* dB, void* workspace, void* stream) {
   using namespace b200q;
   using namespace b200q::lora;
   int rc = check_sizes("lora_backward", T, D, N, r, L, dtype);
   if (rc) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool need_dlo = dx || dA;
-  if (T > 0 && (!plan || !dy || (need_dlo && (!A || !B || !dlo)) || (dA && !x) || (dB && !lo)))
+  if (!dx && !dA && !dB) return B200Q_OK;
+  if (T > 0 && (!plan || !dy || (need_dlo && (!A || !B)) || (dA && !x) || (dB && !lo)))
     return fail(B200Q_ERR_SHAPE, "lora_backward: null pointer argument");
-  if (misaligned({x, dy, base, A, B, plan, lo, dlo, dx, dA, dB}))
+  if (misaligned({x, dy, base, A, B, plan, lo, scratch, dx, dA, dB}))
     return fail(B200Q_ERR_ALIGN, "lora_backward: pointers must be 16-byte aligned");
+  if (T > 0 && (!scratch || scratch_bytes < b200q_lora_backward_scratch_bytes(T, D, N, r, L, dtype)))
+    return fail(B200Q_ERR_WORKSPACE, "lora_backward: scratch of " +
+                                         std::to_string(b200q_lora_backward_scratch_bytes(T, D, N, r, L, dtype)) +
+                                         " bytes required");
+  float* dlo = reinterpret_cast<float*>(scratch);
+  float* part = dlo + b200q_lora_mid_bytes(T, r) / 4;
   if (T > 0 && need_dlo) {
     const Args a = {dy, base, B, A, scaling, plan, plan_layout(T, L), (int)N, (int)D, (int)r, mid_pitch(r), dx, dlo, T, L,
                     reinterpret_cast<int*>(workspace)};
     if ((rc = launch(a, dtype, true, st))) return rc;
   }
-  return dA || dB ? launch_grads(x, dy, lo, dlo, plan, plan_layout(T, L), T, D, N, r, L, dtype, dA, dB, st) : B200Q_OK;
+  return dA || dB ? launch_grads(x, dy, lo, dlo, plan, plan_layout(T, L), T, D, N, r, L, dtype, part, dA, dB, st) : B200Q_OK;
 }
 
 }  // extern "C"

@@ -644,14 +644,17 @@ def _lora_backward(ctx, dy):
     dx = torch.empty_like(x) if need_x else None
     dA = torch.empty_like(A) if need_A else None
     dB = torch.empty_like(B) if need_B else None
-    dlo = torch.empty_like(lo) if need_x or need_A else None
     if need_x or need_A or need_B:
         n_adapters, D, r = A.shape
+        sizes = (x.shape[0], D, B.shape[2], r, n_adapters, _dtype_code(x.dtype))
+        L = _lib.lib()
         with _device(dev):
-            _lib.check(_lib.lib().b200q_lora_backward(
+            nbytes = L.b200q_lora_backward_scratch_bytes(*sizes)
+            scratch = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+            _lib.check(L.b200q_lora_backward(
                 x.data_ptr(), d.data_ptr(), None, A.data_ptr(), B.data_ptr(), _ptr(scaling), ctx.plan.data_ptr(),
-                lo.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters, _dtype_code(x.dtype), _ptr(dlo), _ptr(dx),
-                _ptr(dA), _ptr(dB), workspace(dev, 256).data_ptr(), _stream_ptr(dev)))
+                lo.data_ptr(), *sizes, scratch.data_ptr(), nbytes, _ptr(dx), _ptr(dA), _ptr(dB),
+                workspace(dev, 256).data_ptr(), _stream_ptr(dev)))
     return dy if need_base else None, dx, dA, dB, None, None
 
 

@@ -452,11 +452,16 @@ def test_refusals_without_gpu():
     assert call(dtype=2) == _lib.ERR_UNSUPPORTED
     assert call(T=0) == _lib.OK
 
-    def back(T=64, r=8, x=p, dy=p, A=p, dx=p, dA=p, dB=p, lo=p, dlo=p):
-        return L.b200q_lora_backward(x, dy, None, A, p, None, p, lo, T, 64, 64, r, 4, 0, dlo, dx, dA, dB, None, None)
+    need = L.b200q_lora_backward_scratch_bytes(64, 64, 64, 8, 4, 0)
+    assert need >= L.b200q_lora_mid_bytes(64, 8) > 0
+    assert L.b200q_lora_backward_scratch_bytes(64, 64, 64, 65, 4, 0) == 0
+
+    def back(T=64, r=8, x=p, dy=p, A=p, dx=p, dA=p, dB=p, lo=p, scratch=p, nbytes=need):
+        return L.b200q_lora_backward(x, dy, None, A, p, None, p, lo, T, 64, 64, r, 4, 0, scratch, nbytes, dx, dA, dB,
+                                     None, None)
 
     assert back(x=None) == back(dy=None) == back(A=None) == back(lo=None) == back(r=65) == _lib.ERR_SHAPE
-    assert back(dlo=None) == back(dlo=None, dA=None, dB=None) == _lib.ERR_SHAPE
+    assert back(scratch=None) == back(nbytes=need - 4) == _lib.ERR_WORKSPACE
     assert back(dB=8) == back(dx=4) == _lib.ERR_ALIGN
     assert back(dx=None, dA=None, dB=None) == back(T=0, dA=None, dB=None) == _lib.OK
 
