@@ -162,9 +162,7 @@ class LoRAW4A16Linear(nn.Module):
         lead = x.shape[:-1]
         x2 = x.reshape(-1, K)
         ids = lora_ids.reshape(-1) if isinstance(lora_ids, torch.Tensor) else lora_ids
-        base = ops.w4a16_gemm(x2, qweight, scales, zeros, K // scales.shape[0])
-        grad = torch.is_grad_enabled() and (base.requires_grad or A.requires_grad or B.requires_grad)
-        y = ops.lora_apply(base, x2, A, B, ids, scaling, out=None if grad else base)
+        y = ops.lora_w4a16(x2, qweight, scales, zeros, K // scales.shape[0], A, B, ids, scaling)
         return y.reshape(*lead, y.shape[-1])
 
 

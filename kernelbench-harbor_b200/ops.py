@@ -635,27 +635,94 @@ class _LoraApply(torch.autograd.Function):
         return _once(_lora_backward, ctx, dy)
 
 
-def _lora_backward(ctx, dy):
-    x, A, B, scaling = ctx.saved_tensors
-    lo = ctx.lo
-    need_base, need_x, need_A, need_B = ctx.needs_input_grad[:4]
-    dev = x.device
-    d = _aligned(dy)
-    dx = torch.empty_like(x) if need_x else None
+def _lora_grads(ctx, x, A, B, scaling, d, dx, base, need_A, need_B):
+    """dA and dB; and dx (if given) = base (None: 0) + the adapters' part."""
     dA = torch.empty_like(A) if need_A else None
     dB = torch.empty_like(B) if need_B else None
+    n_adapters, D, r = A.shape
+    sizes = (x.shape[0], D, B.shape[2], r, n_adapters, _dtype_code(x.dtype))
+    dev = x.device
+    L = _lib.lib()
+    with _device(dev):
+        nbytes = L.b200q_lora_backward_scratch_bytes(*sizes)
+        scratch = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        _lib.check(L.b200q_lora_backward(
+            x.data_ptr(), d.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling), ctx.plan.data_ptr(),
+            ctx.lo.data_ptr(), *sizes, scratch.data_ptr(), nbytes, _ptr(dx), _ptr(dA), _ptr(dB),
+            workspace(dev, 256).data_ptr(), _stream_ptr(dev)))
+    return dA, dB
+
+
+def _lora_backward(ctx, dy):
+    x, A, B, scaling = ctx.saved_tensors
+    need_base, need_x, need_A, need_B = ctx.needs_input_grad[:4]
+    dx = torch.empty_like(x) if need_x else None
+    dA = dB = None
     if need_x or need_A or need_B:
-        n_adapters, D, r = A.shape
-        sizes = (x.shape[0], D, B.shape[2], r, n_adapters, _dtype_code(x.dtype))
-        L = _lib.lib()
-        with _device(dev):
-            nbytes = L.b200q_lora_backward_scratch_bytes(*sizes)
-            scratch = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-            _lib.check(L.b200q_lora_backward(
-                x.data_ptr(), d.data_ptr(), None, A.data_ptr(), B.data_ptr(), _ptr(scaling), ctx.plan.data_ptr(),
-                lo.data_ptr(), *sizes, scratch.data_ptr(), nbytes, _ptr(dx), _ptr(dA), _ptr(dB),
-                workspace(dev, 256).data_ptr(), _stream_ptr(dev)))
+        dA, dB = _lora_grads(ctx, x, A, B, scaling, _aligned(dy), dx, None, need_A, need_B)
     return dy if need_base else None, dx, dA, dB, None, None
+
+
+class _LoRAW4A16(torch.autograd.Function):
+    """w4a16_gemm with lora_apply in place on its output; one gradient of x for both."""
+
+    @staticmethod
+    def forward(ctx, x, A, B, qweight, scales, zeros, group, scaling, plan):
+        x, A, B = _aligned(x), _aligned(A), _aligned(B)
+        y, lo = w4a16_gemm(x, qweight, scales, zeros, group), _lora_mid(x, A.shape[2])
+        _lora_run(x, y, A, B, scaling, plan.data, y, lo)
+        ctx.save_for_backward(x, A, B, scaling, qweight, scales, zeros)
+        ctx.lo, ctx.plan, ctx.group = lo, plan.data, group
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _once(_lora_w4a16_backward, ctx, dy)
+
+
+def _lora_w4a16_backward(ctx, dy):
+    x, A, B, scaling, qweight, scales, zeros = ctx.saved_tensors
+    need_x, need_A, need_B, _, need_scales, need_zeros = ctx.needs_input_grad[:6]
+    if need_scales or need_zeros:
+        raise RuntimeError("lora_w4a16: the quantised weight is frozen, scales and zeros have no gradient")
+    d = _aligned(dy)
+    dx = w4a16_dgrad(d, qweight, scales, zeros, ctx.group) if need_x else None
+    dA, dB = _lora_grads(ctx, x, A, B, scaling, d, dx, dx, need_A, need_B)
+    return dx, dA, dB, None, None, None, None, None, None
+
+
+def _lora_check(op, x, A, B, plan, scaling):
+    """Checks the adapter operands that lora_apply and lora_w4a16 share; returns
+    A and B in x's dtype, the plan and scaling as fp32."""
+    if not x.is_cuda:
+        raise RuntimeError(f"b200q {op} runs on CUDA tensors only")
+    if x.dim() != 2 or A.dim() != 3 or B.dim() != 3:
+        raise ValueError(f"{op}: x [T, D], A [L, D, r] and B [L, r, N] expected")
+    T, D = x.shape
+    n_adapters, Da, r = A.shape
+    Lb, rb, _ = B.shape
+    if Da != D or Lb != n_adapters or rb != r:
+        raise ValueError(f"{op}: shapes do not fit: x {tuple(x.shape)}, A {tuple(A.shape)}, B {tuple(B.shape)}")
+    dt = x.dtype
+    _dtype_code(dt)
+    if isinstance(plan, torch.Tensor):
+        plan = lora_plan(plan, n_adapters)
+    if plan.tokens != T or plan.adapters != n_adapters:
+        raise ValueError(f"{op}: the plan is for {plan.tokens} tokens and {plan.adapters} adapters, "
+                         f"not {T} and {n_adapters}")
+    _same_device(op, x, A, B, plan.data, scaling)
+    if scaling is not None:
+        if scaling.shape != (n_adapters,):
+            raise ValueError(f"{op}: scaling must be [{n_adapters}]")
+        if scaling.requires_grad:
+            raise ValueError(f"{op}: scaling is a constant and has no gradient")
+        if scaling.dtype != torch.float32 or not scaling.is_contiguous():
+            scaling = scaling.to(torch.float32).contiguous()
+    if A.dtype != dt:
+        A = A.to(dt)
+    if B.dtype != dt:
+        B = B.to(dt)
+    return A, B, plan, scaling
 
 
 def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
@@ -670,37 +737,13 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     fp32; y is rounded once.  Differentiable in base, x, A and B (scaling is a
     constant).  ``out`` (which may be ``base``: in place) takes the result
     where no gradient is wanted."""
-    if not x.is_cuda:
-        raise RuntimeError("b200q lora_apply runs on CUDA tensors only")
-    if x.dim() != 2 or A.dim() != 3 or B.dim() != 3:
-        raise ValueError("lora_apply: base [T, N], x [T, D], A [L, D, r] and B [L, r, N] expected")
-    T, D = x.shape
-    n_adapters, Da, r = A.shape
-    Lb, rb, N = B.shape
-    if base.shape != (T, N) or Da != D or Lb != n_adapters or rb != r:
-        raise ValueError(f"lora_apply: shapes do not fit: base {tuple(base.shape)}, x {tuple(x.shape)}, "
-                         f"A {tuple(A.shape)}, B {tuple(B.shape)}")
-    dt = x.dtype
-    _dtype_code(dt)
+    A, B, plan, scaling = _lora_check("lora_apply", x, A, B, plan, scaling)
+    if base.shape != (x.shape[0], B.shape[2]):
+        raise ValueError(f"lora_apply: base must be [{x.shape[0]}, {B.shape[2]}], got {tuple(base.shape)}")
+    T, dt = x.shape[0], x.dtype
     if base.dtype != dt:
         raise TypeError(f"lora_apply: base is {base.dtype}, x is {dt}")
-    if isinstance(plan, torch.Tensor):
-        plan = lora_plan(plan, n_adapters)
-    if plan.tokens != T or plan.adapters != n_adapters:
-        raise ValueError(f"lora_apply: the plan is for {plan.tokens} tokens and {plan.adapters} adapters, "
-                         f"not {T} and {n_adapters}")
-    _same_device("lora_apply", x, base, A, B, plan.data, scaling, out)
-    if scaling is not None:
-        if scaling.shape != (n_adapters,):
-            raise ValueError(f"lora_apply: scaling must be [{n_adapters}]")
-        if scaling.requires_grad:
-            raise ValueError("lora_apply: scaling is a constant and has no gradient")
-        if scaling.dtype != torch.float32 or not scaling.is_contiguous():
-            scaling = scaling.to(torch.float32).contiguous()
-    if A.dtype != dt:
-        A = A.to(dt)
-    if B.dtype != dt:
-        B = B.to(dt)
+    _same_device("lora_apply", x, base, out)
     if torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad or base.requires_grad):
         if out is not None:
             raise ValueError("lora_apply: out cannot be given where a gradient is wanted")
@@ -710,7 +753,7 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
         base = _aligned(base)
         out = torch.empty_like(base)
     else:
-        if out.shape != (T, N) or out.dtype != dt or not out.is_contiguous() or out.data_ptr() % 16:
+        if out.shape != base.shape or out.dtype != dt or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("lora_apply: out must be a contiguous, 16-byte aligned [T, N] tensor of x's dtype")
         if out is not base:
             base = _aligned(base)
@@ -718,9 +761,30 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     if out_given and (any(_overlap(out, t) for t in (x, A, B)) or (out.data_ptr() != base.data_ptr() and _overlap(out, base))):
         raise ValueError("lora_apply: out shares memory with an input (it may be base itself)")
     # the one-launch kernel needs no room for the row between
-    lo = None if T <= _LORA_SMALL else _lora_mid(x, r)
+    lo = None if T <= _LORA_SMALL else _lora_mid(x, A.shape[2])
     _lora_run(x, base, A, B, scaling, plan.data, out, lo)
     return out
+
+
+def lora_w4a16(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor, group: int,
+               A: torch.Tensor, B: torch.Tensor, plan: Union[LoraPlan, torch.Tensor],
+               scaling: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """w4a16_gemm(x, qweight, scales, zeros, group) with lora_apply's adapters
+    beside it, in place on the projection's output.  Differentiable in x, A and
+    B: x's gradient is w4a16_dgrad's with the adapters' part added to it in
+    place."""
+    A, B, plan, scaling = _lora_check("lora_w4a16", x, A, B, plan, scaling)
+    if qweight.dim() != 2 or qweight.shape[1] * 8 != B.shape[2]:
+        raise ValueError(f"lora_w4a16: qweight {tuple(qweight.shape)} does not fit B {tuple(B.shape)}")
+    _same_device("lora_w4a16", x, qweight, scales, zeros)
+    if torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad):
+        return _LoRAW4A16.apply(x, A, B, qweight, scales, zeros, group, scaling, plan)
+    y = w4a16_gemm(x, qweight, scales, zeros, group)
+    x = _aligned(x)
+    lo = None if x.shape[0] <= _LORA_SMALL else _lora_mid(x, A.shape[2])
+    with torch.no_grad():
+        _lora_run(x, y, _aligned(A), _aligned(B), scaling, plan.data, y, lo)
+    return y
 
 
 def moe_gather(x: torch.Tensor, slot_token: torch.Tensor) -> torch.Tensor:

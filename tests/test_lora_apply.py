@@ -361,11 +361,25 @@ def test_module_forward_and_gradients(T):
     dy = c["dy"].double()
     dlo, part, edlo, edx = pair(c["dy"], c["B"].transpose(1, 2), c["A"].transpose(1, 2), c["scaling"], c["ids"])
     u = 2.0 ** -8
-    # the frozen weight's bf16 rounding, both summands' and the sum's
+    # the frozen weight's bf16 rounding, the first summand's and the sum's
     S = dy.abs() @ w.abs().t()
     full = dy @ w.t()
     assert ((dx.double() - full - part).abs() <= edx + (u + 1e-5) * S + 2.1 * u * (full.abs() + part.abs())).all()
     close(dA, *grads(x, dlo, edlo, c["ids"], 3), torch.bfloat16)
+    lo, _, elo, _ = pair(x, c["A"], c["B"], c["scaling"], c["ids"])
+    wB, eB = grads(c["dy"], lo, elo, c["ids"], 3)
+    close(dB, wB.transpose(1, 2), eB.transpose(1, 2), torch.bfloat16)
+    # one gradient at a time, and the operator that the module calls
+    for i, want in enumerate((dx, dA, dB)):
+        one = [t.detach().requires_grad_(i == k) for k, t in enumerate(leaves)]
+        y = ops.lora_w4a16(one[0], q, s, z, 128, one[1], one[2], c["ids"], c["scaling"])
+        assert torch.equal(torch.autograd.grad(y, one[i], c["dy"])[0], want)
+    with pytest.raises(RuntimeError, match="frozen"):
+        ops.lora_w4a16(leaves[0], q, s.clone().requires_grad_(), z, 128, c["A"], c["B"], c["ids"]).sum().backward()
+    for bad in ((x, q[:, :16], s, z, 128, c["A"], c["B"]), (x, q, s, z, 64, c["A"], c["B"]),
+                (x[:, :256], q, s, z, 128, c["A"], c["B"]), (x.float(), q, s, z, 128, c["A"], c["B"])):
+        with pytest.raises((ValueError, TypeError)):
+            ops.lora_w4a16(*bad, c["ids"])
 
 
 @pytest.mark.gpu
