@@ -35,7 +35,7 @@ struct SmallCfg {
 };
 
 template <class T, int RP, bool TR, bool VEC>
-__global__ void __launch_bounds__(THREADS) lora_small_kernel(const Args a) {
+__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(THREADS) lora_small_kernel(const Args a) {
   using C = SmallCfg<RP>;
   extern __shared__ __align__(16) uint8_t sm[];
   const int32_t* plan = a.plan;
@@ -316,19 +316,8 @@ int launch_small(const Args& a, int dtype, bool tr, cudaStream_t st) {
     constexpr int smem = SmallCfg<RP>::SMEM;
     const int rc2 = allow_smem((const void*)kern, smem, "cudaFuncSetAttribute(lora small)");
     if (rc2) return rc2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.lay.max_small * CL));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CL;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&cfg, kern, a), "lora_apply launch");
+    kern<<<(unsigned)(a.lay.max_small * CL), THREADS, smem, st>>>(a);
+    return check_cuda(cudaGetLastError(), "lora_apply launch");
   });
 }
 

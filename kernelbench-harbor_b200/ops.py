@@ -93,8 +93,9 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _same_device(op: str, first: torch.Tensor, *rest: Optional[torch.Tensor]) -> None:
+    d = first.get_device()
     for t in rest:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != d:
             raise ValueError(f"{op}: tensors on {first.device} and {t.device}")
 
 
@@ -608,12 +609,15 @@ def lora_plan(lora_ids: torch.Tensor, n_adapters: int) -> LoraPlan:
 def _lora_run(x, base, A, B, scaling, plan, out, lo):
     """One b200q_lora_apply call on contiguous, aligned tensors."""
     n_adapters, D, r = A.shape
+    T = x.shape[0]
     dev = x.device
     with _device(dev):
-        _lib.check(_lib.lib().b200q_lora_apply(x.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling),
-                                               plan.data_ptr(), x.shape[0], D, B.shape[2], r, n_adapters,
-                                               _dtype_code(x.dtype), out.data_ptr(), _ptr(lo),
-                                               workspace(dev, 256).data_ptr(), _stream_ptr(dev)))
+        # the one-launch kernel has no wait that could run out
+        status = None if T <= _LORA_SMALL else workspace(dev, 256).data_ptr()
+        _lib.check(_lib.lib().b200q_lora_apply(x.data_ptr(), base.data_ptr(), A.data_ptr(), B.data_ptr(), _ptr(scaling),
+                                               plan.data_ptr(), T, D, B.shape[2], r, n_adapters,
+                                               _dtype_code(x.dtype), out.data_ptr(), _ptr(lo), status,
+                                               _stream_ptr(dev)))
 
 
 def _lora_mid(x: torch.Tensor, r: int) -> torch.Tensor:
@@ -738,9 +742,9 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     constant).  ``out`` (which may be ``base``: in place) takes the result
     where no gradient is wanted."""
     A, B, plan, scaling = _lora_check("lora_apply", x, A, B, plan, scaling)
-    if base.shape != (x.shape[0], B.shape[2]):
-        raise ValueError(f"lora_apply: base must be [{x.shape[0]}, {B.shape[2]}], got {tuple(base.shape)}")
     T, dt = x.shape[0], x.dtype
+    if base.shape != (T, B.shape[2]):
+        raise ValueError(f"lora_apply: base must be [{T}, {B.shape[2]}], got {tuple(base.shape)}")
     if base.dtype != dt:
         raise TypeError(f"lora_apply: base is {base.dtype}, x is {dt}")
     _same_device("lora_apply", x, base, out)
