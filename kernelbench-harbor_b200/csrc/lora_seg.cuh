@@ -1,5 +1,5 @@
 // Shared pieces of the multi-adapter kernels (lora_plan.cu, lora_small.cu,
-// lora_tiles.cu, lora_grads.cu): adapters of many requests beside one shared
+// lora_tiles.cu, lora_shrink_tc.cu, lora_grads.cu): adapters of many requests beside one shared
 // projection,
 //   y[t]  = base[t] + s[id_t] (x[t] . A[id_t]) . B[id_t]
 //   dx[t] = base[t] + s[id_t] (dy[t] . B[id_t]^T) . A[id_t]^T
@@ -9,13 +9,13 @@
 // rows shares one adapter and the products run on the tensor cores; mid, the
 // row between the two (s included), stays in fp32.
 //
-// mma.sync m16n8k16 is used, not tcgen05: the operators read and write wide
-// rows once and do 2 r flops per value (r <= 64), so memory bounds them
-// up to r = 64 and the register fragments let a row go from HBM into the
-// multiply without shared memory: of the contraction index, any order serves
-// that both operands share, so a thread takes 8 consecutive values of a row
-// (one 16-byte load) as its parts of two k16 steps; of the output columns, the
-// order is chosen so that a thread ends with 8 consecutive ones.
+// Wide rows are read and written once and take 2 r flops per value (r <= 64), so
+// memory is the bound.  Most products use mma.sync m16n8k16, whose register
+// fragments fit wide rows: of the contraction index, any order serves that both
+// operands share, so a thread takes 8 consecutive values of a row (one 16-byte
+// load) as its parts of two k16 steps; of the output columns, the order is
+// chosen so that a thread ends with 8 consecutive ones.  From rank 33 on the
+// fragments of P cost more than the rows, and shrink runs on tcgen05.
 #pragma once
 #include <type_traits>
 #include <utility>
