@@ -14,7 +14,8 @@
 // cluster the parts would need no second launch, but clusters of 3 fill only
 // 142 x 3 of the SMs' 444 places: 144 column blocks took two rounds.)
 // Bound: HBM, x and dy once; at r = 64 the legacy tensor rate is as near (two
-// halves: 4 T r (D + N) flop).
+// halves: 4 T r (D + N) flop).  Measured, one adapter, 8192 tokens, 4096 + 14336
+// columns (302 MB), r = 16: 63 us, 4.8 TB/s; the copies alone take 52.
 #include <type_traits>
 
 #include "lora_seg.cuh"
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 2) lora_gra
   const int seg = blockIdx.y, rank = blockIdx.z;
   const int b0 = a.plan[a.lay.seg + seg], b1 = a.plan[a.lay.seg + seg + 1];
   const int nst_all = (b1 - b0 + TK - 1) / TK;
-  // whole stages per rank
+  // whole stages per part
   const int f0 = b0 + (int)((int64_t)rank * nst_all / S) * TK;
   const int f1 = min(b1, b0 + (int)((int64_t)(rank + 1) * nst_all / S) * TK);
   const int nst = (f1 - f0 + TK - 1) / TK;

@@ -14,6 +14,8 @@
 // and y pass as 16-byte pieces.  A warp takes 16 rows; mid is split into two
 // halves of the type once, in registers, and serves all the CTA's columns.
 // Bound: HBM -- x once, base once, y once; mid (4 r bytes a token) stays in L2.
+// Measured, 8192 tokens, r = 16: shrink of 14336 columns (235 MB) 42.6 us, 5.5
+// TB/s; expand to 14336 columns (470 MB) 79 us, 5.9 TB/s.
 #include <algorithm>
 #include <type_traits>
 
