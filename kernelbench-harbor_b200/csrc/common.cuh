@@ -92,8 +92,10 @@ int current_device();
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize), once per kernel and device
 // (`kernel` identifies the instantiation: its host-side function pointer)
 int allow_smem(const void* kernel, int bytes, const char* what);
-// Clusters of `size` CTAs that fit on the current device at once (looked up once per kernel, size and device)
-int resident_clusters(const void* kernel, int threads, int smem, int size);
+// Clusters of s CTAs that fit on the current device at once, s = 1 .. 8 at
+// [s] (found once per kernel, shared-memory size and device); sets the kernel's
+// shared-memory attribute first
+const int* resident_clusters(const void* kernel, int threads, int smem);
 
 // encodes a 2D tiled tensor map; returns 0 or a negative b200q status
 int encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner,

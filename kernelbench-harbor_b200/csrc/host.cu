@@ -1,6 +1,7 @@
 // Host-side plumbing shared by every entry point: error strings, device
 // properties, tensor-map encoding through the driver entry point, the device
 // status word.
+#include <array>
 #include <atomic>
 #include <map>
 #include <mutex>
@@ -61,31 +62,33 @@ int allow_smem(const void* kernel, int bytes, const char* what) {
   return rc;
 }
 
-int resident_clusters(const void* kernel, int threads, int smem, int size) {
+const int* resident_clusters(const void* kernel, int threads, int smem) {
   static std::mutex mu;
-  static std::map<std::tuple<const void*, int, int, int>, int> known;
-  const auto key = std::make_tuple(kernel, smem, size, current_device());
+  static std::map<std::tuple<const void*, int, int>, std::array<int, 9>> known;  // nodes stay where they are
+  allow_smem(kernel, smem, "cudaFuncSetAttribute");
+  const auto key = std::make_tuple(kernel, smem, current_device());
   std::lock_guard<std::mutex> lk(mu);
   auto it = known.find(key);
-  if (it != known.end()) return it->second;
-  cudaLaunchConfig_t q = {};
-  q.gridDim = dim3((unsigned)size);
-  q.blockDim = dim3((unsigned)threads);
-  q.dynamicSmemBytes = (size_t)smem;
-  cudaLaunchAttribute a[1];
-  a[0].id = cudaLaunchAttributeClusterDimension;
-  a[0].val.clusterDim.x = (unsigned)size;
-  a[0].val.clusterDim.y = 1;
-  a[0].val.clusterDim.z = 1;
-  q.attrs = a;
-  q.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kernel, &q) != cudaSuccess || n < 1) {
-    cudaGetLastError();
-    n = 1;
+  if (it != known.end()) return it->second.data();
+  std::array<int, 9> fit = {};
+  for (int size = 1; size <= 8; ++size) {
+    cudaLaunchConfig_t q = {};
+    q.gridDim = dim3((unsigned)size);
+    q.blockDim = dim3((unsigned)threads);
+    q.dynamicSmemBytes = (size_t)smem;
+    cudaLaunchAttribute a[1];
+    a[0].id = cudaLaunchAttributeClusterDimension;
+    a[0].val.clusterDim.x = (unsigned)size;
+    a[0].val.clusterDim.y = 1;
+    a[0].val.clusterDim.z = 1;
+    q.attrs = a;
+    q.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&fit[size], kernel, &q) != cudaSuccess || fit[size] < 1) {
+      cudaGetLastError();
+      fit[size] = 1;
+    }
   }
-  known[key] = n;
-  return n;
+  return known.emplace(key, fit).first->second.data();
 }
 
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

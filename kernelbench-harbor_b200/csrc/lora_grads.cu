@@ -300,7 +300,7 @@ constexpr int MAX_PARTS = 8;
 // where the column blocks leave places free, so the parts' sums stay small.
 template <class T, int RP, bool VEC>
 int parts_of(int64_t T_, int64_t blocks, int64_t L) {
-  const int64_t fit = resident_clusters((const void*)lora_grads_kernel<T, RP, VEC>, THREADS, GradCfg<RP>::SMEM, 1);
+  const int64_t fit = resident_clusters((const void*)lora_grads_kernel<T, RP, VEC>, THREADS, GradCfg<RP>::SMEM)[1];
   const int64_t nst = (T_ + TK * L - 1) / (TK * L);
   int S = 1;
   int64_t best = INT64_MAX;
@@ -318,7 +318,6 @@ size_t grads_part_bytes(int64_t T_, int64_t D, int64_t N, int64_t r, int64_t L, 
   by_type(dtype, r, aligned_widths(D, N, r), [&](auto tc, auto rc, auto vc) -> int {
     using T = decltype(tc);
     constexpr int RP = decltype(rc)::value;
-    allow_smem((const void*)lora_grads_kernel<T, RP, decltype(vc)::value>, GradCfg<RP>::SMEM, "cudaFuncSetAttribute(lora grads)");
     const int64_t blocks = (column_blocks(D) + column_blocks(N)) * L;
     const int S = parts_of<T, RP, decltype(vc)::value>(T_, blocks, L);
     bytes = S > 1 ? (size_t)S * blocks * (RP * CT) * 4 : 0;

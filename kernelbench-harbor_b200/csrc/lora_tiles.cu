@@ -509,13 +509,14 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_ke
 // contraction that has the shortest estimate: rounds of co-resident clusters x
 // (stages of a part + 5 for start, joining and ending), for about half a tile
 // more than T / 128 with each adapter that ends inside one.
-template <class Kern, class Fit>
-int launch_split(Kern kern, int threads, int smem, const Args& a, cudaStream_t st, Fit fit) {
+// `fit`: resident_clusters of the kernel, `per`: times as many really fit.
+template <class Kern>
+int launch_split(Kern kern, int threads, int smem, const Args& a, cudaStream_t st, const int* fit, int per) {
   const int64_t whole = (a.T + ROWS_L - 1) / ROWS_L, tiles = whole + std::min(a.L, whole) / 2, nst = (a.D + SK - 1) / SK;
   int S = 1;
   int64_t best = INT64_MAX;
   for (int s = 1; s <= MAX_SPLIT && (s == 1 || nst >= 4 * s); ++s) {
-    const int64_t at_once = fit(s), cost = ((tiles + at_once - 1) / at_once) * ((nst + s - 1) / s + 5);
+    const int64_t at_once = (int64_t)per * fit[s], cost = ((tiles + at_once - 1) / at_once) * ((nst + s - 1) / s + 5);
     if (cost < best) best = cost, S = s;
   }
   cudaLaunchConfig_t cfg = {};
@@ -545,7 +546,7 @@ int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
     int status = allow_smem((const void*)expand, smem_e, "cudaFuncSetAttribute(lora expand)");
     if (status) return status;
     const int64_t whole = (a.T + ROWS_L - 1) / ROWS_L, tiles = whole + std::min(a.L, whole) / 2;
-    const int64_t nsteps = (a.N + SK - 1) / SK, slots = resident_clusters((const void*)expand, THREADS, smem_e, 1);
+    const int64_t nsteps = (a.N + SK - 1) / SK, slots = resident_clusters((const void*)expand, THREADS, smem_e)[1];
     int steps = 2;
     int64_t best = INT64_MAX;
     for (int s = 2; s <= 16; ++s) {
@@ -564,13 +565,12 @@ int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
       // the occupancy query counts a kernel with tensor memory once per SM; its 64 of 512 columns and its shared memory
       // let two share one
       status = launch_split(reinterpret_cast<ShrinkFn>(const_cast<void*>(kern)), SHRINK_TC_THREADS, SHRINK_TC_SMEM, a, st,
-                            [&](int s) { return 2 * resident_clusters(kern, SHRINK_TC_THREADS, SHRINK_TC_SMEM, s); });
+                            resident_clusters(kern, SHRINK_TC_THREADS, SHRINK_TC_SMEM), 2);
     } else {
       auto shrink = tr ? lora_shrink_tile_kernel<T, RP, true, VEC> : lora_shrink_tile_kernel<T, RP, false, VEC>;
       const int smem_s = tr ? ShrinkCfg<RP, true>::SMEM : ShrinkCfg<RP, false>::SMEM;
       if ((status = allow_smem((const void*)shrink, smem_s, "cudaFuncSetAttribute(lora shrink)"))) return status;
-      status = launch_split(shrink, THREADS, smem_s, a, st,
-                            [&](int s) { return resident_clusters((const void*)shrink, THREADS, smem_s, s); });
+      status = launch_split(shrink, THREADS, smem_s, a, st, resident_clusters((const void*)shrink, THREADS, smem_s), 1);
     }
     if (status || !a.y) return status;  // no y: mid alone was asked for
     // the expand kernel's start overlaps the shrink kernel's end

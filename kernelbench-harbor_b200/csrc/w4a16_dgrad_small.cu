@@ -285,9 +285,9 @@ int w4a16_dgrad_small(const void* dy, const int32_t* qweight, const void* scales
   const int64_t tiles = (K + TILE - 1) / TILE, chunks = (N + CHUNK - 1) / CHUNK;
   int S = 1;
   int64_t best = INT64_MAX;
+  const int* fit = resident_clusters((const void*)kern, THREADS, SMEM);
   for (int s = 1; s <= MAX_S && (s == 1 || s * WARPS < chunks + WARPS); s *= 2) {
-    const int64_t fit = resident_clusters((const void*)kern, THREADS, SMEM, s);
-    const int64_t cost = ((tiles + fit - 1) / fit) * ((chunks + s * WARPS - 1) / (s * WARPS) + 2);
+    const int64_t cost = ((tiles + fit[s] - 1) / fit[s]) * ((chunks + s * WARPS - 1) / (s * WARPS) + 2);
     if (cost < best) best = cost, S = s;
   }
   cudaLaunchConfig_t cfg = {};

@@ -8,6 +8,7 @@ and calls the library on the current CUDA stream.  No CPU path exists: a CPU
 tensor is an error."""
 from __future__ import annotations
 
+import functools
 import threading
 from typing import Optional, Union
 
@@ -348,11 +349,16 @@ def _(router_logits):
 _LOGITS_CODES = {torch.float16: _lib.DTYPE_FP16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_FP32}
 
 
+@functools.lru_cache(maxsize=256)
+def _balance_scratch(T: int, E: int) -> int:
+    return _lib.lib().b200q_moe_balance_scratch_bytes(T, E)
+
+
 def _balance_forward(logits, topi, mask):
     T, E = logits.shape
     dev = logits.device
     L = _lib.lib()
-    nbytes = L.b200q_moe_balance_scratch_bytes(T, E)
+    nbytes = _balance_scratch(T, E)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     coef = torch.empty((E + nbytes // 4,), dtype=torch.float32, device=dev)  # the kernel's scratch behind it
     counts = torch.empty((E,), dtype=torch.int32, device=dev)
@@ -620,8 +626,19 @@ def _lora_run(x, base, A, B, scaling, plan, out, lo):
                                                _stream_ptr(dev)))
 
 
+@functools.lru_cache(maxsize=256)
+def _lora_mid_values(T: int, r: int) -> int:
+    return _lib.lib().b200q_lora_mid_bytes(T, r) // 4
+
+
 def _lora_mid(x: torch.Tensor, r: int) -> torch.Tensor:
-    return torch.empty((_lib.lib().b200q_lora_mid_bytes(x.shape[0], r) // 4,), dtype=torch.float32, device=x.device)
+    return torch.empty((_lora_mid_values(x.shape[0], r),), dtype=torch.float32, device=x.device)
+
+
+@functools.lru_cache(maxsize=256)
+def _lora_scratch(T: int, D: int, N: int, r: int, n_adapters: int, dtype: int, device: int) -> int:
+    # the split of the token sums depends on the device (the current one)
+    return _lib.lib().b200q_lora_backward_scratch_bytes(T, D, N, r, n_adapters, dtype)
 
 
 class _LoraApply(torch.autograd.Function):
@@ -644,16 +661,17 @@ def _lora_grads(ctx, x, A, B, scaling, d, dx, base, need_A, need_B):
     dA = torch.empty_like(A) if need_A else None
     dB = torch.empty_like(B) if need_B else None
     n_adapters, D, r = A.shape
-    sizes = (x.shape[0], D, B.shape[2], r, n_adapters, _dtype_code(x.dtype))
+    T = x.shape[0]
+    sizes = (T, D, B.shape[2], r, n_adapters, _dtype_code(x.dtype))
     dev = x.device
-    L = _lib.lib()
     with _device(dev):
-        nbytes = L.b200q_lora_backward_scratch_bytes(*sizes)
+        nbytes = _lora_scratch(*sizes, dev.index)
         scratch = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-        _lib.check(L.b200q_lora_backward(
+        status = None if T <= _LORA_SMALL else workspace(dev, 256).data_ptr()
+        _lib.check(_lib.lib().b200q_lora_backward(
             x.data_ptr(), d.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling), ctx.plan.data_ptr(),
-            ctx.lo.data_ptr(), *sizes, scratch.data_ptr(), nbytes, _ptr(dx), _ptr(dA), _ptr(dB),
-            workspace(dev, 256).data_ptr(), _stream_ptr(dev)))
+            ctx.lo.data_ptr(), *sizes, scratch.data_ptr(), nbytes, _ptr(dx), _ptr(dA), _ptr(dB), status,
+            _stream_ptr(dev)))
     return dA, dB
 
 
