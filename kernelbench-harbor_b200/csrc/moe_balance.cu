@@ -18,9 +18,9 @@
 // that one block adds in block order: no floating-point atomics, the same bits
 // every time.  Counts are integers, where order does not matter.  Batches of
 // at most SINGLE_ELEMS logits take one block and one launch.
-// Measured: 512 tokens, 8 experts 5 us forward, 3 us backward; 131072 tokens, 64
-// experts, fp32 (34 MB) 22 us forward and 14 us backward -- latency of a block's
-// rows, under a host call of 90 us.
+// Measured: 512 tokens, 8 experts 7 us forward and backward; 131072 tokens, 64
+// experts, fp32 (34 MB) 34 us, 18 of them the partial sums -- the latency of a
+// block's rows, under a host call of 90 us.
 #include <algorithm>
 
 #include "common.cuh"
@@ -28,11 +28,11 @@
 namespace b200q {
 namespace balance {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 1024, GRAD_THREADS = 256;
 constexpr int MAX_EXPERTS = 256, MAX_K = 8;
 constexpr int64_t SINGLE_ELEMS = 16384;
-constexpr int MAX_BLOCKS = 296;  // two per SM: few partials to add
-constexpr int UNROLL = 4;        // rows per lane requested before the first is used
+constexpr int MAX_BLOCKS = 148;  // one per SM: few partials to add
+constexpr int UNROLL = 2;        // rows per lane requested before the first is used
 
 template <class T>
 __device__ __forceinline__ float tf(T v);
@@ -236,17 +236,15 @@ __global__ void __launch_bounds__(THREADS) partial_kernel(const T* __restrict__ 
   }
 }
 
-constexpr int FINISH_THREADS = 1024;
-
-__global__ void __launch_bounds__(FINISH_THREADS) finish_kernel(const float* p_part, const int* c_part, const int* n_part,
+__global__ void __launch_bounds__(THREADS) finish_kernel(const float* p_part, const int* c_part, const int* n_part,
                                                          int nb, int E, int k, float* loss, int32_t* counts,
                                                          float* coef) {
   pdl_wait_previous();
-  finish<FINISH_THREADS>(p_part, c_part, n_part, nb, E, k, loss, counts, coef);
+  finish<THREADS>(p_part, c_part, n_part, nb, E, k, loss, counts, coef);
 }
 
 template <class T, int G, bool VEC>
-__global__ void __launch_bounds__(THREADS) grad_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
+__global__ void __launch_bounds__(GRAD_THREADS) grad_kernel(const T* __restrict__ logits, const uint8_t* __restrict__ mask,
                                                        const float* __restrict__ coef,
                                                        const float* __restrict__ dloss, int64_t T_, int E,
                                                        T* __restrict__ dlogits) {
@@ -257,11 +255,16 @@ __global__ void __launch_bounds__(THREADS) grad_kernel(const T* __restrict__ log
   float f[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = e0 + i < E ? coef[e0 + i] : 0.f;
-  const int64_t step = (int64_t)gridDim.x * (THREADS / 32) * RPW;
-  for (int64_t t0 = ((int64_t)blockIdx.x * (THREADS / 32) + warp) * RPW; t0 < T_; t0 += step) {
+  const int64_t step = (int64_t)gridDim.x * (GRAD_THREADS / 32) * RPW;
+  float next[8];  // the row after this one is requested before this one is used
+  int64_t t0 = ((int64_t)blockIdx.x * (GRAD_THREADS / 32) + warp) * RPW;
+  load_row<T, VEC>(logits, mask, t0 + gr, T_, e0, E, next);
+  for (; t0 < T_; t0 += step) {
     const int64_t t = t0 + gr;
     float v[8];
-    load_row<T, VEC>(logits, mask, t, T_, e0, E, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = next[i];
+    load_row<T, VEC>(logits, mask, t + step, T_, e0, E, next);
     const bool live = softmax8<G>(v);
     float dot = 0.f;
 #pragma unroll
@@ -342,7 +345,7 @@ void launch_forward(const void* logits, const int32_t* topi, const uint8_t* mask
   if (nb > 1) {  // its start overlaps the partial kernel's end
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(1);
-    cfg.blockDim = dim3(FINISH_THREADS);
+    cfg.blockDim = dim3(THREADS);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -357,11 +360,11 @@ template <class T>
 void launch_grad(const void* logits, const uint8_t* mask, const float* coef, const float* dloss, int64_t T_, int E,
                  void* dlogits, cudaStream_t st) {
   const int g = lanes_per_row(E);
-  const int64_t rows = (THREADS / 32) * (32 / g);
+  const int64_t rows = (GRAD_THREADS / 32) * (32 / g);
   const unsigned nb = (unsigned)std::min<int64_t>((T_ + rows - 1) / rows, 8 * 148);
   const bool vec = E % 8 == 0 && ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dlogits)) & 15) == 0;
   by_width<T>(g, vec, [&](auto gc, auto vc) {
-    grad_kernel<T, decltype(gc)::value, decltype(vc)::value><<<nb, THREADS, 0, st>>>(
+    grad_kernel<T, decltype(gc)::value, decltype(vc)::value><<<nb, GRAD_THREADS, 0, st>>>(
         reinterpret_cast<const T*>(logits), mask, coef, dloss, T_, E, reinterpret_cast<T*>(dlogits));
   });
 }
