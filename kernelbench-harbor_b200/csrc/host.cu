@@ -104,10 +104,26 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// Encodes; a thread that has made no runtime call yet has no current context,
+// which the driver's call needs: then the current device's is bound, and the
+// call made again.
+static CUresult encode(CUtensorMap* map, CUtensorMapDataType dt, cuuint32_t rank, const void* base, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swz) {
+  const cuuint32_t estr[3] = {1, 1, 1};
+  for (bool again = false;; again = true) {
+    const CUresult r = encode_fn()(map, dt, rank, const_cast<void*>(base), dims, strides, box, estr,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    int device;
+    if (r != CUDA_ERROR_INVALID_CONTEXT || again || cudaGetDevice(&device) != cudaSuccess ||
+        cudaSetDevice(device) != cudaSuccess)
+      return r;
+  }
+}
+
 int encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t outer,
               uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swz) {
-  auto fn = encode_fn();
-  if (!fn) return fail(B200Q_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  if (!encode_fn()) return fail(B200Q_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   if ((reinterpret_cast<uintptr_t>(base) & 15) != 0)
     return fail(B200Q_ERR_ALIGN, "tensor base address is not 16-byte aligned");
   if (row_stride_bytes % 16 != 0)
@@ -116,9 +132,7 @@ int encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64
   cuuint64_t dims[2] = {inner, outer};
   cuuint64_t strides[1] = {row_stride_bytes};
   cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode(map, dt, 2, base, dims, strides, box, swz);
   if (r != CUDA_SUCCESS)
     return fail(B200Q_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r));
   return B200Q_OK;
@@ -127,8 +141,7 @@ int encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64
 int encode_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
               uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0, uint32_t b1, uint32_t b2,
               CUtensorMapSwizzle swz) {
-  auto fn = encode_fn();
-  if (!fn) return fail(B200Q_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  if (!encode_fn()) return fail(B200Q_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   if ((reinterpret_cast<uintptr_t>(base) & 15) != 0)
     return fail(B200Q_ERR_ALIGN, "tensor base address is not 16-byte aligned");
   if (stride1_bytes % 16 != 0 || stride2_bytes % 16 != 0)
@@ -136,9 +149,7 @@ int encode_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64
   cuuint64_t dims[3] = {d0, d1, d2};
   cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
   cuuint32_t box[3] = {b0, b1, b2};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode(map, dt, 3, base, dims, strides, box, swz);
   if (r != CUDA_SUCCESS)
     return fail(B200Q_ERR_CUDA, "cuTensorMapEncodeTiled (3d) failed with CUresult " + std::to_string((int)r));
   return B200Q_OK;

@@ -158,3 +158,24 @@ def test_refusals():
     y = ops.w4a16_gemm(x, q, s.clone().requires_grad_(), z, 128)
     with pytest.raises(RuntimeError, match="frozen"):
         y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_from_a_thread_that_has_not_used_the_gpu():
+    """A thread's first call (autograd's own thread makes one, too) once every
+    attribute that a first call looks up is known."""
+    import threading
+
+    dy, q, s, z = grads_in(40, 256, 128, 64, "fp16", seed=3)
+    x = torch.randn(40, 256, dtype=torch.float16, device="cuda")
+    calls = [lambda: ops.w4a16_dgrad(dy, q, s, z, 64), lambda: ops.w4a16_dgrad(dy[:8], q, s, z, 64),
+             lambda: ops.w4a16_gemm(x, q, s, z, 64)]
+    for call in calls:
+        want = call()
+        torch.cuda.synchronize()
+        got = []
+        th = threading.Thread(target=lambda: got.append(call()))
+        th.start()
+        th.join()
+        torch.cuda.synchronize()
+        assert got and torch.equal(got[0], want)
