@@ -21,7 +21,7 @@ int w4a16_tc_dgrad(const void* dy, const int32_t* qweight, const void* scales, c
                    cudaStream_t stream);
 
 int w4a16_dgrad_small(const void* dy, const int32_t* qweight, const void* scales, const void* zeros, void* dx, int64_t M,
-                      int64_t N, int64_t K, int64_t group, int dtype, cudaStream_t stream);
+                      int64_t N, int64_t K, int64_t group, int dtype, void* workspace, cudaStream_t stream);
 
 size_t w8a8_ws_bytes(int64_t M, int64_t N, int64_t K, int device);
 int w8a8_tc(const void* x_int8, const void* w_int8, const void* x_scale, const void* w_scale, void* y, int64_t M,
@@ -80,7 +80,8 @@ int b200q_w4a16_dgrad(const void* dy, const int32_t* qweight, const void* scales
     return fail(B200Q_ERR_WORKSPACE, "w4a16 dgrad: workspace of 256 bytes required");
   // one 16-row operand: see w4a16_dgrad_small.cu
   if (M < W4A16_TC_MIN_M)
-    return w4a16_dgrad_small(dy, qweight, scales, zeros, dx, M, N, K, group, dtype, reinterpret_cast<cudaStream_t>(stream));
+    return w4a16_dgrad_small(dy, qweight, scales, zeros, dx, M, N, K, group, dtype, workspace,
+                             reinterpret_cast<cudaStream_t>(stream));
   return w4a16_tc_dgrad(dy, qweight, scales, zeros, dx, M, N, K, group, dtype, workspace, workspace_bytes,
                         reinterpret_cast<cudaStream_t>(stream));
 }

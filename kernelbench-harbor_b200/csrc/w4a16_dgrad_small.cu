@@ -24,21 +24,19 @@
 namespace b200q {
 namespace dx16 {
 
-using tc::as_u32;
-using tc::fma_f16x2;
-using tc::mul_bf16x2;
-using tc::mul_f16x2;
-using tc::sub_bf16x2;
-using tc::sub_f16x2;
-
-constexpr int TILE = 64, RB = TILE / 8;  // weight rows of a CTA; 8-row blocks
-constexpr int WARPS = 8, THREADS = WARPS * 32;
-constexpr int CHUNK = 128;  // columns of a warp's step
-constexpr int MAX_S = 8;
-constexpr int RPITCH = TILE + 4;
-constexpr int STAGES = 3, STAGE = TILE * CHUNK / 2;  // a warp's ring of packed weights: a lane's 16 bytes of 8 row blocks
-constexpr int RED = (WARPS + 1) * 16 * RPITCH * 4;
-constexpr int SMEM = WARPS * STAGES * STAGE > RED ? WARPS * STAGES * STAGE : RED;
+constexpr int TILE = 128, ROWS = 64, RB = ROWS / 8;  // weight rows of a CTA, of a warp; a warp's 8-row blocks
+constexpr int WC = 8, WARPS = WC * TILE / ROWS, THREADS = WARPS * 32;  // warps across the columns; all
+constexpr int CHUNK = 128;  // columns of a step of the two warps that share them
+constexpr int MAX_S = 8, STAGES = 2;
+// A stage: dy as two boxes of 64 columns (128-byte swizzle), the packed words, the groups' scales and zero points
+constexpr int DY_BYTES = 16 * CHUNK * 2, W_BYTES = TILE * CHUNK / 2, SZ_BYTES = CHUNK * 2;
+constexpr int OFF_W = DY_BYTES, OFF_S = OFF_W + W_BYTES;
+constexpr int RPITCH = TILE + 4, RED = (WC + 1) * 16 * RPITCH * 4;
+template <int GROUPS>
+constexpr int STAGE_BYTES = (OFF_S + 2 * GROUPS * SZ_BYTES + 1023) / 1024 * 1024;
+template <int GROUPS>
+constexpr int SMEM = 1024 + WC * STAGES * STAGE_BYTES<GROUPS> + 256;
+static_assert(SMEM<4> <= 227 * 1024 && RED <= WC * STAGES * STAGE_BYTES<1>, "shared memory budget");
 
 // 8 consecutive values -> the pairs (0,4) (1,5) (2,6) (3,7)
 __device__ __forceinline__ void pairs(const uint4 v, uint32_t* p) {
@@ -48,252 +46,195 @@ __device__ __forceinline__ void pairs(const uint4 v, uint32_t* p) {
   p[3] = prmt(v.y, v.w, 0x7632);
 }
 
-// larger magnitude of each half (its sign bit means nothing)
-__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-
-// Exponent e of the largest magnitude among the 4 lanes' 32 fp16 values each
-// (0 where all are 0, the type's largest where one is infinite) and 2^-e twice.
-__device__ __forceinline__ uint32_t scale_of(const uint32_t (*v)[4], int& e) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) m = max_f16x2(m, v[i][j]);
-  m = max_f16x2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max_f16x2(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  m &= 0x7FFF7FFFu;
-  const uint32_t top = max(m & 0xffffu, m >> 16) >> 10;  // biased exponent; 0: zero or subnormal, 31: infinite
-  // 2^-e has to be a normal fp16: e in -15 .. 14 (2^15 <= v: one step short of [1, 2), still far from the range's end)
-  e = top == 0 ? -14 : min((int)top, 29) - 15;
-  if (m == 0) e = 0;
-  const uint32_t inv = (uint32_t)(15 - e) << 10;
-  return inv | (inv << 16);
-}
-
-// A load that stays where it is written (the compiler would gather all of them at the top and spill)
-__device__ __forceinline__ uint4 ldg_ordered(const uint32_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
+__device__ __forceinline__ uint4 lds(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
 template <bool BF16>
-__device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float* d, const uint32_t (*a)[4], int j, uint32_t b0, uint32_t b1) {
   if (BF16)
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "r"(a[0][j]), "r"(a[1][j]), "r"(a[0][j + 1]), "r"(a[1][j + 1]), "r"(b0), "r"(b1));
   else
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "r"(a[0][j]), "r"(a[1][j]), "r"(a[0][j + 1]), "r"(a[1][j + 1]), "r"(b0), "r"(b1));
 }
 
-// GT: weight rows of the tile that share a group (the group size, at most TILE).
-template <bool BF16, int GT>
-__global__ void __launch_bounds__(THREADS, 2)
-    dgrad_small_kernel(const uint16_t* __restrict__ dy, const uint32_t* __restrict__ qw,
-                       const uint16_t* __restrict__ scales, const uint16_t* __restrict__ zeros,
-                       uint16_t* __restrict__ dx, int M, int N, int K, int group, int S) {
-  extern __shared__ __align__(16) uint8_t sm[];
-  const int k0 = (int)(blockIdx.x / S) * TILE, rank = S > 1 ? (int)cluster_ctarank() : 0;
+template <bool BF16>
+__device__ __forceinline__ uint16_t rounded(float v) {
+  if (BF16) {
+    const __nv_bfloat16 b = __float2bfloat16_rn(v);
+    return *reinterpret_cast<const uint16_t*>(&b);
+  }
+  const __half h = __float2half_rn(v);
+  return *reinterpret_cast<const uint16_t*>(&h);
+}
+
+// GROUPS: weight groups of a tile (1: the group size is 128 or 256).
+template <bool BF16, int GROUPS>
+__global__ void __launch_bounds__(THREADS, 1)
+    dgrad_small_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_w,
+                       const __grid_constant__ CUtensorMap tm_s, const __grid_constant__ CUtensorMap tm_z,
+                       uint16_t* __restrict__ dx, int M, int N, int K, int group, int S, int* status) {
+  extern __shared__ uint8_t sm_raw[];
+  uint8_t* const sm = align_smem_1024(sm_raw);
+  constexpr int STAGE = STAGE_BYTES<GROUPS>, SUBS = GROUPS == 4 ? 2 : 1;  // groups of a warp's rows
+  uint64_t* const full = reinterpret_cast<uint64_t*>(sm + WC * STAGES * STAGE);  // [wc][stage]
+  const int tile = (int)blockIdx.x / S, rank = S > 1 ? (int)cluster_ctarank() : 0;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int words = N / 8;
-  float tot[RB][4] = {};
-  uint8_t* ring = sm + warp * STAGES * STAGE + lane * 16;
-  auto request = [&](int n0, int slot) {  // the packed words that this lane multiplies in the step at n0
-    const int n = n0 + 32 * t;
+  const int wc = warp % WC, half = warp / WC;  // columns and rows of the tile
+  uint8_t* const ring = sm + wc * STAGES * STAGE;
+  uint64_t* const bar = full + wc * STAGES;
+  const bool asks = half == 0 && lane == 0;
+  auto request = [&](int n, int slot) {  // one thread; beyond the tensors' ends the copies write zeros
+    uint8_t* const st = ring + slot * STAGE;
+    mbar_arrive_expect_tx(bar + slot, DY_BYTES + W_BYTES + 2 * GROUPS * SZ_BYTES);
+    tma_load_2d(st + OFF_W, &tm_w, n / 8, tile * TILE, bar + slot);
+    tma_load_2d(st, &tm_dy, n, 0, bar + slot);
+    tma_load_2d(st + DY_BYTES / 2, &tm_dy, n + CHUNK / 2, 0, bar + slot);
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const bool here = n < N && k0 + 8 * b < K;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(ring + slot * STAGE + b * 512)),
-                   "l"(here ? qw + (size_t)(k0 + 8 * b + g) * words + n / 8 : qw), "r"(here ? 16 : 0)
-                   : "memory");
+    for (int i = 0; i < GROUPS; ++i) {
+      const int row = (tile * TILE + i * (TILE / GROUPS)) / group;
+      tma_load_2d(st + OFF_S + i * SZ_BYTES, &tm_s, n, row, bar + slot);
+      tma_load_2d(st + OFF_S + (GROUPS + i) * SZ_BYTES, &tm_z, n, row, bar + slot);
     }
   };
-  const int nstep = S * WARPS * CHUNK, nfirst = (rank * WARPS + warp) * CHUNK;
+  // Steps of this warp pair: every (S WC)-th chunk, from a start that differs from tile to tile, so that the tiles do not
+  // all ask for the same lines of dy at once
+  const int chunks = (N + CHUNK - 1) / CHUNK, stride = S * WC, first = (rank * WC + wc + 5 * tile) % stride;
+  const int steps = first < chunks ? (chunks - first + stride - 1) / stride : 0;
+  const int turn = steps ? tile % steps : 0;
+  auto column = [&](int step) { return (first + (step + turn) % steps * stride) * CHUNK; };
+  if (asks) {
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) {
-    request(nfirst + i * nstep, i);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int i = 0; i < STAGES; ++i) mbar_init(bar + i, 1);
+    fence_barrier_init();
+    for (int i = 0; i < STAGES && i < steps; ++i) request(column(i), i);
   }
-  int slot = 0;
-  for (int n0 = nfirst; n0 < N; n0 += nstep) {
-    request(n0 + (STAGES - 1) * nstep, slot == 0 ? STAGES - 1 : slot - 1);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    const int n = n0 + 32 * t;  // this lane's 32 columns: all inside the row or none (N % 32 == 0)
-    const bool in = n < N;
+  __syncthreads();  // the barriers are there
+  float tot[RB][4] = {};
+  bool ok = true;
+  for (int step = 0; step < steps; ++step) {
+    const int slot = step % STAGES;
+    const uint8_t* const st = ring + slot * STAGE;
+    ok = ok && mbar_wait(bar + slot, (step / STAGES) & 1, status);
 #pragma unroll
-    for (int sub = 0; sub < TILE / GT; ++sub) {
-      const int ks = k0 + sub * GT;
-      if (ks >= K) break;  // K is a multiple of the group
-      const uint16_t* srow = scales + (size_t)(ks / group) * N + n;
-      const uint16_t* zrow = zeros + (size_t)(ks / group) * N + n;
-      // pairs of columns (0,4) (1,5) (2,6) (3,7) of each word, as the unpacked nibbles come: the zero points as the
-      // subtraction wants them, and dy . s of rows g, g + 8
-      uint32_t zp[4][4], sp[4][4], a[2][4][4];
+    for (int sub = 0; sub < SUBS; ++sub) {
+      constexpr int NB = RB / SUBS;
+      uint4 wb[NB];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 zv = in ? ldg_ordered(reinterpret_cast<const uint32_t*>(zrow) + 4 * i) : make_uint4(0, 0, 0, 0);
-        pairs(zv, zp[i]);
-        if (!BF16) {  // 1024 + z, and -(64 + z) for the nibbles that stay 16 times too large
-          zp[i][0] = fma_f16x2(zp[i][0], 0x3C003C00u, 0x64006400u);
-          zp[i][1] = fma_f16x2(zp[i][1], 0xBC00BC00u, 0xD400D400u);
-          zp[i][2] = fma_f16x2(zp[i][2], 0x3C003C00u, 0x64006400u);
-          zp[i][3] = fma_f16x2(zp[i][3], 0xBC00BC00u, 0xD400D400u);
-        } else {  // 128 + z
+      for (int b = 0; b < NB; ++b) wb[b] = lds(st + OFF_W + (half * ROWS + (sub * NB + b) * 8 + g) * (CHUNK / 2) + t * 16);
+      const uint8_t* const srow = st + OFF_S + (GROUPS == 1 ? 0 : half * SUBS + sub) * SZ_BYTES;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) zp[i][j] = as_u32(__hadd2(tc::as_b2(zp[i][j]), __float2bfloat162_rn(128.f)));
+      for (int i = 0; i < 4; ++i) {  // 8 of the lane's 32 columns: its part of two k16 steps
+        const tc::ColQ q = tc::load_colq<BF16>(srow, srow + GROUPS * SZ_BYTES, 4 * t + i);
+        uint32_t a[2][4];  // dy of rows g, g + 8
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          pairs(lds(st + (t >> 1) * (DY_BYTES / 2) + (g + 8 * h) * 128 + (((t & 1) * 4 + i) ^ g) * 16), a[h]);
+#pragma unroll
+        for (int b = 0; b < NB; b += 2) {  // two row blocks in turn: their products do not wait for one another
+          const uint4 v0 = tc::dequant_word<BF16>(reinterpret_cast<const uint32_t*>(&wb[b])[i], q);
+          const uint4 v1 = tc::dequant_word<BF16>(reinterpret_cast<const uint32_t*>(&wb[b + 1])[i], q);
+          float *c0 = tot[sub * NB + b], *c1 = tot[sub * NB + b + 1];
+          mma<BF16>(c0, a, 0, v0.x, v0.y);
+          mma<BF16>(c1, a, 0, v1.x, v1.y);
+          mma<BF16>(c0, a, 2, v0.z, v0.w);
+          mma<BF16>(c1, a, 2, v1.z, v1.w);
         }
-        pairs(in ? ldg_ordered(reinterpret_cast<const uint32_t*>(srow) + 4 * i) : make_uint4(0, 0, 0, 0), sp[i]);
-      }
-      float fac[2] = {1.f, 1.f};
-      uint32_t sinv = 0;
-      int es = 0;
-      if (!BF16) {
-        sinv = scale_of(sp, es);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sp[i][j] = mul_f16x2(sp[i][j], sinv);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          pairs(in && g + 8 * h < M ? ldg_ordered(reinterpret_cast<const uint32_t*>(dy + (size_t)(g + 8 * h) * N + n) + 4 * i)
-                                    : make_uint4(0, 0, 0, 0),
-                a[h][i]);
-        if (!BF16) {  // row and scales brought to [1, 2) at their largest, exactly; their product is the one rounding
-          int ed;
-          const uint32_t dinv = scale_of(a[h], ed);
-          fac[h] = __uint_as_float((uint32_t)(127 + es + ed) << 23);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) a[h][i][j] = mul_f16x2(mul_f16x2(a[h][i][j], dinv), sp[i][j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) a[h][i][j] = mul_bf16x2(a[h][i][j], sp[i][j]);
-        }
-      }
-      if (sub == 0) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");  // this lane's own copies
-#pragma unroll
-      for (int b = 0; b < GT / 8; ++b) {
-        float c[4] = {};
-        const uint4 wb = *reinterpret_cast<const uint4*>(ring + slot * STAGE + (sub * (GT / 8) + b) * 512);
-        const uint32_t ww[4] = {wb.x, wb.y, wb.z, wb.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t v[4];
-          if (!BF16) {
-            const uint32_t r16 = 0x2C002C00u, w8 = ww[i] >> 8;  // 1/16
-            v[0] = sub_f16x2(and_or(ww[i], 0x000F000Fu, 0x64006400u), zp[i][0]);
-            v[1] = fma_f16x2(and_or(ww[i], 0x00F000F0u, 0x64006400u), r16, zp[i][1]);
-            v[2] = sub_f16x2(and_or(w8, 0x000F000Fu, 0x64006400u), zp[i][2]);
-            v[3] = fma_f16x2(and_or(w8, 0x00F000F0u, 0x64006400u), r16, zp[i][3]);
-          } else {
-            v[0] = sub_bf16x2(and_or(ww[i], 0x000F000Fu, 0x43004300u), zp[i][0]);
-            v[1] = sub_bf16x2(and_or(ww[i] >> 4, 0x000F000Fu, 0x43004300u), zp[i][1]);
-            v[2] = sub_bf16x2(and_or(ww[i] >> 8, 0x000F000Fu, 0x43004300u), zp[i][2]);
-            v[3] = sub_bf16x2(and_or(ww[i] >> 12, 0x000F000Fu, 0x43004300u), zp[i][3]);
-          }
-          mma<BF16>(c, a[0][i][0], a[1][i][0], a[0][i][1], a[1][i][1], v[0], v[1]);
-          mma<BF16>(c, a[0][i][2], a[1][i][2], a[0][i][3], a[1][i][3], v[2], v[3]);
-        }
-        float* o = tot[sub * (GT / 8) + b];
-        o[0] = fmaf(c[0], fac[0], o[0]);
-        o[1] = fmaf(c[1], fac[0], o[1]);
-        o[2] = fmaf(c[2], fac[1], o[2]);
-        o[3] = fmaf(c[3], fac[1], o[3]);
       }
     }
-    slot = slot + 1 == STAGES ? 0 : slot + 1;
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + wc) : "memory");  // both warps have read the stage
+    if (asks && ok && step + STAGES < steps) request(column(step + STAGES), slot);
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (asks && !ok)  // given up: what was asked for may still arrive
+    for (int i = 0; i < STAGES && i < steps; ++i) {
+      const int last = steps - 1 - (steps - 1 - i) % STAGES;
+      mbar_wait(bar + i, (last / STAGES) & 1, nullptr);
+    }
   __syncthreads();
-  float* red = reinterpret_cast<float*>(sm);  // [warp][16][RPITCH], then this CTA's sums
-  // the warps' sums, then the cluster's
+  // the warps' sums, then the cluster's, in order
+  float* red = reinterpret_cast<float*>(sm);  // [wc][16][RPITCH], then this CTA's sums
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    *reinterpret_cast<float2*>(red + (warp * 16 + g) * RPITCH + 8 * b + 2 * t) = make_float2(tot[b][0], tot[b][1]);
-    *reinterpret_cast<float2*>(red + (warp * 16 + g + 8) * RPITCH + 8 * b + 2 * t) = make_float2(tot[b][2], tot[b][3]);
+    float* r = red + (wc * 16 + g) * RPITCH + half * ROWS + 8 * b + 2 * t;
+    *reinterpret_cast<float2*>(r) = make_float2(tot[b][0], tot[b][1]);
+    *reinterpret_cast<float2*>(r + 8 * RPITCH) = make_float2(tot[b][2], tot[b][3]);
   }
   __syncthreads();
-  float* part = red + WARPS * 16 * RPITCH;
-  for (int i = tid; i < 16 * TILE; i += THREADS) {
-    const int m = i / TILE, c = i % TILE;
-    float v = 0.f;
+  float* const part = red + WC * 16 * RPITCH;
 #pragma unroll
-    for (int q = 0; q < WARPS; ++q) v += red[(q * 16 + m) * RPITCH + c];
-    part[m * RPITCH + c] = v;
-  }
-  if (S > 1)
-    cluster_sync();
-  else
-    __syncthreads();
-  // this rank's columns of the tile
-  const int q0 = rank * TILE / S, q1 = (rank + 1) * TILE / S, nq = q1 - q0;
-  for (int i = tid; i < M * nq; i += THREADS) {
-    const int m = i / nq, c = q0 + i % nq;
-    if (k0 + c >= K) continue;
-    float v = 0.f;
-    if (S > 1) {
-      const uint32_t addr = smem_u32(part + m * RPITCH + c);
-      for (int q = 0; q < S; ++q) {
-        float u;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u) : "r"(map_shared_rank(addr, q)) : "memory");
-        v += u;
-      }
-    } else {
-      v = part[m * RPITCH + c];
+  for (int i = tid; i < 16 * TILE / 2; i += THREADS) {
+    const int m = i / (TILE / 2), c = i % (TILE / 2) * 2;
+    float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int q = 0; q < WC; ++q) {
+      const float2 u = *reinterpret_cast<const float2*>(red + (q * 16 + m) * RPITCH + c);
+      v.x += u.x, v.y += u.y;
     }
-    uint16_t r;
-    if (BF16) {
-      const __nv_bfloat16 b = __float2bfloat16_rn(v);
-      r = *reinterpret_cast<const uint16_t*>(&b);
-    } else {
-      const __half h = __float2half_rn(v);
-      r = *reinterpret_cast<const uint16_t*>(&h);
-    }
-    dx[(size_t)m * K + k0 + c] = r;
+    if (S > 1)
+      *reinterpret_cast<float2*>(part + m * RPITCH + c) = v;
+    else if (m < M && tile * TILE + c < K)  // K is even
+      *reinterpret_cast<uint32_t*>(dx + (size_t)m * K + tile * TILE + c) =
+          (uint32_t)rounded<BF16>(v.x) | (uint32_t)rounded<BF16>(v.y) << 16;
   }
-  if (S > 1) cluster_sync();  // the others have read this CTA's sums
+  if (S == 1) return;
+  cluster_sync();
+  const int nq = TILE / S, q0 = rank * nq;  // this rank's columns of the tile
+  for (int i = tid; i < 16 * nq / 2; i += THREADS) {
+    const int m = i / (nq / 2), c = q0 + i % (nq / 2) * 2;
+    if (m >= M || tile * TILE + c >= K) continue;
+    float2 v = make_float2(0.f, 0.f);
+    const uint32_t addr = smem_u32(part + m * RPITCH + c);
+    for (int q = 0; q < S; ++q) {
+      float2 u;
+      asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(u.x), "=f"(u.y) : "r"(map_shared_rank(addr, q)) : "memory");
+      v.x += u.x, v.y += u.y;
+    }
+    *reinterpret_cast<uint32_t*>(dx + (size_t)m * K + tile * TILE + c) =
+        (uint32_t)rounded<BF16>(v.x) | (uint32_t)rounded<BF16>(v.y) << 16;
+  }
+  cluster_sync();  // the others have read this CTA's sums
 }
 
 }  // namespace dx16
 
 int w4a16_dgrad_small(const void* dy, const int32_t* qweight, const void* scales, const void* zeros, void* dx, int64_t M,
-                      int64_t N, int64_t K, int64_t group, int dtype, cudaStream_t stream) {
+                      int64_t N, int64_t K, int64_t group, int dtype, void* workspace, cudaStream_t stream) {
   using namespace dx16;
-  const uintptr_t any = reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(qweight) |
-                        reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(zeros);
-  if (any & 15) return fail(B200Q_ERR_ALIGN, "w4a16 dgrad: pointers must be 16-byte aligned");
   const bool bf = dtype == B200Q_DTYPE_BF16;
-  auto kern = group == 32 ? (bf ? dgrad_small_kernel<true, 32> : dgrad_small_kernel<false, 32>)
-                          : (bf ? dgrad_small_kernel<true, 64> : dgrad_small_kernel<false, 64>);
-  int rc = allow_smem((const void*)kern, SMEM, "cudaFuncSetAttribute(w4a16 dgrad small)");
+  const int groups = group == 32 ? 4 : group == 64 ? 2 : 1;
+  auto kern = groups == 4   ? (bf ? dgrad_small_kernel<true, 4> : dgrad_small_kernel<false, 4>)
+              : groups == 2 ? (bf ? dgrad_small_kernel<true, 2> : dgrad_small_kernel<false, 2>)
+                            : (bf ? dgrad_small_kernel<true, 1> : dgrad_small_kernel<false, 1>);
+  const int smem = groups == 4 ? SMEM<4> : groups == 2 ? SMEM<2> : SMEM<1>;
+  int rc = allow_smem((const void*)kern, smem, "cudaFuncSetAttribute(w4a16 dgrad small)");
+  if (rc) return rc;
+  const CUtensorMapDataType dt = bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap tm_dy, tm_w, tm_s, tm_z;
+  rc = encode_2d(&tm_dy, dt, dy, (uint64_t)N, (uint64_t)M, (uint64_t)N * 2, CHUNK / 2, 16, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc)
+    rc = encode_2d(&tm_w, CU_TENSOR_MAP_DATA_TYPE_INT32, qweight, (uint64_t)N / 8, (uint64_t)K, (uint64_t)N / 2, CHUNK / 8,
+                   TILE, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (!rc)
+    rc = encode_2d(&tm_s, dt, scales, (uint64_t)N, (uint64_t)(K / group), (uint64_t)N * 2, CHUNK, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (!rc)
+    rc = encode_2d(&tm_z, dt, zeros, (uint64_t)N, (uint64_t)(K / group), (uint64_t)N * 2, CHUNK, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (rc) return rc;
   // the split of the columns with the shortest estimate: rounds of co-resident
-  // clusters x (a warp's steps + 2 for start and joining)
+  // clusters x (a pair's steps + 2 for start and joining)
   const int64_t tiles = (K + TILE - 1) / TILE, chunks = (N + CHUNK - 1) / CHUNK;
   int S = 1;
   int64_t best = INT64_MAX;
-  const int* fit = resident_clusters((const void*)kern, THREADS, SMEM);
-  for (int s = 1; s <= MAX_S && (s == 1 || s * WARPS < chunks + WARPS); s *= 2) {
-    const int64_t cost = ((tiles + fit[s] - 1) / fit[s]) * ((chunks + s * WARPS - 1) / (s * WARPS) + 2);
+  const int* fit = resident_clusters((const void*)kern, THREADS, smem);
+  for (int s = 1; s <= MAX_S && (s == 1 || s * WC < chunks + WC); s *= 2) {
+    const int64_t cost = ((tiles + fit[s] - 1) / fit[s]) * ((chunks + s * WC - 1) / (s * WC) + 2);
     if (cost < best) best = cost, S = s;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * S));
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -302,11 +243,8 @@ int w4a16_dgrad_small(const void* dy, const int32_t* qweight, const void* scales
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, reinterpret_cast<const uint16_t*>(dy),
-                                       reinterpret_cast<const uint32_t*>(qweight),
-                                       reinterpret_cast<const uint16_t*>(scales),
-                                       reinterpret_cast<const uint16_t*>(zeros), reinterpret_cast<uint16_t*>(dx), (int)M,
-                                       (int)N, (int)K, (int)group, S),
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, tm_dy, tm_w, tm_s, tm_z, reinterpret_cast<uint16_t*>(dx), (int)M, (int)N,
+                                       (int)K, (int)group, S, reinterpret_cast<int*>(workspace)),
                     "w4a16 dgrad small launch");
 }
 
