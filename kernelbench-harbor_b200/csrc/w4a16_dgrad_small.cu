@@ -1,22 +1,23 @@
 // Input gradient of the frozen W4A16 projection for few rows (M <= 16):
-//   dx[m, k] = sum_n (dy[m, n] s[k/g, n]) (nib(k, n) - z[k/g, n]).
+//   dx[m, k] = sum_n dy[m, n] ((nib(k, n) - z[k/g, n]) s[k/g, n]).
 //
 // With one 16-row operand the dequantising tensor-core tile (w4a16_tc.cu's
-// MODE_DX, 128 rows) spends its time forming weights for rows that are not
-// there.  Here the scale goes to the other side of the product: A = dy . s, 16
-// rows x 128 columns per warp, once per weight group, and B = nib - z, an exact
-// small integer, straight from a lane's 16 packed bytes into the fragment of
-// mma.sync m16n8k16.  Of the contraction any order serves that both operands
-// share: a lane's 32 columns of a weight row are its parts of 8 k16 steps, so
-// nothing passes through shared memory.  A = dy . s is rounded once to the
-// activation type (where the other path rounds nib - z times s); fp16 scales a
-// row by a power of two first, since s takes it towards the subnormals.
-// A CTA takes 64 weight rows; its 8 warps and the S CTAs of its cluster share
-// the columns, and their sums are added in a fixed order.
+// MODE_DX, 128 rows of dy) spends its time on rows that are not there.  Here
+// mma.sync m16n8k16 takes dy as the 16 rows, and the weight, dequantised as the
+// forward does, straight from a lane's packed words as the other fragment.  Of
+// the contraction any order serves that both operands share: a lane's 32 columns
+// of a weight row are its parts of 8 k16 steps, in the order in which a word
+// unpacks, so no dequantised value passes through shared memory.
+// A CTA takes 128 weight rows: 8 column parts x 2 halves of 64 rows, one warp
+// each; the two warps at the same columns share a two-stage TMA ring of dy, words,
+// scales and zero points.  The S CTAs of a cluster share the columns too; sums are
+// joined in a fixed order.
 // Bound: HBM (the packed weight once: 32 MB at N=4096, K=14336, 4.9 us at the
-// measured copy rate) but for the instructions: 9 integer and half-precision
-// operations per packed word, and forming A for each 64 weight rows, half as
-// many again.  Measured there: 21 us, against 29 us for the 128-row tile.
+// measured copy rate) but for the instructions: 15 per packed word, 8 of them on
+// the half-rate fp16 pipe.  Measured there: 15.0 us, 9 us of it in the products (by
+// clock stamps), 2 in start and 1.5 in joining.  Before: the same tile fed by
+// 16-byte copies of the lanes 23 us (they held up the load unit), 64-row tiles with
+// the scale on dy's side 21 us, the 128-row tensor-core tile 29 us.
 #include <algorithm>
 
 #include "w4a16_dq.cuh"
@@ -99,12 +100,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       tma_load_2d(st + OFF_S + (GROUPS + i) * SZ_BYTES, &tm_z, n, row, bar + slot);
     }
   };
-  // Steps of this warp pair: every (S WC)-th chunk, from a start that differs from tile to tile, so that the tiles do not
-  // all ask for the same lines of dy at once
-  const int chunks = (N + CHUNK - 1) / CHUNK, stride = S * WC, first = (rank * WC + wc + 5 * tile) % stride;
+  // Steps of this warp pair: every (S WC)-th chunk
+  const int chunks = (N + CHUNK - 1) / CHUNK, stride = S * WC, first = rank * WC + wc;
   const int steps = first < chunks ? (chunks - first + stride - 1) / stride : 0;
-  const int turn = steps ? tile % steps : 0;
-  auto column = [&](int step) { return (first + (step + turn) % steps * stride) * CHUNK; };
+  auto column = [&](int step) { return (first + step * stride) * CHUNK; };
   if (asks) {
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) mbar_init(bar + i, 1);
