@@ -63,7 +63,8 @@ struct Grouped {
   int E;
 };
 
-enum { MODE_PLAIN = 0, MODE_GROUPED = 1, MODE_GLU = 2, MODE_DX = 3 };
+// MODE_DXH: MODE_DX with 128 weight rows a tile
+enum { MODE_PLAIN = 0, MODE_GROUPED = 1, MODE_GLU = 2, MODE_DX = 3, MODE_DXH = 4 };
 
 template <bool BF16, int MB, int MODE>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -72,10 +73,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const __grid_constant__ OutSet out, int M, int N, int K, int group, int splits, uint8_t* __restrict__ ws,
                     const __grid_constant__ Grouped grp) {
   constexpr bool GLU = MODE == MODE_GLU;
-  constexpr bool DX = MODE == MODE_DX;  // N: weight rows (output columns), K: weight columns (contraction)
+  constexpr bool DX = MODE == MODE_DX || MODE == MODE_DXH;  // N: weight rows (output columns), K: weight columns (contraction)
   // accumulator column p of a group of 8 -> output column
   auto out_col = [](int p) { return DX ? p : slot_col(p); };
-  constexpr int OUTC = GLU ? BN / 2 : BN;  // output columns per tile
+  constexpr int BNT = MODE == MODE_DXH ? BN / 2 : BN;  // accumulator columns per tile
+  constexpr int OUTC = GLU ? BN / 2 : BNT;  // output columns per tile
+  // DX, 128 rows: two halves of the dequantising warps take stages in turn, so that one half's latency (loads, arithmetic,
+  // the proxy fence) runs beside the other's
+  constexpr int TURNS = DX && MB == 1 ? 2 : 1, NDQ_T = NDQ / TURNS, DX_ROWS = BNT / NDQ_T, WORDS_T = DX ? DX_ROWS / 4 : WORDS;
   using T = typename DT<BF16>::T;
   using C = Cfg<MB>;
   constexpr int SX = C::SX, SW = C::SW, S2 = C::S2;
@@ -120,7 +125,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int k_begin = (int)((long long)split * nk_total / splits);
   const int k_end = (int)((long long)(split + 1) * nk_total / splits);
   const int nk = k_end - k_begin;
-  const int srows = DX ? BN / group : (group >= BK ? 1 : BK / group);  // scale rows of a stage
+  const int srows = DX ? max(BNT / group, 1) : (group >= BK ? 1 : BK / group);  // scale rows of a stage
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < SX; ++s) {
@@ -129,10 +134,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int s = 0; s < SW; ++s) {
       mbar_init(&w_full[s], 1);
-      mbar_init(&w_empty[s], NDQ);
+      mbar_init(&w_empty[s], NDQ_T);
     }
     for (int j = 0; j < S2; ++j) {
-      mbar_init(&b_full[j], NDQ);
+      mbar_init(&b_full[j], NDQ_T);
       mbar_init(&b_empty[j], 1);
     }
     mbar_init(acc_full, 1);
@@ -155,7 +160,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == W_PROD) {
     // ---------------------------------------------------------------- weight producer
     if (lane == 0) {
-      const uint32_t stage_tx = WQ_BYTES + 2u * srows * (DX ? BK : BN) * 2u;
+      const uint32_t stage_tx = (DX ? BNT * BK / 2 : WQ_BYTES) + 2u * srows * (DX ? BK : BN) * 2u;
       for (int it = 0; it < nk; ++it) {
         const int s = it % SW;
         if (it >= SW && !mbar_wait(&w_empty[s], ((it / SW) - 1) & 1, status)) {
@@ -208,7 +213,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp == W_MMA) {
     // ---------------------------------------------------------------- MMA issuer
     if (lane == 0) {
-      const uint32_t idesc = idesc_f16(BM, BN, BF16 ? 1 : 0, /*a_mn=*/0, /*b_mn=*/DX ? 0 : 1);
+      const uint32_t idesc = idesc_f16(BM, BNT, BF16 ? 1 : 0, /*a_mn=*/0, /*b_mn=*/DX ? 0 : 1);
       for (int it = 0; it < nk; ++it) {
         const int s = it % SX, j = it % S2;
         if (!mbar_wait(&x_full[s], (it / SX) & 1, status) || !mbar_wait(&b_full[j], (it / S2) & 1, status)) {
@@ -243,20 +248,22 @@ __global__ void __launch_bounds__(THREADS, 1)
     static_assert(WPR == 2, "a thread's words i < WORDS/2 lie in K rows 0..31 of the stage, the rest in 32..63");
     // loop-invariant parts of every address; ring slots and phases advance
     // incrementally (no divisions in the loop)
-    // DX: warp dw has weight rows 16 dw .. 16 dw + 15 of the tile, four per
-    // word index i; lane = (row within the four, word column)
+    // DX: a warp has DX_ROWS weight rows of its stages, four per word index i;
+    // lane = (row within the four, word column)
+    const int dx_row0 = dw % NDQ_T * DX_ROWS, turn = dw / NDQ_T;
     const uint32_t* wq_t = reinterpret_cast<const uint32_t*>(smem + OFF_WQ) +
-                           (DX ? dw * 128 + lane
+                           (DX ? dx_row0 * 8 + lane
                             : GLU ? (lane >> 4) * (BK * 16) + (rr + 8 * (dw >> 3)) * 16 + (lane & 15)
                                 : (rr + 8 * (dw >> 3)) * 32 + lane);
     constexpr int WQ_ROW_STEP = DX ? 32 : GLU ? 8 * WPR * 16 : 8 * WPR * 32;  // words between a thread's words i, i+1
-    uint8_t* b_t = smem + OFF_B + (DX ? dw * 2048 : ((dw >> 3) * 4 + nb) * 1024 + rr * 128 + ((ch ^ rr) << 4));
+    uint8_t* b_t = smem + OFF_B + (DX ? dx_row0 * 128 : ((dw >> 3) * 4 + nb) * 1024 + rr * 128 + ((ch ^ rr) << 4));
     // DX: operand row (4 (i & 1) + nb) of an 8-row group, chunk ch, for even and odd i
     const int dx_even = nb * 128 + ((ch ^ nb) << 4), dx_odd = (nb + 4) * 128 + ((ch ^ (nb + 4)) << 4);
-    const int dx_srow = DX ? (dw * 16 / group) * (BK * 2) : 0;
-    int s = 0, j = 0;
+    const int dx_srow = DX ? (dx_row0 / group) * (BK * 2) : 0;
+    static_assert(TURNS <= S2 && TURNS <= SW, "a turn passes a ring's end at most once");
+    int s = turn, j = turn;
     uint32_t ph_w = 0, ph_b = 1;
-    for (int it = 0; it < nk; ++it) {
+    for (int it = turn; it < nk; it += TURNS) {
       if (!mbar_wait(&w_full[s], ph_w, status)) {
         s_err = 1;
         break;
@@ -274,15 +281,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       const ColQ q0 = load_colq<BF16>(srow0, zrow0, DX ? ch : lane);
       const ColQ q1 = !DX && srows > 1 ? load_colq<BF16>(srow0 + BN * 2, zrow0 + BN * 2, lane) : q0;
       const uint32_t* wq = wq_t + s * (WQ_BYTES / 4);
-      uint32_t wv[WORDS];
+      uint32_t wv[WORDS_T];
 #pragma unroll
-      for (int i = 0; i < WORDS; ++i) wv[i] = wq[i * WQ_ROW_STEP];
+      for (int i = 0; i < WORDS_T; ++i) wv[i] = wq[i * WQ_ROW_STEP];
       __syncwarp();
       if (lane == 0) mbar_arrive(&w_empty[s]);
       uint8_t* bt = b_t + j * B_BYTES;
 #pragma unroll
-      for (int i = 0; i < WORDS; ++i) {
-        const uint4 v = dequant_word<BF16>(wv[i], i >= WORDS / 2 ? q1 : q0);
+      for (int i = 0; i < WORDS_T; ++i) {
+        const uint4 v = dequant_word<BF16>(wv[i], !DX && i >= WORDS / 2 ? q1 : q0);
         if (DX)
           *reinterpret_cast<uint4*>(bt + (i >> 1) * 1024 + ((i & 1) ? dx_odd : dx_even)) =
               make_uint4(prmt(v.x, v.y, 0x5410), prmt(v.z, v.w, 0x5410), prmt(v.x, v.y, 0x7632), prmt(v.z, v.w, 0x7632));
@@ -292,12 +299,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&b_full[j]);
-      if (++s == SW) {
-        s = 0;
+      if ((s += TURNS) >= SW) {
+        s -= SW;
         ph_w ^= 1;
       }
-      if (++j == S2) {
-        j = 0;
+      if ((j += TURNS) >= S2) {
+        j -= S2;
         ph_b ^= 1;
       }
     }
@@ -405,12 +412,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_after();
       const int dw = warp - W_DQ0;
       const int qd = warp & 3, part = dw >> 2;
-      constexpr int COLS = BN / (NDQ / 4);
+      constexpr int COLS = BNT / (NDQ / 4);
       const uint32_t trow = qd * 32 + lane;
       uint32_t owner = trow * S / BM;
       while ((owner + 1) * BM / S <= trow) ++owner;
       const uint32_t lr = trow - owner * BM / S;
-      const uint32_t base = map_shared_rank(smem_u32(smem), owner) + ((rank * MAXR + lr) * BN) * 4;
+      const uint32_t base = map_shared_rank(smem_u32(smem), owner) + ((rank * MAXR + lr) * BNT) * 4;
 #pragma unroll 1
       for (int c0 = 0; c0 < COLS; c0 += 32) {
         const int cslot = part * COLS + c0;
@@ -442,11 +449,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (!s_clu_err) {
       const float* buf = reinterpret_cast<const float*>(smem);
       const int r0 = (int)(rank * BM / S), nr = (int)((rank + 1) * BM / S) - r0;
-      for (int e = threadIdx.x * 4; e < nr * BN; e += THREADS * 4) {
-        const int lr = e / BN, c = e % BN;
-        float4 acc4 = reinterpret_cast<const float4*>(buf + lr * BN + c)[0];
+      for (int e = threadIdx.x * 4; e < nr * BNT; e += THREADS * 4) {
+        const int lr = e / BNT, c = e % BNT;
+        float4 acc4 = reinterpret_cast<const float4*>(buf + lr * BNT + c)[0];
         for (uint32_t src = 1; src < S; ++src) {
-          const float4 p4 = reinterpret_cast<const float4*>(buf + (src * MAXR + lr) * BN + c)[0];
+          const float4 p4 = reinterpret_cast<const float4*>(buf + (src * MAXR + lr) * BNT + c)[0];
           acc4.x += p4.x;
           acc4.y += p4.y;
           acc4.z += p4.z;
@@ -482,7 +489,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 
 struct Plan {
-  int mb, tiles_m, tiles_n, splits;
+  int mb, tiles_m, tiles_n, splits, bn = BN;
   size_t ws_bytes;
 };
 
@@ -520,28 +527,34 @@ Plan plan(int64_t M, int64_t N, int64_t K, int sms) {
 }
 
 // The same choice for MODE_DX (N: weight rows, K: weight columns), from its own
-// measurements: a 128-row stage takes 0.5 us and a 256-row one 1.34 times that;
-// joining a split through distributed shared memory costs as much as 11 stages
-// (two passes: 24), start and end 15.  M=1000, N=1408, K=2048: 18 us unsplit
-// with 128-row tiles, 26 us as 256-row tiles split four ways; M=17, N=4096,
-// K=14336: 39 us unsplit, 29 us split in two.
+// measurements at 22 to 224 stages.  A stage of a 128 x 256 tile takes 0.49 us --
+// the shared memory's rate: 48 KB of operand reads, 32 KB of dequantised and 28
+// KB of copied writes and reads at 128 bytes a clock --, of a 256 x 256 tile 1.35
+// and of a 128 x 128 tile 0.8 times that; start and end, and the joining of a
+// split through distributed shared memory, are counted in such stages too.
+// M=1000, N=1408, K=2048: 13.5 us as 128 x 128 tiles, 16.5 as 128 x 256; M=2048,
+// N = K = 4096: 118 and 74 us, 52 as 256 x 256; M=17 there: 15.1 us as 128 x 128
+// tiles split four ways, 18.4 as 128 x 256 split six ways.
 Plan plan_dx(int64_t M, int64_t N, int64_t K, int sms) {
   Plan p;
-  p.tiles_n = (int)((N + BN - 1) / BN);
   const int nk = (int)((K + BK - 1) / BK);
+  const struct { int mb, bn; double stage, start, join; } kinds[3] = {
+      {1, BN, 1.0, 11, 12}, {2, BN, 1.35, 15, 22}, {1, BN / 2, 0.8, 9, 6}};
   double best = 0;
-  for (int mb = 1; mb <= 2; ++mb) {
-    const int64_t tm = (M + BM * mb - 1) / (BM * mb), tiles = tm * p.tiles_n;
+  p.mb = 0;
+  for (const auto& k : kinds) {
+    const int64_t tm = (M + BM * k.mb - 1) / (BM * k.mb), tn = (N + k.bn - 1) / k.bn, tiles = tm * tn;
     for (int sp = 1; sp <= MAX_SPLITS; ++sp) {
       if (sp > 1 && (tiles * sp > sms || nk < 4 * sp)) break;
       const int64_t waves = (tiles * sp + sms - 1) / sms;
-      const double cost = (double)waves * ((nk + sp - 1) / sp) * (mb == 2 ? 1.34 : 1.0) +
-                          (sp == 1 ? 0.0 : mb == 2 ? 24.0 : 11.0) + 15.0;
-      if ((mb == 1 && sp == 1) || cost < best) {
+      const double cost = (double)waves * ((nk + sp - 1) / sp) * k.stage + k.start + (sp == 1 ? 0.0 : k.join);
+      if (p.mb == 0 || cost < best) {
         best = cost;
-        p.mb = mb;
+        p.mb = k.mb;
+        p.bn = k.bn;
         p.splits = sp;
         p.tiles_m = (int)std::min<int64_t>(tm, 1 << 30);
+        p.tiles_n = (int)tn;
       }
     }
   }
@@ -638,11 +651,11 @@ int w4a16_tc_dgrad(const void* dy, const int32_t* qweight, const void* scales, c
   if (!workspace || workspace_bytes < p.ws_bytes)
     return fail(B200Q_ERR_WORKSPACE, "w4a16 dgrad: workspace of " + std::to_string(p.ws_bytes) + " bytes required");
   const CUtensorMapDataType h16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
-  const uint32_t srows = (uint32_t)(BN / group);
+  const uint32_t srows = (uint32_t)std::max<int64_t>(p.bn / group, 1);
   CUtensorMap tdy, twq, ts, tz;
   int rc;
   if ((rc = encode_2d(&tdy, h16, dy, N, M, (uint64_t)N * 2, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
-  if ((rc = encode_2d(&twq, CU_TENSOR_MAP_DATA_TYPE_INT32, qweight, N / 8, K, (uint64_t)N / 2, BK / 8, BN,
+  if ((rc = encode_2d(&twq, CU_TENSOR_MAP_DATA_TYPE_INT32, qweight, N / 8, K, (uint64_t)N / 2, BK / 8, (uint32_t)p.bn,
                       CU_TENSOR_MAP_SWIZZLE_NONE)))
     return rc;
   if ((rc = encode_2d(&ts, h16, scales, N, K / group, (uint64_t)N * 2, BK, srows, CU_TENSOR_MAP_SWIZZLE_NONE)))
@@ -650,8 +663,9 @@ int w4a16_tc_dgrad(const void* dy, const int32_t* qweight, const void* scales, c
   if ((rc = encode_2d(&tz, h16, zeros, N, K / group, (uint64_t)N * 2, BK, srows, CU_TENSOR_MAP_SWIZZLE_NONE)))
     return rc;
   const bool bf = dtype == B200Q_DTYPE_BF16;
-  auto kern = p.mb == 2 ? (bf ? w4a16_tc_kernel<true, 2, MODE_DX> : w4a16_tc_kernel<false, 2, MODE_DX>)
-                        : (bf ? w4a16_tc_kernel<true, 1, MODE_DX> : w4a16_tc_kernel<false, 1, MODE_DX>);
+  auto kern = p.mb == 2    ? (bf ? w4a16_tc_kernel<true, 2, MODE_DX> : w4a16_tc_kernel<false, 2, MODE_DX>)
+              : p.bn == BN ? (bf ? w4a16_tc_kernel<true, 1, MODE_DX> : w4a16_tc_kernel<false, 1, MODE_DX>)
+                           : (bf ? w4a16_tc_kernel<true, 1, MODE_DXH> : w4a16_tc_kernel<false, 1, MODE_DXH>);
   const uint32_t smem = p.mb == 2 ? Cfg<2>::SMEM : Cfg<1>::SMEM;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(w4a16 dgrad)");
