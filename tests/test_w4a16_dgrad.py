@@ -9,11 +9,10 @@ from tests.helpers import tdt, torch_dequant_fp32, w4a16_inputs
 
 def check(dx, dy, q, s, z, group):
     """Elementwise bounds from the two roundings.  Against the weight rounded to
-    the activation type (as the tensor-core kernel, M >= 17, and the reference
-    module hold it): the last rounding, u |dx|, and the fp32 accumulation, at
+    the activation type (as the kernels and the reference module hold it): the last rounding, u |dx|, and the fp32 accumulation, at
     most one 2^-23 step per 16-wide multiply-add of the N / 16 in the chain, of
     S = sum |dy| |w|.  Against the weight in full: u S more, from the rounding
-    of the weight or (M <= 16) of dy times the scale."""
+    of the weight."""
     u = torch.finfo(dy.dtype).eps / 2
     w = torch_dequant_fp32(q, s, z, group).double()
     K = w.shape[0]
@@ -24,7 +23,7 @@ def check(dx, dy, q, s, z, group):
     tiny = 2.0 ** -25 if dy.dtype == torch.float16 else 0.0
     assert dx.shape == (dy.shape[0], K) and dx.dtype == dy.dtype
     ref = d @ wr.t()
-    assert dy.shape[0] <= 16 or ((dx.double() - ref).abs() <= u * (ref.abs() + acc) + acc + tiny).all()
+    assert ((dx.double() - ref).abs() <= u * (ref.abs() + acc) + acc + tiny).all()
     full = d @ w.t()
     assert ((dx.double() - full).abs() <= u * (full.abs() + 2 * S) + acc + tiny).all()
 
@@ -40,7 +39,7 @@ def grads_in(M, K, N, group, dtype, seed=0):
 @pytest.mark.parametrize("M,K,N,group", [
     (1, 128, 32, 128), (2, 256, 1056, 256), (7, 96, 160, 32), (16, 192, 2048, 64), (5, 1408, 2080, 64), (1, 4096, 4096, 128), (3, 32, 64, 32), (16, 14336, 4096, 128), (17, 96, 96, 32),
     (129, 192, 224, 64), (130, 512, 1408, 256), (255, 2048, 1408, 64), (300, 320, 160, 64), (1000, 2048, 1408, 64),
-    (777, 288, 4096, 32)])
+    (777, 288, 4096, 32), (17, 2048, 1408, 256), (40, 1056, 8192, 32), (2048, 4096, 512, 128), (2000, 4096, 544, 256)])
 def test_against_float64(M, K, N, group, dtype):
     args = grads_in(M, K, N, group, dtype)
     check(ops.w4a16_dgrad(*args, group), *args, group)
@@ -51,9 +50,10 @@ def test_against_float64(M, K, N, group, dtype):
 def test_one_weight_at_a_time():
     """Unit rows of dy give the dequantised weight's columns bit for bit."""
     _, q, s, z = grads_in(1, 256, 96, 32, "fp16", seed=4)
-    dx = ops.w4a16_dgrad(torch.eye(96, dtype=torch.float16, device="cuda"), q, s, z, 32)
+    eye = torch.eye(96, dtype=torch.float16, device="cuda")
     w = torch_dequant_fp32(q, s, z, 32).half()  # (nib - z) s: one rounding
-    assert torch.equal(dx, w.t())
+    assert torch.equal(ops.w4a16_dgrad(eye, q, s, z, 32), w.t())
+    assert torch.equal(torch.cat([ops.w4a16_dgrad(e, q, s, z, 32) for e in eye.split(16)]), w.t())
 
 
 @pytest.mark.gpu
