@@ -71,7 +71,8 @@ _no_switch = _NoSwitch()
 
 def _device(device: torch.device):
     """Context in which ``device`` is the current one (kernels launch on the current device)."""
-    return _no_switch if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    # a CUDA tensor exists, so what torch.cuda.current_device() first looks up is there
+    return _no_switch if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -613,17 +614,19 @@ def lora_plan(lora_ids: torch.Tensor, n_adapters: int) -> LoraPlan:
 
 
 def _lora_run(x, base, A, B, scaling, plan, out, lo):
-    """One b200q_lora_apply call on contiguous, aligned tensors."""
+    """One b200q_lora_apply call on contiguous, aligned tensors; returns the
+    sizes as the library takes them and the device."""
     n_adapters, D, r = A.shape
     T = x.shape[0]
     dev = x.device
+    sizes = (T, D, B.shape[2], r, n_adapters, _dtype_code(x.dtype))
     with _device(dev):
         # the one-launch kernel has no wait that could run out
         status = None if T <= _LORA_SMALL else workspace(dev, 256).data_ptr()
         _lib.check(_lib.lib().b200q_lora_apply(x.data_ptr(), base.data_ptr(), A.data_ptr(), B.data_ptr(), _ptr(scaling),
-                                               plan.data_ptr(), T, D, B.shape[2], r, n_adapters,
-                                               _dtype_code(x.dtype), out.data_ptr(), _ptr(lo), status,
+                                               plan.data_ptr(), *sizes, out.data_ptr(), _ptr(lo), status,
                                                _stream_ptr(dev)))
+    return sizes, dev
 
 
 @functools.lru_cache(maxsize=256)
@@ -647,7 +650,7 @@ class _LoraApply(torch.autograd.Function):
     def forward(ctx, base, x, A, B, scaling, plan):
         base, x, A, B = _aligned(base), _aligned(x), _aligned(A), _aligned(B)
         y, lo = torch.empty_like(base), _lora_mid(plan, A.shape[2])
-        _lora_run(x, base, A, B, scaling, plan.data, y, lo)
+        ctx.sizes = _lora_run(x, base, A, B, scaling, plan.data, y, lo)
         ctx.save_for_backward(x, A, B, scaling)
         ctx.lo, ctx.plan = lo, plan.data  # seen by nobody else
         return y
@@ -661,14 +664,11 @@ def _lora_grads(ctx, x, A, B, scaling, d, dx, base, need_A, need_B):
     """dA and dB; and dx (if given) = base (None: 0) + the adapters' part."""
     dA = torch.empty_like(A) if need_A else None
     dB = torch.empty_like(B) if need_B else None
-    n_adapters, D, r = A.shape
-    T = x.shape[0]
-    sizes = (T, D, B.shape[2], r, n_adapters, _dtype_code(x.dtype))
-    dev = x.device
+    sizes, dev = ctx.sizes
     with _device(dev):
         nbytes = _lora_scratch(*sizes, dev.index)
         scratch = ctx.plan.new_empty(nbytes // 4)  # fp32 sums
-        status = None if T <= _LORA_SMALL else workspace(dev, 256).data_ptr()
+        status = None if sizes[0] <= _LORA_SMALL else workspace(dev, 256).data_ptr()
         _lib.check(_lib.lib().b200q_lora_backward(
             x.data_ptr(), d.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling), ctx.plan.data_ptr(),
             ctx.lo.data_ptr(), *sizes, scratch.data_ptr(), nbytes, _ptr(dx), _ptr(dA), _ptr(dB), status,
@@ -693,7 +693,7 @@ class _LoRAW4A16(torch.autograd.Function):
     def forward(ctx, x, A, B, qweight, scales, zeros, group, scaling, plan):
         x, A, B = _aligned(x), _aligned(A), _aligned(B)
         y, lo = w4a16_gemm(x, qweight, scales, zeros, group), _lora_mid(plan, A.shape[2])
-        _lora_run(x, y, A, B, scaling, plan.data, y, lo)
+        ctx.sizes = _lora_run(x, y, A, B, scaling, plan.data, y, lo)
         ctx.save_for_backward(x, A, B, scaling, qweight, scales, zeros)
         ctx.lo, ctx.plan, ctx.group = lo, plan.data, group
         return y
