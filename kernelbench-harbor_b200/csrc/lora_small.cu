@@ -7,8 +7,8 @@
 // the output columns.  The row between, mid, is written once for a backward
 // pass.  Bound: latency -- 0.3 to 4 MB of adapters and rows at decode, against
 // one launch, two dependent rounds of loads and one cluster barrier; the first
-// group's Q, and base, are requested before the shrink starts.  Measured: 5.2 us
-// for one token, 5.6 us for 64 tokens of 8 adapters, at 4096 x 4096, r = 16.
+// group's Q, and base, are requested before the shrink starts.  Measured: 4.9 us
+// for one token, 5.5 us for 64 tokens of 8 adapters, at 4096 x 4096, r = 16.
 #include <type_traits>
 
 #include "lora_seg.cuh"
