@@ -38,8 +38,9 @@
 // one packed word is one 16-byte chunk of a 128-byte operand row, put into
 // column order by four PRMTs (the nibble pairs lie along the contraction, where
 // dy's order is fixed, not along the output, where the epilogue could undo it).
-// A tile's 256 weight rows span 256 / g groups, so a stage carries that many
-// 64-wide scale and zero rows; a warp's 16 rows lie in one group.
+// A tile's 256 weight rows (128 with MODE_DXH) span 256 / g groups, so a stage
+// carries that many 64-wide scale and zero rows; a warp's 16 or 32 rows lie in
+// one group.
 // Bound: the tensor cores, as the forward; M=4096, N=4096, K=14336 g128 moves
 // 182 MB (28 us at the measured copy rate) against 481 GFLOP (292 us at the
 // measured bf16 rate) and takes 420 us, power-bound like the forward.
