@@ -29,19 +29,26 @@ constexpr int ROWB = SK * 2;               // bytes of a stage's wide row; 16-by
 constexpr int WIDE = ROWS_L * ROWB;        // bytes of a stage's wide rows
 constexpr int MAX_SPLIT = 8;
 
-// Stages of the ring and CTAs per SM: 4 and 2 at rank 64, else 3 and 3 -- as many
-// bytes in flight, and half as many warps again to hide each other's latencies.
-__host__ __device__ constexpr int stages_of(int rp) { return rp == 64 ? 4 : 3; }
-__host__ __device__ constexpr int ctas_of(int rp, bool vec) { return !vec || rp == 64 ? 2 : 3; }
+// Stages of the ring and CTAs per SM: 4 and 2, or 3 and 3 -- as many bytes in
+// flight, and half as many warps again to hide each other's latencies, but 85
+// registers a thread.  Up to rank 16 these are enough; at rank 64 they never are.
+// At rank 32 the shrink spills with them, and the expand, with a few words, gains
+// where an adapter has few tokens: 8192 tokens in 16s, 4096 x 4096, bf16 209 us
+// with three and 230 with two, in 512s 54.6 and 50.8 (with the shrink, r = 32).
+__host__ __device__ constexpr int stages_of(int ctas) { return ctas == 2 ? 4 : 3; }
+__host__ __device__ constexpr int shrink_ctas(int rp, bool vec) { return !vec || rp >= 32 ? 2 : 3; }
+__host__ __device__ constexpr int expand_ctas(int rp, bool vec, bool few) { return !vec || rp == 64 || (rp == 32 && !few) ? 2 : 3; }
+// tokens per adapter up to which the expand kernel takes three CTAs
+constexpr int FEW_TOKENS = 32;
 
 // Swizzle of a row's 16-byte pieces: 8 rows x 1 piece (a fragment's words) and
 // 2 rows x 4 pieces (a quarter warp's 16-byte loads) both meet all banks once.
 __device__ __forceinline__ int swz(int row) { return ((row & 1) << 2) | ((row >> 1) & 3); }
 
 // The 64 contraction rows of P / the rank rows of Q lie RP or 64 values wide.
-template <int RP, bool TR>
+template <int RP, bool TR, bool VEC>
 struct ShrinkCfg {
-  static constexpr int STG = stages_of(RP);
+  static constexpr int STG = stages_of(shrink_ctas(RP, VEC));
   static constexpr int PITCH = RP * 2 + 16;                    // !TR: bytes per contraction row
   static constexpr int THIN = TR ? RP * ROWB : SK * PITCH;     // TR: rank rows of 64 values
   static constexpr int STAGE = WIDE + THIN;
@@ -51,8 +58,8 @@ struct ShrinkCfg {
 };
 
 template <class T, int RP, bool TR, bool VEC>
-__global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_shrink_tile_kernel(const Args a, int S) {
-  using C = ShrinkCfg<RP, TR>;
+__global__ void __launch_bounds__(THREADS, shrink_ctas(RP, VEC)) lora_shrink_tile_kernel(const Args a, int S) {
+  using C = ShrinkCfg<RP, TR, VEC>;
   constexpr int STG = C::STG;
   extern __shared__ __align__(128) uint8_t sm[];
   const int tile = blockIdx.x / S, rank = S > 1 ? (int)cluster_ctarank() : 0;
@@ -265,9 +272,9 @@ __global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_shrink_tile_ke
   if (S > 1) cluster_sync();  // the others have read this CTA's part
 }
 
-template <int RP, bool TR>
+template <int RP, bool TR, int CTAS>
 struct ExpandCfg {
-  static constexpr int STG = stages_of(RP);
+  static constexpr int STG = stages_of(CTAS);
   // !TR: bytes per rank row of 64 columns; TR: per column row of RP ranks, 8 words mod 32 (no bank conflicts)
   static constexpr int PITCH = !TR ? ROWB + 16 : RP == 16 ? 32 : RP == 32 ? 96 : 160;
   static constexpr int THIN = (TR ? SK : RP) * PITCH;
@@ -276,9 +283,9 @@ struct ExpandCfg {
 };
 
 // CTA = (tile, part): `steps` 64-column steps from step part * steps on.
-template <class T, int RP, bool TR, bool VEC>
-__global__ void __launch_bounds__(THREADS, ctas_of(RP, VEC)) lora_expand_tile_kernel(const Args a, int parts, int steps) {
-  using C = ExpandCfg<RP, TR>;
+template <class T, int RP, bool TR, bool VEC, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) lora_expand_tile_kernel(const Args a, int parts, int steps) {
+  using C = ExpandCfg<RP, TR, CTAS>;
   constexpr int STG = C::STG;
   extern __shared__ __align__(128) uint8_t sm[];
   const int32_t* plan = a.plan;
@@ -540,8 +547,12 @@ int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
     using T = decltype(tc);
     constexpr int RP = decltype(rc)::value;
     constexpr bool VEC = decltype(vc)::value;
-    auto expand = tr ? lora_expand_tile_kernel<T, RP, true, VEC> : lora_expand_tile_kernel<T, RP, false, VEC>;
-    const int smem_e = tr ? ExpandCfg<RP, true>::SMEM : ExpandCfg<RP, false>::SMEM;
+    constexpr int FEW = expand_ctas(RP, VEC, true), MANY = expand_ctas(RP, VEC, false);
+    const bool few = a.T <= FEW_TOKENS * a.L;
+    auto expand = tr ? (few ? lora_expand_tile_kernel<T, RP, true, VEC, FEW> : lora_expand_tile_kernel<T, RP, true, VEC, MANY>)
+                     : (few ? lora_expand_tile_kernel<T, RP, false, VEC, FEW> : lora_expand_tile_kernel<T, RP, false, VEC, MANY>);
+    const int smem_e = tr ? (few ? ExpandCfg<RP, true, FEW>::SMEM : ExpandCfg<RP, true, MANY>::SMEM)
+                          : (few ? ExpandCfg<RP, false, FEW>::SMEM : ExpandCfg<RP, false, MANY>::SMEM);
     // expand: the number of 64-column steps per CTA with the shortest estimate (start: 2 steps)
     int status = allow_smem((const void*)expand, smem_e, "cudaFuncSetAttribute(lora expand)");
     if (status) return status;
@@ -568,7 +579,7 @@ int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
                             resident_clusters(kern, SHRINK_TC_THREADS, SHRINK_TC_SMEM), 2);
     } else {
       auto shrink = tr ? lora_shrink_tile_kernel<T, RP, true, VEC> : lora_shrink_tile_kernel<T, RP, false, VEC>;
-      const int smem_s = tr ? ShrinkCfg<RP, true>::SMEM : ShrinkCfg<RP, false>::SMEM;
+      const int smem_s = tr ? ShrinkCfg<RP, true, VEC>::SMEM : ShrinkCfg<RP, false, VEC>::SMEM;
       if ((status = allow_smem((const void*)shrink, smem_s, "cudaFuncSetAttribute(lora shrink)"))) return status;
       status = launch_split(shrink, THREADS, smem_s, a, st, resident_clusters((const void*)shrink, THREADS, smem_s), 1);
     }
