@@ -337,11 +337,23 @@ template <class T, bool VEC>
 __device__ __forceinline__ void copy_rows(const T* base, T* y, const int32_t* rows, int count, int N, int n0, int n1,
                                           const T* end) {
   if (base == y) return;
-  const int g8 = (n1 - n0 + 7) / 8;
-  for (int i = threadIdx.x; i < count * g8; i += THREADS) {
-    const size_t off = (size_t)rows[i / g8] * N;
-    const int n = n0 + i % g8 * 8;
-    st8<T, VEC>(y + off + n, n1 - n, base ? ld8<T, VEC>(base + off, n, N, end) : make_uint4(0, 0, 0, 0));
+  // four pieces at a time: their rows are looked up, then loaded, then stored together
+  const int g8 = (n1 - n0 + 7) / 8, total = count * g8;
+  for (int i0 = threadIdx.x; i0 < total; i0 += 4 * THREADS) {
+    size_t off[4];
+    int n[4];
+    uint4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = min(i0 + k * THREADS, total - 1);
+      off[k] = (size_t)rows[i / g8] * N;
+      n[k] = n0 + i % g8 * 8;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = base ? ld8<T, VEC>(base + off[k], n[k], N, end) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i0 + k * THREADS < total) st8<T, VEC>(y + off[k] + n[k], n1 - n[k], v[k]);
   }
 }
 
@@ -364,6 +376,11 @@ int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st);
 using ShrinkFn = void (*)(const Args, int);
 constexpr int SHRINK_TC_THREADS = THREADS + 32, SHRINK_TC_SMEM = 4 * (128 * 128 + 64 * 128) + 1024;
 const void* shrink_tc_kernel(int dtype, bool tr);
+
+// lora_expand_tc.cu: the same ranks
+using ExpandFn = void (*)(const Args, int, int);
+constexpr int EXPAND_TC_SMEM = 2 * 128 * 128 + 3 * (128 * 128 + 64 * 128) + 1024;
+const void* expand_tc_kernel(int dtype, bool tr);
 
 inline bool aligned_widths(int64_t D, int64_t N, int64_t r) { return D % 8 == 0 && N % 8 == 0 && r % 4 == 0; }
 

@@ -40,6 +40,13 @@ __host__ __device__ constexpr int shrink_ctas(int rp, bool vec) { return !vec ||
 __host__ __device__ constexpr int expand_ctas(int rp, bool vec, bool few) { return !vec || rp == 64 || (rp == 32 && !few) ? 2 : 3; }
 // tokens per adapter up to which the expand kernel takes three CTAs
 constexpr int FEW_TOKENS = 32;
+// Tokens per adapter, and values of y, from which rank 64 expands through tensor
+// memory (lora_expand_tc.cu): below, its tiles' start costs more than the
+// fragments that it saves.  4096 tokens, D=4096, N=14336, bf16, shrink and expand:
+// 82.2 us with fragments and 74.8 without in 128s, 113.5 and 124.8 in 64s; N=1408,
+// D=2048: 14.3 and 13.0 us at 1024 tokens, 11.8 and 13.0 at 512.
+constexpr int TC_TOKENS = 96;
+constexpr int64_t TC_VALUES = 1 << 20;
 
 // Swizzle of a row's 16-byte pieces: 8 rows x 1 piece (a fragment's words) and
 // 2 rows x 4 pieces (a quarter warp's 16-byte loads) both meet all banks once.
@@ -417,10 +424,10 @@ __global__ void __launch_bounds__(THREADS, CTAS) lora_expand_tile_kernel(const A
     if (nst > 1) request();
   }
   if constexpr (!TR) load_q(0);
-  pdl_wait_previous();  // mid comes from the kernel before; all else was there when that one began
   // mid: rows m, m + 8; values 4t .. 4t + 3 of each 16 ranks, split into hi + lo
   const int m = warp * 16 + g;
   const int64_t ra = m < count ? rows[m] : -1, rb = m + 8 < count ? rows[m + 8] : -1;
+  pdl_wait_previous();  // mid comes from the kernel before; all else was there when that one began
   float fac[2];
   uint2 ha[RP / 16][2], la[RP / 16][2];
 #pragma unroll
@@ -549,15 +556,22 @@ int launch_tiles(const Args& a, int dtype, bool tr, cudaStream_t st) {
     constexpr bool VEC = decltype(vc)::value;
     constexpr int FEW = expand_ctas(RP, VEC, true), MANY = expand_ctas(RP, VEC, false);
     const bool few = a.T <= FEW_TOKENS * a.L;
-    auto expand = tr ? (few ? lora_expand_tile_kernel<T, RP, true, VEC, FEW> : lora_expand_tile_kernel<T, RP, true, VEC, MANY>)
-                     : (few ? lora_expand_tile_kernel<T, RP, false, VEC, FEW> : lora_expand_tile_kernel<T, RP, false, VEC, MANY>);
-    const int smem_e = tr ? (few ? ExpandCfg<RP, true, FEW>::SMEM : ExpandCfg<RP, true, MANY>::SMEM)
-                          : (few ? ExpandCfg<RP, false, FEW>::SMEM : ExpandCfg<RP, false, MANY>::SMEM);
+    ExpandFn expand =
+        tr ? (few ? lora_expand_tile_kernel<T, RP, true, VEC, FEW> : lora_expand_tile_kernel<T, RP, true, VEC, MANY>)
+           : (few ? lora_expand_tile_kernel<T, RP, false, VEC, FEW> : lora_expand_tile_kernel<T, RP, false, VEC, MANY>);
+    int smem_e = tr ? (few ? ExpandCfg<RP, true, FEW>::SMEM : ExpandCfg<RP, true, MANY>::SMEM)
+                    : (few ? ExpandCfg<RP, false, FEW>::SMEM : ExpandCfg<RP, false, MANY>::SMEM);
+    int per_e = 1;
+    if (VEC && RP == 64 && a.T > TC_TOKENS * a.L && a.T * a.N >= TC_VALUES) {
+      expand = reinterpret_cast<ExpandFn>(const_cast<void*>(expand_tc_kernel(dtype, tr)));
+      smem_e = EXPAND_TC_SMEM;
+      per_e = 2;  // see the shrink below
+    }
     // expand: the number of 64-column steps per CTA with the shortest estimate (start: 2 steps)
     int status = allow_smem((const void*)expand, smem_e, "cudaFuncSetAttribute(lora expand)");
     if (status) return status;
     const int64_t whole = (a.T + ROWS_L - 1) / ROWS_L, tiles = whole + std::min(a.L, whole) / 2;
-    const int64_t nsteps = (a.N + SK - 1) / SK, slots = resident_clusters((const void*)expand, THREADS, smem_e)[1];
+    const int64_t nsteps = (a.N + SK - 1) / SK, slots = per_e * resident_clusters((const void*)expand, THREADS, smem_e)[1];
     int steps = 2;
     int64_t best = INT64_MAX;
     for (int s = 2; s <= 16; ++s) {

@@ -153,7 +153,8 @@ def test_ids_out_of_range_count_as_none():
     (64, 4096, 4096, 16, 8, "mixed"), (100, 257, 129, 33, 3, "mixed"), (129, 1000, 264, 64, 2, "runs"),
     (256, 2048, 512, 24, 5, "runs"), (257, 128, 128, 16, 3, "runs"), (300, 4100, 64, 12, 2, "mixed"),
     (300, 70, 333, 5, 4, "runs"), (700, 1408, 2048, 8, 60, "runs"), (1000, 512, 1152, 64, 1, "one"),
-    (1300, 72, 2056, 48, 3, "runs"), (2049, 3584, 256, 32, 5, "mixed"), (600, 264, 264, 16, 2, "none")])
+    (1300, 72, 2056, 48, 3, "runs"), (2049, 3584, 256, 32, 5, "mixed"), (600, 264, 264, 16, 2, "none"),
+    (1100, 1096, 1096, 36, 2, "mixed"), (4100, 264, 264, 60, 3, "runs"), (1024, 1024, 1032, 64, 1, "none")])
 def test_against_float64(T, D, N, r, L, kind, dtype):
     check(inputs(T, D, N, r, L, dtype, kind))
 
