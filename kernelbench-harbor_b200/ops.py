@@ -158,11 +158,15 @@ def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, z
     if group <= 0 or K % group:
         raise ValueError(f"K={K} is not a multiple of group={group}")
     for name, t in (("scales", scales), ("zeros", zeros)):
-        if tuple(t.shape) != (K // group, N):
+        if t.shape != (K // group, N):
             raise ValueError(f"{name} must be [{K // group}, {N}], got {tuple(t.shape)}")
     dt = _dtype_code(dy.dtype)
     _same_device("w4a16_dgrad", dy, qweight, scales, zeros)
-    dy, qweight, scales, zeros = (_aligned(t) for t in (dy, qweight, scales.to(dy.dtype), zeros.to(dy.dtype)))
+    if scales.dtype != dy.dtype:
+        scales = scales.to(dy.dtype)
+    if zeros.dtype != dy.dtype:
+        zeros = zeros.to(dy.dtype)
+    dy, qweight, scales, zeros = _aligned(dy), _aligned(qweight), _aligned(scales), _aligned(zeros)
     dx = dy.new_empty((M, K))
     if M == 0:
         return dx
@@ -424,8 +428,8 @@ def moe_balance_loss(router_logits: torch.Tensor, topi: torch.Tensor,
             raise ValueError("token_mask must be bool [T]")
         token_mask = token_mask.contiguous()
     if topi.dtype == torch.int64:  # what 32 bits do not hold stays out of range
-        topi = topi.clamp(-2, router_logits.shape[1])
-    topi = topi.to(torch.int32).contiguous()
+        topi = topi.clamp(-2, router_logits.shape[1]).to(torch.int32)
+    topi = topi.contiguous()
     if torch.is_grad_enabled() and router_logits.requires_grad:
         return _BalanceLoss.apply(router_logits, topi, token_mask)
     return _balance_forward(router_logits.contiguous(), topi, token_mask)[:2]
