@@ -304,11 +304,11 @@ def test_no_tokens():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [64, 1000])
-def test_the_same_bits_on_other_streams_and_in_graphs(T):
+@pytest.mark.parametrize("T,D,N,r", [(64, 512, 384, 16), (1000, 512, 384, 16), (1200, 1024, 1096, 64)])
+def test_the_same_bits_on_other_streams_and_in_graphs(T, D, N, r):
     """Forward and backward captured twice, replayed at the same time on two
     streams, on new inputs."""
-    c = inputs(T, 512, 384, 16, 4, "bf16", "runs")
+    c = inputs(T, D, N, r, 4, "bf16", "runs")
     leaves = [c[k].clone().requires_grad_() for k in ("x", "A", "B")]
     plan = ops.lora_plan(c["ids"], 4)
 
@@ -339,6 +339,19 @@ def test_the_same_bits_on_other_streams_and_in_graphs(T):
         torch.cuda.synchronize()
         for _, out, _ in graphs:
             assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N,r,L", [(40, 264, 16, 3), (700, 264, 32, 3), (700, 264, 32, 60), (1300, 1032, 60, 3), (1300, 1032, 60, 40)])
+def test_in_place_on_the_base(T, N, r, L):
+    """y over base, rows without an adapter left as they are; the same bits as beside it."""
+    c = inputs(T, 264, N, r, L, "fp16", "mixed")
+    plan = ops.lora_plan(c["ids"], L)
+    args = (c["x"], c["A"], c["B"], plan, c["scaling"])
+    want = ops.lora_apply(c["base"], *args)
+    y = c["base"].clone()
+    assert ops.lora_apply(y, *args, out=y) is y
+    assert torch.equal(y, want) and torch.equal(y[c["ids"] < 0], c["base"][c["ids"] < 0])
 
 
 # ---------------------------------------------------------------- the module
