@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(THREADS, 2) lora_expand_tc_kernel(const Args a
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       float fac, inv;
-      pow2_of(mx, fac, inv);
+      scale_of<T>(mx, fac, inv);
       if ((lane & 15) == 0) s_fac[m] = fac;
       T hi[4], lo[4];
       split(v[i].x * inv, hi[0], lo[0]);

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(THREADS, VEC ? GradCfg<RP>::CTAS : 2) lora_gra
       const unsigned m = s_max[st & 3];
       if (m > emax) {
         float nf, ni;
-        pow2_of(__uint_as_float(m << 23), nf, ni);
+        scale_of<T>(__uint_as_float(m << 23), nf, ni);
         scale = fac * ni;  // both powers of two
         fac = nf;
         inv = ni;

@@ -90,7 +90,8 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
 }
 
 // v = hi + lo to twice the type's significand: the products of mid with the
-// thin matrix keep fp32's accuracy to ~2^-16 (bf16) or 2^-22 (fp16) of a value.
+// thin matrix keep a value to 2^-16 (bf16) or 2^-22 (fp16) of itself, in fp16 at
+// least to 2^-39 of the largest value that is scaled together with it (scale_of).
 // An infinity or NaN stays in hi alone.
 template <class T>
 __device__ __forceinline__ void split(float v, T& hi, T& lo) {
@@ -99,18 +100,18 @@ __device__ __forceinline__ void split(float v, T& hi, T& lo) {
   lo = ft<T>(fabsf(rest) < INFINITY ? rest : 0.f);
 }
 
-// Power-of-two factor of a value's exponent and its inverse, so that v * inv
-// lies in [1, 2): fp16 has 5 exponent bits, and mid may leave their range.
-// 0, subnormals, infinities and NaN give 1.
-__device__ __forceinline__ void pow2_of(float v, float& fac, float& inv) {
-  const uint32_t e = (__float_as_uint(v) >> 23) & 0xffu;
-  fac = 1.f;
-  inv = 1.f;
-  if (e != 0 && e != 255) {
-    const uint32_t c = e > 253 ? 253 : e;
-    fac = __uint_as_float(c << 23);
-    inv = __uint_as_float((254 - c) << 23);
-  }
+// Power-of-two factor for values up to |v| (finite) and its inverse: fp16 has 5
+// exponent bits, and mid may leave their range.  fp16: |v * inv| lies in [2^14,
+// 2^15), the last binade but one, so that the smallest step of the halves, 2^-24,
+// is 2^-39 of the largest value; the sums of products (below 2^31 each) are
+// fp32.  bf16, with fp32's exponents: in [1, 2).  Less for the tiniest v, whose
+// factor would be subnormal.
+template <class T>
+__device__ __forceinline__ void scale_of(float v, float& fac, float& inv) {
+  constexpr uint32_t UP = std::is_same<T, __half>::value ? 14 : 0;
+  const uint32_t e = min(max((__float_as_uint(v) >> 23) & 0xffu, UP + 1), UP ? 254u : 253u) - UP;
+  fac = __uint_as_float(e << 23);
+  inv = __uint_as_float((254 - e) << 23);
 }
 
 template <class T>

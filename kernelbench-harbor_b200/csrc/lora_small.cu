@@ -230,7 +230,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(THREADS) lora_small
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float fac, inv;
-  pow2_of(mx, fac, inv);
+  scale_of<T>(mx, fac, inv);
   T* hi = reinterpret_cast<T*>(sm + C::OFF_HI);
   T* lo = reinterpret_cast<T*>(sm + C::OFF_LO);
   float* facs = reinterpret_cast<float*>(sm + C::OFF_FAC);

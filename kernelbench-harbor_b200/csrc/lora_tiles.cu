@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) lora_expand_tile_kernel(const A
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     float inv;
-    pow2_of(mx, fac[h], inv);
+    scale_of<T>(mx, fac[h], inv);
 #pragma unroll
     for (int k = 0; k < RP / 16; ++k) {
       T hi[4], lo[4];
