@@ -141,10 +141,26 @@ def _(x, qweight, scales, zeros, group):
     return x.new_empty((x.shape[0], qweight.shape[1] * 8))
 
 
+def _dispatched(t: torch.Tensor) -> bool:
+    """Whether a call on t has to go through PyTorch's dispatcher as a registered
+    operator: while a program is traced (torch.compile, export, fake tensors),
+    under a dispatch mode, or for a tensor subclass.  Other calls take the
+    library directly (a registered operator costs 10 us more on the host)."""
+    return (torch.compiler.is_compiling() or type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter
+            or torch._C._len_torch_dispatch_stack() > 0)
+
+
 def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
                 group: int) -> torch.Tensor:
     """dx[M, K] = dy[M, N] . ((unpack(qweight) - zeros) * scales)^T, dx in dy.dtype:
-    the input gradient of w4a16_gemm (the weights are frozen)."""
+    the input gradient of w4a16_gemm (the weights are frozen).  Differentiable
+    in dy, w4a16_gemm being its gradient in turn."""
+    if (torch.is_grad_enabled() and (dy.requires_grad or scales.requires_grad or zeros.requires_grad)) or _dispatched(dy):
+        return w4a16_dgrad_op(dy, qweight, scales, zeros, group)
+    return _w4a16_dgrad(dy, qweight, scales, zeros, group)
+
+
+def _w4a16_dgrad(dy, qweight, scales, zeros, group):
     if not dy.is_cuda:
         raise RuntimeError("b200q w4a16_dgrad runs on CUDA tensors only (no CPU implementation)")
     if dy.dim() != 2 or qweight.dim() != 2:
@@ -178,20 +194,45 @@ def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, z
     return dx
 
 
+@torch.library.custom_op("b200q::w4a16_dgrad", mutates_args=())
+def w4a16_dgrad_op(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
+                   group: int) -> torch.Tensor:
+    """w4a16_dgrad as a registered operator."""
+    return _w4a16_dgrad(dy, qweight, scales, zeros, group)
+
+
+@w4a16_dgrad_op.register_fake
+def _(dy, qweight, scales, zeros, group):
+    return dy.new_empty((dy.shape[0], qweight.shape[0]))
+
+
 def _w4a16_setup(ctx, inputs, output):
-    x, qweight, scales, zeros, group = inputs
+    _, qweight, scales, zeros, group = inputs
     ctx.save_for_backward(qweight, scales, zeros)
     ctx.group = group
 
 
-def _w4a16_backward(ctx, dy):
+def _frozen(ctx, op):
     if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
-        raise RuntimeError("w4a16_gemm: the quantised weight is frozen, scales and zeros have no gradient")
+        raise RuntimeError(f"{op}: the quantised weight is frozen, scales and zeros have no gradient")
+
+
+# The two are linear, and each other's gradient: gradients of any order.
+def _w4a16_backward(ctx, dy):
+    _frozen(ctx, "w4a16_gemm")
     qweight, scales, zeros = ctx.saved_tensors
     dx = w4a16_dgrad(dy, qweight, scales, zeros, ctx.group) if ctx.needs_input_grad[0] else None
     return dx, None, None, None, None
 
 
+def _w4a16_dgrad_backward(ctx, ddx):
+    _frozen(ctx, "w4a16_dgrad")
+    qweight, scales, zeros = ctx.saved_tensors
+    ddy = w4a16_gemm(ddx, qweight, scales, zeros, ctx.group) if ctx.needs_input_grad[0] else None
+    return ddy, None, None, None, None
+
+
+w4a16_dgrad_op.register_autograd(_w4a16_dgrad_backward, setup_context=_w4a16_setup)
 w4a16_gemm.register_autograd(_w4a16_backward, setup_context=_w4a16_setup)
 
 
