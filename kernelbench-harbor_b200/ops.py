@@ -79,15 +79,6 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _once(backward, ctx, *grads):
-    """Runs a backward pass that has no gradient of its own; under create_graph
-    its results refuse to be differentiated (the wrapper for that costs 5 us,
-    so it is taken only there)."""
-    if torch.is_grad_enabled():
-        return torch.autograd.function.once_differentiable(backward)(ctx, *grads)
-    return backward(ctx, *grads)
-
-
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two contiguous tensors share memory."""
     pa, pb = a.data_ptr(), b.data_ptr()
@@ -417,31 +408,54 @@ def _balance_forward(logits, topi, mask):
     return loss, counts, coef
 
 
+def _balance_grad(lg, mask, coef, dloss):
+    T, E = lg.shape
+    d = torch.empty_like(lg)
+    with _device(lg.device):
+        _lib.check(_lib.lib().b200q_moe_balance_grad(lg.data_ptr(), _ptr(mask), coef.data_ptr(), dloss.data_ptr(), T, E,
+                                                     _LOGITS_CODES[lg.dtype], d.data_ptr(), _stream_ptr(lg.device)))
+    return d
+
+
+@torch.library.custom_op("b200q::moe_balance_grad", mutates_args=())
+def moe_balance_grad_op(logits: torch.Tensor, mask: Optional[torch.Tensor], coef: torch.Tensor,
+                        dloss: torch.Tensor) -> torch.Tensor:
+    """moe_balance_loss's gradient of contiguous logits; coef (32-bit words, the
+    first E used) from its forward pass, dloss fp32 [].  It has no derivative
+    of its own: differentiating its output raises."""
+    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _LOGITS_CODES:
+        raise TypeError("moe_balance_grad: router_logits must be [T, E] float16, bfloat16 or float32 on a GPU")
+    if coef.dtype not in (torch.int32, torch.float32) or coef.numel() < logits.shape[1] or not coef.is_contiguous():
+        raise ValueError("moe_balance_grad: coef must hold E contiguous 32-bit words")
+    if dloss.dtype != torch.float32 or dloss.numel() != 1:
+        raise ValueError("moe_balance_grad: dloss must be one float32")
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != logits.shape[:1] or not mask.is_contiguous()):
+        raise ValueError("moe_balance_grad: mask must be contiguous bool [T]")
+    _same_device("moe_balance_grad", logits, mask, coef, dloss)
+    return _balance_grad(logits.contiguous(), mask, coef, dloss)
+
+
+@moe_balance_grad_op.register_fake
+def _(logits, mask, coef, dloss):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, topi, mask):
-        lg = logits.contiguous()
-        loss, counts, coef = _balance_forward(lg, topi, mask)
-        ctx.save_for_backward(lg, mask, coef)
+        loss, counts, coef = _balance_forward(logits, topi, mask)
+        ctx.save_for_backward(logits, mask, coef)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)  # no zeros for counts
         return loss, counts
 
     @staticmethod
     def backward(ctx, dloss, _):
-        return _once(_balance_backward, ctx, dloss)
-
-
-def _balance_backward(ctx, dloss):
-    if dloss is None:
-        return None, None, None
-    lg, mask, coef = ctx.saved_tensors
-    T, E = lg.shape
-    d = torch.empty_like(lg)
-    with _device(lg.device):
-        _lib.check(_lib.lib().b200q_moe_balance_grad(lg.data_ptr(), _ptr(mask), coef.data_ptr(), dloss.data_ptr(), T, E,
-                                                     _LOGITS_CODES[lg.dtype], d.data_ptr(), _stream_ptr(lg.device)))
-    return d, None, None
+        if dloss is None:
+            return None, None, None
+        # under create_graph as an operator that refuses to be differentiated again
+        grad = moe_balance_grad_op if torch.is_grad_enabled() else _balance_grad
+        return grad(*ctx.saved_tensors, dloss), None, None
 
 
 def moe_balance_loss(router_logits: torch.Tensor, topi: torch.Tensor,
@@ -471,9 +485,10 @@ def moe_balance_loss(router_logits: torch.Tensor, topi: torch.Tensor,
     if topi.dtype == torch.int64:  # what 32 bits do not hold stays out of range
         topi = topi.clamp(-2, router_logits.shape[1]).to(torch.int32)
     topi = topi.contiguous()
-    if torch.is_grad_enabled() and router_logits.requires_grad:
-        return _BalanceLoss.apply(router_logits, topi, token_mask)
-    return _balance_forward(router_logits.contiguous(), topi, token_mask)[:2]
+    logits = router_logits.contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _BalanceLoss.apply(logits, topi, token_mask)
+    return _balance_forward(logits, topi, token_mask)[:2]
 
 
 def moe_grouped_gemm(x: torch.Tensor, offsets: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
@@ -660,7 +675,7 @@ def lora_plan(lora_ids: torch.Tensor, n_adapters: int) -> LoraPlan:
 
 def _lora_run(x, base, A, B, scaling, plan, out, lo):
     """One b200q_lora_apply call on contiguous, aligned tensors; returns the
-    sizes as the library takes them and the device."""
+    sizes as the library takes them."""
     n_adapters, D, r = A.shape
     T = x.shape[0]
     dev = x.device
@@ -671,7 +686,7 @@ def _lora_run(x, base, A, B, scaling, plan, out, lo):
         _lib.check(_lib.lib().b200q_lora_apply(x.data_ptr(), base.data_ptr(), A.data_ptr(), B.data_ptr(), _ptr(scaling),
                                                plan.data_ptr(), *sizes, out.data_ptr(), _ptr(lo), status,
                                                _stream_ptr(dev)))
-    return sizes, dev
+    return sizes
 
 
 @functools.lru_cache(maxsize=256)
@@ -690,10 +705,83 @@ def _lora_scratch(T: int, D: int, N: int, r: int, n_adapters: int, dtype: int, d
     return _lib.lib().b200q_lora_backward_scratch_bytes(T, D, N, r, n_adapters, dtype)
 
 
+def _lora_grads(sizes, x, d, base, A, B, scaling, plan, lo, dx, want_A, want_B):
+    """dA and dB; and dx (if given) = base (None: 0) + the adapters' part."""
+    dA = torch.empty_like(A) if want_A else None
+    dB = torch.empty_like(B) if want_B else None
+    dev = x.device
+    with _device(dev):
+        nbytes = _lora_scratch(*sizes, dev.index)
+        scratch = plan.new_empty(nbytes // 4)  # fp32 sums
+        status = None if sizes[0] <= _LORA_SMALL else workspace(dev, 256).data_ptr()
+        _lib.check(_lib.lib().b200q_lora_backward(
+            x.data_ptr(), d.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling), plan.data_ptr(),
+            lo.data_ptr(), *sizes, scratch.data_ptr(), nbytes, _ptr(dx), _ptr(dA), _ptr(dB), status, _stream_ptr(dev)))
+    return dA, dB
+
+
+@torch.library.custom_op("b200q::lora_backward", mutates_args=())
+def lora_backward_op(x: torch.Tensor, dy: torch.Tensor, base: Optional[torch.Tensor], A: torch.Tensor, B: torch.Tensor,
+                     scaling: Optional[torch.Tensor], plan: torch.Tensor, lo: torch.Tensor, want_x: bool, want_A: bool,
+                     want_B: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """lora_apply's gradients (dx = base + its part, dA, dB), empty where one is not
+    wanted; plan and lo from the forward pass.  They have no derivative of
+    their own: differentiating them raises."""
+    sizes = _lora_operands("lora_backward", x, A, B, scaling, plan, dy=dy, base=base, lo=lo)
+    x, dy, A, B = _aligned(x), _aligned(dy), _aligned(A), _aligned(B)
+    dx = torch.empty_like(x) if want_x else x.new_empty(0)
+    dA, dB = _lora_grads(sizes, x, dy, None if base is None else _aligned(base), A, B, scaling, plan, lo,
+                         dx if want_x else None, want_A, want_B)
+    return dx, dA if want_A else A.new_empty(0), dB if want_B else B.new_empty(0)
+
+
+@lora_backward_op.register_fake
+def _(x, dy, base, A, B, scaling, plan, lo, want_x, want_A, want_B):
+    return tuple(t.new_empty(t.shape) if want else t.new_empty(0) for t, want in ((x, want_x), (A, want_A), (B, want_B)))
+
+
+def _lora_operands(op, x, A, B, scaling, plan, *, dy=None, base=None, lo=None):
+    """Checks what a registered operator is given; returns the sizes as the library takes them."""
+    if not x.is_cuda or x.dim() != 2 or A.dim() != 3 or B.dim() != 3:
+        raise ValueError(f"{op}: x [T, D], A [L, D, r] and B [L, r, N] on a GPU expected")
+    (T, D), (n_adapters, _, r), N = x.shape, A.shape, B.shape[2]
+    code = _dtype_code(x.dtype)
+    for t, shape in ((A, (n_adapters, D, r)), (B, (n_adapters, r, N)), (dy, (T, N)), (base, (T, D) if dy is not None else (T, N))):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != x.dtype):
+            raise ValueError(f"{op}: {list(shape)} of {x.dtype} expected, got {tuple(t.shape)} of {t.dtype}")
+    if plan.dtype != torch.int32 or not plan.is_contiguous() or plan.data_ptr() % 16 or \
+            4 * plan.numel() < max(1, _lib.lib().b200q_lora_plan_bytes(T, n_adapters)):
+        raise ValueError(f"{op}: not a plan of {T} tokens and {n_adapters} adapters")
+    if lo is not None and (lo.dtype not in (torch.int32, torch.float32) or not lo.is_contiguous() or
+                           4 * lo.numel() < _lib.lib().b200q_lora_mid_bytes(T, r)):
+        raise ValueError(f"{op}: lo is not the forward pass's")
+    if scaling is not None and (scaling.dtype != torch.float32 or tuple(scaling.shape) != (n_adapters,) or
+                                not scaling.is_contiguous()):
+        raise ValueError(f"{op}: scaling must be contiguous float32 [{n_adapters}]")
+    _same_device(op, x, A, B, scaling, plan, dy, base, lo)
+    return T, D, N, r, n_adapters, code
+
+
+def _lora_backward(sizes, x, d, base, A, B, scaling, plan, lo, dx, want_x, want_A, want_B):
+    """(dx, dA, dB) for a Function's backward pass; dx: where to put it (base itself), or None."""
+    if torch.is_grad_enabled():
+        # create_graph: operators that refuse to be differentiated again, one for each
+        # gradient, so that each refuses exactly where it depends on something that
+        # asks for a gradient of its own
+        rest = (scaling, plan, lo)
+        return (lora_backward_op(x.detach(), d, base, A, B, *rest, True, False, False)[0] if want_x else None,
+                lora_backward_op(x, d, None, A.detach(), B, *rest, False, True, False)[1] if want_A else None,
+                lora_backward_op(x, d, None, A, B.detach(), *rest, False, False, True)[2] if want_B else None)
+    if dx is None and want_x:
+        dx = torch.empty_like(x)
+    if not (want_x or want_A or want_B):
+        return None, None, None
+    return (dx, *_lora_grads(sizes, x, d, base, A, B, scaling, plan, lo, dx, want_A, want_B))
+
+
 class _LoraApply(torch.autograd.Function):
     @staticmethod
     def forward(ctx, base, x, A, B, scaling, plan):
-        base, x, A, B = _aligned(base), _aligned(x), _aligned(A), _aligned(B)
         y, lo = torch.empty_like(base), _lora_mid(plan, A.shape[2])
         ctx.sizes = _lora_run(x, base, A, B, scaling, plan.data, y, lo)
         ctx.save_for_backward(x, A, B, scaling)
@@ -702,33 +790,10 @@ class _LoraApply(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _once(_lora_backward, ctx, dy)
-
-
-def _lora_grads(ctx, x, A, B, scaling, d, dx, base, need_A, need_B):
-    """dA and dB; and dx (if given) = base (None: 0) + the adapters' part."""
-    dA = torch.empty_like(A) if need_A else None
-    dB = torch.empty_like(B) if need_B else None
-    sizes, dev = ctx.sizes
-    with _device(dev):
-        nbytes = _lora_scratch(*sizes, dev.index)
-        scratch = ctx.plan.new_empty(nbytes // 4)  # fp32 sums
-        status = None if sizes[0] <= _LORA_SMALL else workspace(dev, 256).data_ptr()
-        _lib.check(_lib.lib().b200q_lora_backward(
-            x.data_ptr(), d.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling), ctx.plan.data_ptr(),
-            ctx.lo.data_ptr(), *sizes, scratch.data_ptr(), nbytes, _ptr(dx), _ptr(dA), _ptr(dB), status,
-            _stream_ptr(dev)))
-    return dA, dB
-
-
-def _lora_backward(ctx, dy):
-    x, A, B, scaling = ctx.saved_tensors
-    need_base, need_x, need_A, need_B = ctx.needs_input_grad[:4]
-    dx = torch.empty_like(x) if need_x else None
-    dA = dB = None
-    if need_x or need_A or need_B:
-        dA, dB = _lora_grads(ctx, x, A, B, scaling, _aligned(dy), dx, None, need_A, need_B)
-    return dy if need_base else None, dx, dA, dB, None, None
+        x, A, B, scaling = ctx.saved_tensors
+        want_base, *want = ctx.needs_input_grad[:4]
+        grads = _lora_backward(ctx.sizes, x, _aligned(dy), None, A, B, scaling, ctx.plan, ctx.lo, None, *want)
+        return (dy if want_base else None, *grads, None, None)
 
 
 class _LoRAW4A16(torch.autograd.Function):
@@ -736,7 +801,6 @@ class _LoRAW4A16(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, A, B, qweight, scales, zeros, group, scaling, plan):
-        x, A, B = _aligned(x), _aligned(A), _aligned(B)
         y, lo = w4a16_gemm(x, qweight, scales, zeros, group), _lora_mid(plan, A.shape[2])
         ctx.sizes = _lora_run(x, y, A, B, scaling, plan.data, y, lo)
         ctx.save_for_backward(x, A, B, scaling, qweight, scales, zeros)
@@ -745,18 +809,14 @@ class _LoRAW4A16(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _once(_lora_w4a16_backward, ctx, dy)
-
-
-def _lora_w4a16_backward(ctx, dy):
-    x, A, B, scaling, qweight, scales, zeros = ctx.saved_tensors
-    need_x, need_A, need_B, _, need_scales, need_zeros = ctx.needs_input_grad[:6]
-    if need_scales or need_zeros:
-        raise RuntimeError("lora_w4a16: the quantised weight is frozen, scales and zeros have no gradient")
-    d = _aligned(dy)
-    dx = w4a16_dgrad(d, qweight, scales, zeros, ctx.group) if need_x else None
-    dA, dB = _lora_grads(ctx, x, A, B, scaling, d, dx, dx, need_A, need_B)
-    return dx, dA, dB, None, None, None, None, None, None
+        x, A, B, scaling, qweight, scales, zeros = ctx.saved_tensors
+        *want, _, need_scales, need_zeros = ctx.needs_input_grad[:6]
+        if need_scales or need_zeros:
+            raise RuntimeError("lora_w4a16: the quantised weight is frozen, scales and zeros have no gradient")
+        d = _aligned(dy)
+        dx = w4a16_dgrad(d, qweight, scales, zeros, ctx.group) if want[0] else None
+        grads = _lora_backward(ctx.sizes, x, d, dx, A, B, scaling, ctx.plan, ctx.lo, dx, *want)
+        return (*grads, None, None, None, None, None, None)
 
 
 def _lora_check(op, x, A, B, plan, scaling):
@@ -815,7 +875,7 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     if torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad or base.requires_grad):
         if out is not None:
             raise ValueError("lora_apply: out cannot be given where a gradient is wanted")
-        return _LoraApply.apply(base, x, A, B, scaling, plan)
+        return _LoraApply.apply(_aligned(base), _aligned(x), _aligned(A), _aligned(B), scaling, plan)
     out_given = out is not None
     if not out_given:
         base = _aligned(base)
@@ -846,7 +906,7 @@ def lora_w4a16(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zer
         raise ValueError(f"lora_w4a16: qweight {tuple(qweight.shape)} does not fit B {tuple(B.shape)}")
     _same_device("lora_w4a16", x, qweight, scales, zeros)
     if torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad):
-        return _LoRAW4A16.apply(x, A, B, qweight, scales, zeros, group, scaling, plan)
+        return _LoRAW4A16.apply(_aligned(x), _aligned(A), _aligned(B), qweight, scales, zeros, group, scaling, plan)
     y = w4a16_gemm(x, qweight, scales, zeros, group)
     x = _aligned(x)
     lo = None if x.shape[0] <= _LORA_SMALL else _lora_mid(plan, A.shape[2])
