@@ -458,6 +458,39 @@ class _BalanceLoss(torch.autograd.Function):
         return grad(*ctx.saved_tensors, dloss), None, None
 
 
+@torch.library.custom_op("b200q::moe_balance", mutates_args=())
+def moe_balance_op(logits: torch.Tensor, topi: torch.Tensor,
+                   mask: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """moe_balance_loss as a registered operator: topi int32; (loss, counts, coef [E], which the gradient takes)."""
+    if not logits.is_cuda or logits.dim() != 2 or topi.dim() != 2 or topi.shape[0] != logits.shape[0]:
+        raise ValueError("moe_balance: router_logits [T, E] and topi [T, k] on a GPU expected")
+    if logits.dtype not in _LOGITS_CODES or topi.dtype != torch.int32:
+        raise TypeError("moe_balance: router_logits must be float16, bfloat16 or float32, topi int32")
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != logits.shape[:1]):
+        raise ValueError("moe_balance: mask must be bool [T]")
+    _same_device("moe_balance", logits, topi, mask)
+    loss, counts, coef = _balance_forward(logits.contiguous(), topi.contiguous(), None if mask is None else mask.contiguous())
+    return loss, counts, coef[:logits.shape[1]].clone()  # without the kernel's scratch
+
+
+@moe_balance_op.register_fake
+def _(logits, topi, mask):
+    E = logits.shape[1]
+    return logits.new_empty((), dtype=torch.float32), topi.new_empty(E), topi.new_empty(E)
+
+
+def _balance_setup(ctx, inputs, output):
+    ctx.save_for_backward(inputs[0], inputs[2], output[2])
+
+
+def _balance_op_backward(ctx, dloss, *_):
+    lg, mask, coef = ctx.saved_tensors
+    return moe_balance_grad_op(lg, mask, coef, dloss), None, None
+
+
+moe_balance_op.register_autograd(_balance_op_backward, setup_context=_balance_setup)
+
+
 def moe_balance_loss(router_logits: torch.Tensor, topi: torch.Tensor,
                      token_mask: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Load-balance loss of a top-k router and the per-expert token counts.
@@ -486,6 +519,8 @@ def moe_balance_loss(router_logits: torch.Tensor, topi: torch.Tensor,
         topi = topi.clamp(-2, router_logits.shape[1]).to(torch.int32)
     topi = topi.contiguous()
     logits = router_logits.contiguous()
+    if _dispatched(logits):
+        return moe_balance_op(logits, topi, token_mask)[:2]
     if torch.is_grad_enabled() and logits.requires_grad:
         return _BalanceLoss.apply(logits, topi, token_mask)
     return _balance_forward(logits, topi, token_mask)[:2]
@@ -662,6 +697,11 @@ def lora_plan(lora_ids: torch.Tensor, n_adapters: int) -> LoraPlan:
     if lora_ids.dim() != 1 or lora_ids.dtype not in (torch.int32, torch.int64):
         raise ValueError("lora_ids must be int32 or int64 [T]")
     ids = lora_ids.to(torch.int64).contiguous()
+    data = (lora_plan_op if _dispatched(ids) else _lora_plan)(ids, n_adapters)
+    return LoraPlan(data, ids.shape[0], n_adapters)
+
+
+def _lora_plan(ids, n_adapters):
     T, dev = ids.numel(), ids.device
     L = _lib.lib()
     nbytes = L.b200q_lora_plan_bytes(T, n_adapters)
@@ -670,7 +710,27 @@ def lora_plan(lora_ids: torch.Tensor, n_adapters: int) -> LoraPlan:
         ws = workspace(dev, 256)
         _lib.check(L.b200q_lora_plan(ids.data_ptr(), T, n_adapters, data.data_ptr(), nbytes, ws.data_ptr(),
                                      _stream_ptr(dev)))
-    return LoraPlan(data, T, n_adapters)
+    return data
+
+
+@torch.library.custom_op("b200q::lora_plan", mutates_args=())
+def lora_plan_op(lora_ids: torch.Tensor, n_adapters: int) -> torch.Tensor:
+    """lora_plan's words as a registered operator: lora_ids int64 [T]."""
+    if not lora_ids.is_cuda or lora_ids.dim() != 1 or lora_ids.dtype != torch.int64:
+        raise ValueError("lora_plan: lora_ids int64 [T] on a GPU expected")
+    return _lora_plan(lora_ids.contiguous(), n_adapters)
+
+
+def _plan_words(T, n_adapters):
+    """b200q_lora_plan_bytes / 4 (the layout is in lora_seg.cuh); T may be symbolic."""
+    up4 = lambda v: (v + 3) // 4 * 4  # noqa: E731
+    tiles = lambda rows: torch.sym_min(T // rows + n_adapters + 1, T)  # noqa: E731
+    return up4(up4(8 + n_adapters + 2) + T) + 4 * (tiles(16) + tiles(128))
+
+
+@lora_plan_op.register_fake
+def _(lora_ids, n_adapters):
+    return lora_ids.new_empty(_plan_words(lora_ids.shape[0], n_adapters), dtype=torch.int32)
 
 
 def _lora_run(x, base, A, B, scaling, plan, out, lo):
@@ -772,6 +832,9 @@ def _lora_backward(sizes, x, d, base, A, B, scaling, plan, lo, dx, want_x, want_
         return (lora_backward_op(x.detach(), d, base, A, B, *rest, True, False, False)[0] if want_x else None,
                 lora_backward_op(x, d, None, A.detach(), B, *rest, False, True, False)[1] if want_A else None,
                 lora_backward_op(x, d, None, A, B.detach(), *rest, False, False, True)[2] if want_B else None)
+    if _dispatched(d):
+        out = lora_backward_op(x, d, base, A, B, scaling, plan, lo, want_x, want_A, want_B)
+        return tuple(g if want else None for g, want in zip(out, (want_x, want_A, want_B)))
     if dx is None and want_x:
         dx = torch.empty_like(x)
     if not (want_x or want_A or want_B):
@@ -817,6 +880,77 @@ class _LoRAW4A16(torch.autograd.Function):
         dx = w4a16_dgrad(d, qweight, scales, zeros, ctx.group) if want[0] else None
         grads = _lora_backward(ctx.sizes, x, d, dx, A, B, scaling, ctx.plan, ctx.lo, dx, *want)
         return (*grads, None, None, None, None, None, None)
+
+
+@torch.library.custom_op("b200q::lora_apply", mutates_args=())
+def lora_apply_op(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, scaling: Optional[torch.Tensor],
+                  plan: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """lora_apply as a registered operator, on a plan's words: (y, lo), lo as b200q_lora_apply leaves it."""
+    sizes = _lora_operands("lora_apply", x, A, B, scaling, plan, base=base)
+    base, x, A, B = _aligned(base), _aligned(x), _aligned(A), _aligned(B)
+    y, lo = torch.empty_like(base), plan.new_empty(_lora_mid_values(sizes[0], sizes[3]))
+    _lora_run(x, base, A, B, scaling, plan, y, lo)
+    return y, lo
+
+
+@torch.library.custom_op("b200q::lora_w4a16", mutates_args=())
+def lora_w4a16_op(x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
+                  zeros: torch.Tensor, group: int, scaling: Optional[torch.Tensor],
+                  plan: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """lora_w4a16 as a registered operator, on a plan's words: (y, lo)."""
+    sizes = _lora_operands("lora_w4a16", x, A, B, scaling, plan)
+    if qweight.dim() != 2 or qweight.shape[1] * 8 != B.shape[2]:
+        raise ValueError(f"lora_w4a16: qweight {tuple(qweight.shape)} does not fit B {tuple(B.shape)}")
+    x, A, B = _aligned(x), _aligned(A), _aligned(B)
+    y, lo = w4a16_gemm(x, qweight, scales, zeros, group), plan.new_empty(_lora_mid_values(sizes[0], sizes[3]))
+    _lora_run(x, y, A, B, scaling, plan, y, lo)
+    return y, lo
+
+
+def _lo_words(x, A, plan):
+    r = A.shape[2]
+    return plan.new_empty(x.shape[0] * (16 if r <= 16 else 32 if r <= 32 else 64))  # b200q_lora_mid_bytes / 4
+
+
+@lora_apply_op.register_fake
+def _(base, x, A, B, scaling, plan):
+    return base.new_empty(base.shape), _lo_words(x, A, plan)
+
+
+@lora_w4a16_op.register_fake
+def _(x, A, B, qweight, scales, zeros, group, scaling, plan):
+    return x.new_empty((x.shape[0], B.shape[2])), _lo_words(x, A, plan)
+
+
+def _lora_apply_setup(ctx, inputs, output):
+    _, x, A, B, scaling, plan = inputs
+    ctx.save_for_backward(x, A, B, scaling, plan, output[1])
+
+
+def _lora_apply_backward(ctx, dy, _):
+    x, A, B, scaling, plan, lo = ctx.saved_tensors
+    want_base, *want = ctx.needs_input_grad[:4]
+    grads = _lora_backward(None, x, dy, None, A, B, scaling, plan, lo, None, *want)
+    return (dy if want_base else None, *grads, None, None)
+
+
+def _lora_w4a16_setup(ctx, inputs, output):
+    x, A, B, qweight, scales, zeros, ctx.group, scaling, plan = inputs
+    ctx.save_for_backward(x, A, B, qweight, scales, zeros, scaling, plan, output[1])
+
+
+def _lora_w4a16_backward(ctx, dy, _):
+    x, A, B, qweight, scales, zeros, scaling, plan, lo = ctx.saved_tensors
+    *want, _, need_scales, need_zeros = ctx.needs_input_grad[:6]
+    if need_scales or need_zeros:
+        raise RuntimeError("lora_w4a16: the quantised weight is frozen, scales and zeros have no gradient")
+    dx = w4a16_dgrad(dy, qweight, scales, zeros, ctx.group) if want[0] else None
+    grads = _lora_backward(None, x, dy, dx, A, B, scaling, plan, lo, dx, *want)
+    return (*grads, None, None, None, None, None, None)
+
+
+lora_apply_op.register_autograd(_lora_apply_backward, setup_context=_lora_apply_setup)
+lora_w4a16_op.register_autograd(_lora_w4a16_backward, setup_context=_lora_w4a16_setup)
 
 
 def _lora_check(op, x, A, B, plan, scaling):
@@ -872,6 +1006,13 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     if base.dtype != dt:
         raise TypeError(f"lora_apply: base is {base.dtype}, x is {dt}")
     _same_device("lora_apply", x, base, out)
+    if _dispatched(x):
+        y = lora_apply_op(base, x, A, B, scaling, plan.data)[0]
+        if out is None:
+            return y
+        if out.shape != base.shape or out.dtype != dt:
+            raise ValueError("lora_apply: out must be a [T, N] tensor of x's dtype")
+        return out.copy_(y)
     if torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad or base.requires_grad):
         if out is not None:
             raise ValueError("lora_apply: out cannot be given where a gradient is wanted")
@@ -905,6 +1046,8 @@ def lora_w4a16(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zer
     if qweight.dim() != 2 or qweight.shape[1] * 8 != B.shape[2]:
         raise ValueError(f"lora_w4a16: qweight {tuple(qweight.shape)} does not fit B {tuple(B.shape)}")
     _same_device("lora_w4a16", x, qweight, scales, zeros)
+    if _dispatched(x):
+        return lora_w4a16_op(x, A, B, qweight, scales, zeros, group, scaling, plan.data)[0]
     if torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad):
         return _LoRAW4A16.apply(_aligned(x), _aligned(A), _aligned(B), qweight, scales, zeros, group, scaling, plan)
     y = w4a16_gemm(x, qweight, scales, zeros, group)
