@@ -847,15 +847,14 @@ class _LoraApply(torch.autograd.Function):
     def forward(ctx, base, x, A, B, scaling, plan):
         y, lo = torch.empty_like(base), _lora_mid(plan, A.shape[2])
         ctx.sizes = _lora_run(x, base, A, B, scaling, plan.data, y, lo)
-        ctx.save_for_backward(x, A, B, scaling)
-        ctx.lo, ctx.plan = lo, plan.data  # seen by nobody else
+        ctx.save_for_backward(x, A, B, scaling, plan.data, lo)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, A, B, scaling = ctx.saved_tensors
+        x, A, B, scaling, plan, lo = ctx.saved_tensors
         want_base, *want = ctx.needs_input_grad[:4]
-        grads = _lora_backward(ctx.sizes, x, _aligned(dy), None, A, B, scaling, ctx.plan, ctx.lo, None, *want)
+        grads = _lora_backward(ctx.sizes, x, _aligned(dy), None, A, B, scaling, plan, lo, None, *want)
         return (dy if want_base else None, *grads, None, None)
 
 
@@ -866,19 +865,19 @@ class _LoRAW4A16(torch.autograd.Function):
     def forward(ctx, x, A, B, qweight, scales, zeros, group, scaling, plan):
         y, lo = w4a16_gemm(x, qweight, scales, zeros, group), _lora_mid(plan, A.shape[2])
         ctx.sizes = _lora_run(x, y, A, B, scaling, plan.data, y, lo)
-        ctx.save_for_backward(x, A, B, scaling, qweight, scales, zeros)
-        ctx.lo, ctx.plan, ctx.group = lo, plan.data, group
+        ctx.save_for_backward(x, A, B, scaling, qweight, scales, zeros, plan.data, lo)
+        ctx.group = group
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, A, B, scaling, qweight, scales, zeros = ctx.saved_tensors
+        x, A, B, scaling, qweight, scales, zeros, plan, lo = ctx.saved_tensors
         *want, _, need_scales, need_zeros = ctx.needs_input_grad[:6]
         if need_scales or need_zeros:
             raise RuntimeError("lora_w4a16: the quantised weight is frozen, scales and zeros have no gradient")
         d = _aligned(dy)
         dx = w4a16_dgrad(d, qweight, scales, zeros, ctx.group) if want[0] else None
-        grads = _lora_backward(ctx.sizes, x, d, dx, A, B, scaling, ctx.plan, ctx.lo, dx, *want)
+        grads = _lora_backward(ctx.sizes, x, d, dx, A, B, scaling, plan, lo, dx, *want)
         return (*grads, None, None, None, None, None, None)
 
 
