@@ -13,6 +13,7 @@ import threading
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -79,6 +80,13 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _no_tangent(op: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses dual tensors (forward-mode differentiation), whose tangents the kernels do not see."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError(f"{op} has no forward-mode derivative")
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two contiguous tensors share memory."""
     pa, pb = a.data_ptr(), b.data_ptr()
@@ -96,6 +104,7 @@ def _same_device(op: str, first: torch.Tensor, *rest: Optional[torch.Tensor]) ->
 def w4a16_gemm(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
                group: int) -> torch.Tensor:
     """y[M, N] = x[M, K] . ((unpack(qweight) - zeros) * scales), y in x.dtype."""
+    _no_tangent("w4a16_gemm", x)
     if not x.is_cuda:
         raise RuntimeError("b200q::w4a16_gemm runs on CUDA tensors only (no CPU implementation)")
     if x.dim() != 2 or qweight.dim() != 2:
@@ -146,6 +155,7 @@ def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, z
     """dx[M, K] = dy[M, N] . ((unpack(qweight) - zeros) * scales)^T, dx in dy.dtype:
     the input gradient of w4a16_gemm (the weights are frozen).  Differentiable
     in dy, w4a16_gemm being its gradient in turn."""
+    _no_tangent("w4a16_dgrad", dy)
     if (torch.is_grad_enabled() and (dy.requires_grad or scales.requires_grad or zeros.requires_grad)) or _dispatched(dy):
         return w4a16_dgrad_op(dy, qweight, scales, zeros, group)
     return _w4a16_dgrad(dy, qweight, scales, zeros, group)
@@ -502,6 +512,7 @@ def moe_balance_loss(router_logits: torch.Tensor, topi: torch.Tensor,
     probability of e; counts [E] int32.  The loss is differentiable in
     router_logits (f is a count and carries no gradient); see include/b200q.h
     for rows that are all -inf and for indices out of range."""
+    _no_tangent("moe_balance_loss", router_logits)
     if not router_logits.is_cuda:
         raise RuntimeError("b200q moe_balance_loss runs on CUDA tensors only")
     if router_logits.dim() != 2 or topi.dim() != 2 or topi.shape[0] != router_logits.shape[0]:
@@ -955,6 +966,7 @@ lora_w4a16_op.register_autograd(_lora_w4a16_backward, setup_context=_lora_w4a16_
 def _lora_check(op, x, A, B, plan, scaling):
     """Checks the adapter operands that lora_apply and lora_w4a16 share; returns
     A and B in x's dtype, the plan and scaling as fp32."""
+    _no_tangent(op, x, A, B)
     if not x.is_cuda:
         raise RuntimeError(f"b200q {op} runs on CUDA tensors only")
     if x.dim() != 2 or A.dim() != 3 or B.dim() != 3:
@@ -998,6 +1010,7 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     fp32; y is rounded once.  Differentiable in base, x, A and B (scaling is a
     constant).  ``out`` (which may be ``base``: in place) takes the result
     where no gradient is wanted."""
+    _no_tangent("lora_apply", base)
     A, B, plan, scaling = _lora_check("lora_apply", x, A, B, plan, scaling)
     T, dt = x.shape[0], x.dtype
     if base.shape != (T, B.shape[2]):

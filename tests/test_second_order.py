@@ -173,3 +173,42 @@ def test_registered_operators_refuse_what_does_not_fit():
                  (lg, torch.ones(3, dtype=torch.bool, device="cuda"), coef, one), (lg, None, coef, one.cpu())):
         with pytest.raises((ValueError, TypeError)):
             ops.moe_balance_grad_op(*args)
+
+
+# ---------------------------------------------------------------- forward mode: refused
+def test_tangents_are_refused():
+    """On any device: the check comes first, and a tensor without a tangent goes on."""
+    import torch.autograd.forward_ad as fw
+    z = torch.zeros
+    ids, plain = z(4, dtype=torch.int64), dict(base=z(4, 8), x=z(4, 8), A=z(2, 8, 4), B=z(2, 4, 8))
+    q, s = z(8, 1, dtype=torch.int32), z(1, 8)
+    with fw.dual_level():
+        dual = {k: fw.make_dual(t, torch.ones_like(t)) for k, t in plain.items()}
+        for k in plain:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                ops.lora_apply(**{**plain, k: dual[k]}, plan=ids)
+        for k in ("x", "A", "B"):
+            a = {**plain, k: dual[k]}
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                ops.lora_w4a16(a["x"], q, s, s, 8, a["A"], a["B"], ids)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.w4a16_dgrad(dual["x"], q, s, s, 8)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.w4a16_gemm(dual["x"], q, s, s, 8)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.moe_balance_loss(dual["x"], z(4, 2, dtype=torch.int32))
+        with pytest.raises(RuntimeError, match="CUDA"):  # no tangent: on to the next check
+            ops.lora_apply(**plain, plan=ids)
+
+
+@pytest.mark.gpu
+def test_tangent_of_the_base_is_refused():
+    import torch.autograd.forward_ad as fw
+    c, ids = adapters(20)
+    with fw.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.lora_apply(fw.make_dual(c["base"], c["base"]), c["x"], c["A"], c["B"], ids)
+        lg = fw.make_dual(torch.zeros(4, 8, device="cuda"), torch.ones(4, 8, device="cuda"))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.moe_balance_loss(lg, torch.zeros(4, 2, dtype=torch.int32, device="cuda"))
+        ops.lora_apply(c["base"], c["x"], c["A"], c["B"], ids)  # no tangent: as ever
