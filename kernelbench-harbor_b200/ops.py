@@ -671,6 +671,20 @@ def lora_shrink(x: torch.Tensor, A: torch.Tensor, lora_ids: torch.Tensor) -> tor
     return lo
 
 
+class _Overwritten(torch.autograd.Function):
+    """A tensor with a gradient history that an operator without a gradient has written over."""
+
+    @staticmethod
+    def forward(ctx, op, t):
+        ctx.op = op
+        ctx.mark_dirty(t)
+        return t
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"{ctx.op} has no gradient (lora_apply and lora_w4a16 have)")
+
+
 def lora_expand_add(base: torch.Tensor, lo: torch.Tensor, B: torch.Tensor, lora_ids: torch.Tensor,
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """y [T, N] = base + round(lo[t] . B[lora_ids[t]]) (B [L, r, N])."""
@@ -682,6 +696,8 @@ def lora_expand_add(base: torch.Tensor, lo: torch.Tensor, B: torch.Tensor, lora_
     _lib.check(_lib.lib().b200q_lora_expand_add(base.data_ptr(), lo.data_ptr(), B.data_ptr(), ids.data_ptr(), T, r,
                                                 N, L, _dtype_code(base.dtype), y.data_ptr(),
                                                 _stream_ptr(base.device)))
+    if y.requires_grad and torch.is_grad_enabled():  # out=: its history ends here
+        return _Overwritten.apply("lora_expand_add", y)
     return y
 
 
