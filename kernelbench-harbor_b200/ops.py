@@ -671,6 +671,12 @@ def lora_shrink(x: torch.Tensor, A: torch.Tensor, lora_ids: torch.Tensor) -> tor
     return lo
 
 
+def _written(out: torch.Tensor) -> None:
+    """Tells autograd that a kernel has written over out: what saved it refuses its new contents."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 class _Overwritten(torch.autograd.Function):
     """A tensor with a gradient history that an operator without a gradient has written over."""
 
@@ -696,8 +702,10 @@ def lora_expand_add(base: torch.Tensor, lo: torch.Tensor, B: torch.Tensor, lora_
     _lib.check(_lib.lib().b200q_lora_expand_add(base.data_ptr(), lo.data_ptr(), B.data_ptr(), ids.data_ptr(), T, r,
                                                 N, L, _dtype_code(base.dtype), y.data_ptr(),
                                                 _stream_ptr(base.device)))
-    if y.requires_grad and torch.is_grad_enabled():  # out=: its history ends here
-        return _Overwritten.apply("lora_expand_add", y)
+    if out is not None:
+        if out.requires_grad and torch.is_grad_enabled():  # its history ends here
+            return _Overwritten.apply("lora_expand_add", out)
+        _written(out)
     return y
 
 
@@ -1034,6 +1042,10 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     if base.dtype != dt:
         raise TypeError(f"lora_apply: base is {base.dtype}, x is {dt}")
     _same_device("lora_apply", x, base, out)
+    wanted = torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad or base.requires_grad or
+                                          (out is not None and out.requires_grad))
+    if wanted and out is not None:
+        raise ValueError("lora_apply: out cannot be given where a gradient is wanted")
     if _dispatched(x):
         y = lora_apply_op(base, x, A, B, scaling, plan.data)[0]
         if out is None:
@@ -1041,9 +1053,7 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
         if out.shape != base.shape or out.dtype != dt:
             raise ValueError("lora_apply: out must be a [T, N] tensor of x's dtype")
         return out.copy_(y)
-    if torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad or base.requires_grad):
-        if out is not None:
-            raise ValueError("lora_apply: out cannot be given where a gradient is wanted")
+    if wanted:
         return _LoraApply.apply(_aligned(base), _aligned(x), _aligned(A), _aligned(B), scaling, plan)
     out_given = out is not None
     if not out_given:
@@ -1060,6 +1070,8 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     # the one-launch kernel needs no room for the row between
     lo = None if T <= _LORA_SMALL else _lora_mid(plan, A.shape[2])
     _lora_run(x, base, A, B, scaling, plan.data, out, lo)
+    if out_given:
+        _written(out)
     return out
 
 

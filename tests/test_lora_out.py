@@ -26,3 +26,47 @@ def test_module_without_a_gradient_says_so():
     # adapters that ask for a gradient beside an input that does not: as ever, none is recorded
     y = MultiLoRAW4()(c["x"], q, s, c["A"].clone().requires_grad_(), c["B"].clone().requires_grad_(), ids)
     assert torch.equal(y, want) and not y.requires_grad
+
+
+def forms(c):
+    return (lambda out: ops.lora_apply(out, c["x"], c["A"], c["B"], c["ids"], c["scaling"], out=out),
+            lambda out: ops.lora_apply(c["base"], c["x"], c["A"], c["B"], c["ids"], c["scaling"], out=out),
+            lambda out: ops.lora_expand_add(out, c["x"][:, :8].contiguous(), c["B"], c["ids"].clamp(min=0), out=out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [20, 300])
+def test_what_saved_the_base_sees_the_change(T):
+    """base takes no gradient, but an operator before has saved it for its own:
+    written over, its backward refuses, as after PyTorch's in-place operators."""
+    c = inputs(T, 128, 96, 8, 2, "bf16", "runs")
+    for f in forms(c):
+        w, base = torch.ones(96, device="cuda").bfloat16().requires_grad_(), c["base"].clone()
+        z = base * w
+        before = base._version
+        assert f(base) is base and base._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+        # tensors without a version
+        with torch.inference_mode():
+            base = c["base"].clone()
+            want = f(base).clone()
+        with torch.no_grad():
+            base = c["base"].clone()
+            assert torch.equal(f(base), want)
+        with torch.inference_mode():
+            base = c["base"].clone()
+        assert torch.equal(f(base), want)
+
+
+@pytest.mark.gpu
+def test_out_that_asks_for_a_gradient():
+    c = inputs(20, 128, 96, 8, 2, "bf16", "runs")
+    leaf = torch.zeros_like(c["base"]).requires_grad_()
+    for out in (leaf, leaf * 1):
+        with pytest.raises(ValueError, match="out cannot be given"):
+            ops.lora_apply(c["base"], c["x"], c["A"], c["B"], c["ids"], out=out)
+        assert (out == 0).all()
+    with torch.no_grad():
+        ops.lora_apply(c["base"], c["x"], c["A"], c["B"], c["ids"], out=leaf)
+    assert torch.equal(leaf.detach(), ops.lora_apply(c["base"], c["x"], c["A"], c["B"], c["ids"]))
