@@ -129,10 +129,11 @@ def w4a16_gemm(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zer
         return y
     L = _lib.lib()
     nbytes = L.b200q_w4a16_workspace_bytes(M, N, K, group, x.device.index)
-    ws = workspace(x.device, nbytes)
-    _lib.check(L.b200q_w4a16_gemm(x.data_ptr(), qweight.data_ptr(), scales.data_ptr(), zeros.data_ptr(),
-                                  y.data_ptr(), M, N, K, group, dt, ws.data_ptr(), ws.numel(),
-                                  _stream_ptr(x.device)))
+    with _device(x.device):
+        ws = workspace(x.device, nbytes)
+        _lib.check(L.b200q_w4a16_gemm(x.data_ptr(), qweight.data_ptr(), scales.data_ptr(), zeros.data_ptr(),
+                                      y.data_ptr(), M, N, K, group, dt, ws.data_ptr(), ws.numel(),
+                                      _stream_ptr(x.device)))
     return y
 
 
