@@ -25,7 +25,7 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Zero-initialised scratch owned by this process, one per (device, stream).
     Kernels return it to the zero state, so it is allocated (and zeroed) once
     and reused; it is never shared by two streams, whose launches could overlap."""
-    key = (device.index, _stream_ptr(device))
+    key = (_index(device), _stream_ptr(device))
     with _ws_lock:
         buf = _ws.get(key)
         if buf is None or buf.numel() < nbytes:
@@ -54,9 +54,13 @@ def _dtype_code(dt: torch.dtype) -> int:
     raise TypeError(f"activations must be float16 or bfloat16, got {dt}")
 
 
+def _index(device: torch.device) -> int:
+    return torch.cuda.current_device() if device.index is None else device.index
+
+
 def _stream_ptr(device: torch.device) -> int:
     # torch.cuda.current_stream(device).cuda_stream without the Stream object (0.1 us instead of 2.2)
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    return torch._C._cuda_getCurrentRawStream(_index(device))
 
 
 class _NoSwitch:

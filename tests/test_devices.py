@@ -64,3 +64,12 @@ def test_every_launch_is_made_on_the_tensors_device(T, monkeypatch):
     assert {"b200q_" + n for n in ("lora_plan", "lora_apply", "lora_backward", "w4a16_gemm", "w4a16_dgrad", "moe_balance",
                                    "moe_balance_grad")} <= names
     assert [n for n, d in watched.calls if d != x.device] == []
+
+
+@pytest.mark.gpu
+def test_a_device_without_an_index_is_the_current_one():
+    cuda, numbered = torch.device("cuda"), torch.device("cuda", torch.cuda.current_device())
+    assert ops.workspace(cuda, 256) is ops.workspace(numbered, 256)
+    assert ops.device_status(cuda) == 0
+    ops.lora_plan(torch.tensor([0, 5, -1], device="cuda"), 2)
+    assert ops.device_status(cuda) & 2 and ops.device_status(numbered) == 0
