@@ -202,8 +202,18 @@ __device__ __forceinline__ void cp_async_wait() {
 // cut out of the one or two aligned 16-byte blocks that hold them, or read one
 // by one where such a block would reach past the tensor's end.
 
+// RO: through the read-only path.  Not for base, which may be y itself: another
+// CTA may be writing a neighbour's values in the same block (they are dropped).
+template <bool RO>
+__device__ __forceinline__ uint4 ld16(const uint4* p) {
+  if constexpr (RO)
+    return __ldg(p);
+  else
+    return *p;
+}
+
 // Up to 8 values from p on, zeros past `left`; `end`: the tensor's end.
-template <class T>
+template <class T, bool RO = true>
 __device__ __forceinline__ uint4 ld8_any(const T* p, int left, const T* end) {
   if (left <= 0) return make_uint4(0, 0, 0, 0);
   const uintptr_t at = reinterpret_cast<uintptr_t>(p), lo = at & ~(uintptr_t)15;
@@ -211,8 +221,8 @@ __device__ __forceinline__ uint4 ld8_any(const T* p, int left, const T* end) {
   const bool two = shift && 2 * min(left, 8) > 16 - shift;
   uint32_t w[8];
   if (lo + (two ? 32 : 16) <= reinterpret_cast<uintptr_t>(end)) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(lo));
-    const uint4 b = two ? __ldg(reinterpret_cast<const uint4*>(lo) + 1) : make_uint4(0, 0, 0, 0);
+    const uint4 a = ld16<RO>(reinterpret_cast<const uint4*>(lo));
+    const uint4 b = two ? ld16<RO>(reinterpret_cast<const uint4*>(lo) + 1) : make_uint4(0, 0, 0, 0);
     w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
     if (shift & 8) {
 #pragma unroll
@@ -241,12 +251,12 @@ __device__ __forceinline__ uint4 ld8_any(const T* p, int left, const T* end) {
 }
 
 // Values [k, k + 8) of a row of K, zeros past its end (VEC: k a multiple of 8, all in or all out).
-template <class T, bool VEC>
+template <class T, bool VEC, bool RO = true>
 __device__ __forceinline__ uint4 ld8(const T* row, int k, int K, const T* end) {
   if constexpr (VEC)
-    return k < K ? __ldg(reinterpret_cast<const uint4*>(row + k)) : make_uint4(0, 0, 0, 0);
+    return k < K ? ld16<RO>(reinterpret_cast<const uint4*>(row + k)) : make_uint4(0, 0, 0, 0);
   else
-    return ld8_any<T>(row + k, K - k, end);
+    return ld8_any<T, RO>(row + k, K - k, end);
 }
 
 template <class T, bool VEC>

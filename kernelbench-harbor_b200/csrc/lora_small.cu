@@ -65,8 +65,8 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(THREADS) lora_small
   uint2 qt[TR ? RP / 16 : 1][4];
   auto load_group = [&](int q) {
     const int n = q * 32 + 8 * t;
-    bv[0] = base && ra >= 0 ? ld8<T, VEC>(base + ra * N, n, N, base + a.T * N) : make_uint4(0, 0, 0, 0);
-    bv[1] = base && rb >= 0 ? ld8<T, VEC>(base + rb * N, n, N, base + a.T * N) : make_uint4(0, 0, 0, 0);
+    bv[0] = base && ra >= 0 ? ld8<T, VEC, false>(base + ra * N, n, N, base + a.T * N) : make_uint4(0, 0, 0, 0);
+    bv[1] = base && rb >= 0 ? ld8<T, VEC, false>(base + rb * N, n, N, base + a.T * N) : make_uint4(0, 0, 0, 0);
     if constexpr (!TR) {
 #pragma unroll
       for (int i = 0; i < RP / 8; ++i) {  // rank rows in fragment order, 4 lanes per row

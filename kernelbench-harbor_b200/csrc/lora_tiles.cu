@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) lora_expand_tile_kernel(const A
   auto request = [&]() {
     if constexpr (!VEC) {
       static_for<4>([&](auto i) {
-        wv[i] = base && prow + 32 * i < count ? ld8_any<T>(src[i], N - cst - pc * 8, base + a.T * N) : make_uint4(0, 0, 0, 0);
+        wv[i] = base && prow + 32 * i < count ? ld8_any<T, false>(src[i], N - cst - pc * 8, base + a.T * N) : make_uint4(0, 0, 0, 0);
       });
       if constexpr (TR)
         static_for<NP>([&](auto i) {

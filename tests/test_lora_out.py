@@ -70,3 +70,27 @@ def test_out_that_asks_for_a_gradient():
     with torch.no_grad():
         ops.lora_apply(c["base"], c["x"], c["A"], c["B"], c["ids"], out=leaf)
     assert torch.equal(leaf.detach(), ops.lora_apply(c["base"], c["x"], c["A"], c["B"], c["ids"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("T,D,N,r,L", [(1, 63, 61, 5, 1), (40, 129, 33, 8, 3), (256, 250, 1001, 12, 2), (300, 129, 99, 16, 3),
+                                       (700, 333, 1027, 33, 5), (2000, 101, 259, 64, 1), (3000, 257, 65, 4, 700)])
+def test_in_place_at_odd_widths(T, D, N, r, L, dtype):
+    """Rows that share 16-byte blocks with their neighbours, written while others
+    are read: the same bits as beside the base, row by row; dx over the
+    projection's likewise."""
+    c = inputs(T, D, N, r, L, dtype, "mixed")
+    plan = ops.lora_plan(c["ids"], L)
+    args = (c["x"], c["A"], c["B"], plan, c["scaling"])
+    want = ops.lora_apply(c["base"], *args)
+    lo = ops.lora_apply_op(c["base"], c["x"], c["A"], c["B"], c["scaling"], plan.data)[1]
+    back = (c["A"], c["B"], c["scaling"], plan.data, lo)
+    dx = ops.lora_backward_op(c["x"], c["dy"], c["x"], *back, True, False, False)[0]
+    sizes = (T, D, N, r, L, ops._dtype_code(c["x"].dtype))
+    for _ in range(5):
+        y = c["base"].clone()
+        assert ops.lora_apply(y, *args, out=y) is y and torch.equal(y, want)
+        g = c["x"].clone()
+        ops._lora_grads(sizes, c["x"], c["dy"], g, *back, g, False, False)
+        assert torch.equal(g, dx)
