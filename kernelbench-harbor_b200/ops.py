@@ -1070,7 +1070,8 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
         if out is not base:
             base = _aligned(base)
     x, A, B = _aligned(x), _aligned(A), _aligned(B)
-    if out_given and (any(_overlap(out, t) for t in (x, A, B)) or (out.data_ptr() != base.data_ptr() and _overlap(out, base))):
+    if out_given and (any(t is not None and _overlap(out, t) for t in (x, A, B, scaling, plan.data)) or
+                      (out.data_ptr() != base.data_ptr() and _overlap(out, base))):
         raise ValueError("lora_apply: out shares memory with an input (it may be base itself)")
     # the one-launch kernel needs no room for the row between
     lo = None if T <= _LORA_SMALL else _lora_mid(plan, A.shape[2])

@@ -94,3 +94,18 @@ def test_in_place_at_odd_widths(T, D, N, r, L, dtype):
         g = c["x"].clone()
         ops._lora_grads(sizes, c["x"], c["dy"], g, *back, g, False, False)
         assert torch.equal(g, dx)
+
+
+@pytest.mark.gpu
+def test_out_over_the_plan_or_the_scaling_is_refused():
+    """The plan holds row numbers: written over while it is read, it would send a
+    kernel anywhere.  Refused on the host, before any launch."""
+    c = inputs(10, 64, 8, 8, 16, "fp16", "mixed")
+    plan = ops.lora_plan(c["ids"], 16)
+    scaling = torch.ones(64, device="cuda")
+    for words, kw in ((plan.data, {}), (scaling, {"scaling": scaling[:16]})):
+        kept = words.clone()
+        out = words.view(torch.float16)[:80].view(10, 8)
+        with pytest.raises(ValueError, match="shares memory"):
+            ops.lora_apply(c["base"], c["x"], c["A"], c["B"], plan, **kw, out=out)
+        assert torch.equal(words, kept)
