@@ -863,7 +863,8 @@ def _lora_operands(op, x, A, B, scaling, plan, *, dy=None, base=None, lo=None):
 
 
 def _lora_backward(sizes, x, d, base, A, B, scaling, plan, lo, dx, want_x, want_A, want_B):
-    """(dx, dA, dB) for a Function's backward pass; dx: where to put it (base itself), or None."""
+    """(dx, dA, dB) for a backward pass; dx: where to put it (base itself), or None.
+    sizes: None in a registered operator's formula."""
     if torch.is_grad_enabled():
         # create_graph: operators that refuse to be differentiated again, one for each
         # gradient, so that each refuses exactly where it depends on something that
@@ -872,7 +873,7 @@ def _lora_backward(sizes, x, d, base, A, B, scaling, plan, lo, dx, want_x, want_
         return (lora_backward_op(x.detach(), d, base, A, B, *rest, True, False, False)[0] if want_x else None,
                 lora_backward_op(x, d, None, A.detach(), B, *rest, False, True, False)[1] if want_A else None,
                 lora_backward_op(x, d, None, A, B.detach(), *rest, False, False, True)[2] if want_B else None)
-    if _dispatched(d):
+    if sizes is None:
         out = lora_backward_op(x, d, base, A, B, scaling, plan, lo, want_x, want_A, want_B)
         return tuple(g if want else None for g, want in zip(out, (want_x, want_A, want_B)))
     if dx is None and want_x:

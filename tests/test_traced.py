@@ -109,8 +109,12 @@ def test_under_a_dispatch_mode():
         return (y, loss, counts, *torch.autograd.grad(y.float().sum() + loss, leaves))
 
     want = run()
+    with Names():  # backward behind the mode
+        y, loss, counts = Layer()(*args)
+    behind = (y, loss, counts, *torch.autograd.grad(y.float().sum() + loss, leaves))
     with Names() as names:
         got = run()
+    assert all(torch.equal(a, b) for a, b in zip(behind, want))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert {"b200q::lora_plan", "b200q::lora_w4a16", "b200q::lora_apply", "b200q::lora_backward", "b200q::w4a16_dgrad",
             "b200q::moe_balance", "b200q::moe_balance_grad"} <= names.seen
