@@ -19,6 +19,7 @@ from . import _lib
 
 _ws_lock = threading.Lock()
 _ws: dict = {}
+_ws_outgrown: list = []  # captured graphs may use them still
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -29,14 +30,18 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     with _ws_lock:
         buf = _ws.get(key)
         if buf is None or buf.numel() < nbytes:
+            if buf is not None:
+                _ws_outgrown.append(buf)
             buf = torch.zeros(max(nbytes, 4096), dtype=torch.uint8, device=device)
             _ws[key] = buf
         return buf
 
 
 def reset_workspaces() -> None:
+    """Drops all workspaces; graphs captured before must not be replayed again."""
     with _ws_lock:
         _ws.clear()
+        _ws_outgrown.clear()
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
