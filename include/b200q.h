@@ -57,6 +57,11 @@ const char* b200q_last_error(void);
  * before reusing it. */
 int b200q_workspace_status(void* workspace, void* stream);
 
+/* The id of the graph capture that `stream` is in; 0 where it is in none.  A
+ * workspace that is zeroed inside a capture is zeroed when that graph is
+ * replayed, not before. */
+uint64_t b200q_capture_id(void* stream);
+
 /* Weight prefetch across kernel boundaries (off by default; process-wide).
  * When on, the small-M W4A16 kernel (M <= 16, single GPU) is launched with
  * programmatic dependent launch: it starts while the previous kernel in the

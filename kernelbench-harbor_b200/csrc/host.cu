@@ -168,6 +168,16 @@ int b200q_set_weight_prefetch(int enable) {
 
 const char* b200q_last_error(void) { return b200q::g_last_error.c_str(); }
 
+uint64_t b200q_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(reinterpret_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();  // the legacy stream beside a capture: not in it itself
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
+
 int b200q_workspace_status(void* workspace, void* stream) {
   if (!workspace) return b200q::fail(B200Q_ERR_WORKSPACE, "workspace is null");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

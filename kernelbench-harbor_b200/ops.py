@@ -19,21 +19,35 @@ from . import _lib
 
 _ws_lock = threading.Lock()
 _ws: dict = {}
+_ws_captured: dict = {}  # workspaces made inside a graph capture: the capture that zeroed them last
 _ws_outgrown: list = []  # captured graphs may use them still
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Zero-initialised scratch owned by this process, one per (device, stream).
     Kernels return it to the zero state, so it is allocated (and zeroed) once
-    and reused; it is never shared by two streams, whose launches could overlap."""
+    and reused; it is never shared by two streams, whose launches could overlap.
+
+    Inside a graph capture the zeroing becomes a node of that graph: a workspace
+    made there is zeroed in every graph that is captured with it (they may be
+    replayed in any order), and calls outside a capture take another."""
     key = (_index(device), _stream_ptr(device))
     with _ws_lock:
         buf = _ws.get(key)
-        if buf is None or buf.numel() < nbytes:
+        if buf is not None and buf.numel() >= nbytes and key not in _ws_captured:
+            return buf
+        capture = _lib.lib().b200q_capture_id(key[1])
+        if buf is None or buf.numel() < nbytes or not capture:
             if buf is not None:
                 _ws_outgrown.append(buf)
             buf = torch.zeros(max(nbytes, 4096), dtype=torch.uint8, device=device)
             _ws[key] = buf
+        elif _ws_captured[key] != capture:
+            buf.zero_()
+        if capture:
+            _ws_captured[key] = capture
+        else:
+            _ws_captured.pop(key, None)
         return buf
 
 
@@ -41,6 +55,7 @@ def reset_workspaces() -> None:
     """Drops all workspaces; graphs captured before must not be replayed again."""
     with _ws_lock:
         _ws.clear()
+        _ws_captured.clear()
         _ws_outgrown.clear()
 
 
