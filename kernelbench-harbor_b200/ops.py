@@ -60,10 +60,9 @@ def reset_workspaces() -> None:
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
-    if t.data_ptr() % 16:
-        t = t.clone()
-    return t
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def _dtype_code(dt: torch.dtype) -> int:
@@ -105,9 +104,8 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _no_tangent(op: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Refuses dual tensors (forward-mode differentiation), whose tangents the kernels do not see."""
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
-                                              for t in tensors):
+    """Refuses dual tensors (forward-mode differentiation, _current_level >= 0), whose tangents the kernels do not see."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{op} has no forward-mode derivative")
 
 
@@ -128,7 +126,8 @@ def _same_device(op: str, first: torch.Tensor, *rest: Optional[torch.Tensor]) ->
 def w4a16_gemm(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
                group: int) -> torch.Tensor:
     """y[M, N] = x[M, K] . ((unpack(qweight) - zeros) * scales), y in x.dtype."""
-    _no_tangent("w4a16_gemm", x)
+    if forward_ad._current_level >= 0:
+        _no_tangent("w4a16_gemm", x)
     if not x.is_cuda:
         raise RuntimeError("b200q::w4a16_gemm runs on CUDA tensors only (no CPU implementation)")
     if x.dim() != 2 or qweight.dim() != 2:
@@ -166,13 +165,16 @@ def _(x, qweight, scales, zeros, group):
     return x.new_empty((x.shape[0], qweight.shape[1] * 8))
 
 
+_is_compiling, _dispatch_modes = torch.compiler.is_compiling, torch._C._len_torch_dispatch_stack
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
 def _dispatched(t: torch.Tensor) -> bool:
     """Whether a call on t has to go through PyTorch's dispatcher as a registered
     operator: while a program is traced (torch.compile, export, fake tensors),
     under a dispatch mode, or for a tensor subclass.  Other calls take the
     library directly (a registered operator costs 10 us more on the host)."""
-    return (torch.compiler.is_compiling() or type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter
-            or torch._C._len_torch_dispatch_stack() > 0)
+    return _is_compiling() or type(t) not in _PLAIN or _dispatch_modes() > 0
 
 
 def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
@@ -180,7 +182,8 @@ def w4a16_dgrad(dy: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, z
     """dx[M, K] = dy[M, N] . ((unpack(qweight) - zeros) * scales)^T, dx in dy.dtype:
     the input gradient of w4a16_gemm (the weights are frozen).  Differentiable
     in dy, w4a16_gemm being its gradient in turn."""
-    _no_tangent("w4a16_dgrad", dy)
+    if forward_ad._current_level >= 0:
+        _no_tangent("w4a16_dgrad", dy)
     if (torch.is_grad_enabled() and (dy.requires_grad or scales.requires_grad or zeros.requires_grad)) or _dispatched(dy):
         return w4a16_dgrad_op(dy, qweight, scales, zeros, group)
     return _w4a16_dgrad(dy, qweight, scales, zeros, group)
@@ -537,7 +540,8 @@ def moe_balance_loss(router_logits: torch.Tensor, topi: torch.Tensor,
     probability of e; counts [E] int32.  The loss is differentiable in
     router_logits (f is a count and carries no gradient); see include/b200q.h
     for rows that are all -inf and for indices out of range."""
-    _no_tangent("moe_balance_loss", router_logits)
+    if forward_ad._current_level >= 0:
+        _no_tangent("moe_balance_loss", router_logits)
     if not router_logits.is_cuda:
         raise RuntimeError("b200q moe_balance_loss runs on CUDA tensors only")
     if router_logits.dim() != 2 or topi.dim() != 2 or topi.shape[0] != router_logits.shape[0]:
@@ -1016,7 +1020,8 @@ lora_w4a16_op.register_autograd(_lora_w4a16_backward, setup_context=_lora_w4a16_
 def _lora_check(op, x, A, B, plan, scaling):
     """Checks the adapter operands that lora_apply and lora_w4a16 share; returns
     A and B in x's dtype, the plan and scaling as fp32."""
-    _no_tangent(op, x, A, B)
+    if forward_ad._current_level >= 0:
+        _no_tangent(op, x, A, B)
     if not x.is_cuda:
         raise RuntimeError(f"b200q {op} runs on CUDA tensors only")
     if x.dim() != 2 or A.dim() != 3 or B.dim() != 3:
@@ -1060,7 +1065,8 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     fp32; y is rounded once.  Differentiable in base, x, A and B (scaling is a
     constant).  ``out`` (which may be ``base``: in place) takes the result
     where no gradient is wanted."""
-    _no_tangent("lora_apply", base)
+    if forward_ad._current_level >= 0:
+        _no_tangent("lora_apply", base)
     A, B, plan, scaling = _lora_check("lora_apply", x, A, B, plan, scaling)
     T, dt = x.shape[0], x.dtype
     if base.shape != (T, B.shape[2]):
