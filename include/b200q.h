@@ -280,8 +280,9 @@ int b200q_lora_plan(const int64_t* lora_ids, int64_t T, int64_t L, int32_t* plan
 /* y.  base: NULL for zeros; may be y itself; a token without an adapter gets
  * base.  lo: the row between the two products, for the backward pass:
  * b200q_lora_mid_bytes(T, r) bytes, any contents; rows of tokens without an
- * adapter are left as they were.  NULL where T <= 256 and no backward pass
- * follows.  workspace: a status word for waits that run out, or NULL. */
+ * adapter are left as they were.  May be NULL where T <= 256 and no backward
+ * pass follows (with r > 32 and T > 128 the call is faster with it).
+ * workspace: a status word for waits that run out, or NULL. */
 size_t b200q_lora_mid_bytes(int64_t T, int64_t r);
 int b200q_lora_apply(const void* x, const void* base, const void* A, const void* B, const float* scaling,
                      const int32_t* plan, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype, void* y,

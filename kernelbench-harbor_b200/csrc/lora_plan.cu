@@ -129,11 +129,20 @@ int launch_grads(const void* x, const void* dy, const float* lo, const float* dl
 size_t grads_part_bytes(int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype);
 
 // Up to this many tokens the one-launch cluster kernel runs, above it the
-// tiled pair.
-constexpr int64_t SMALL_MAX_T = 256;
+// tiled pair (which needs room for the row between).  Measured, bf16, us with
+// one launch / the pair, one adapter:
+//   4096 x 4096:   r 16, 64 tokens 5.5 / 8.9, 256 6.7 / 10.0, 512 7.4 / 11.0; r 32 7.5 / 10.0, 9.6 / 11.2, 11.3 / 12.7
+//   14336 -> 4096: r 16, 256 tokens 9.3 / 16.8; 4096 -> 14336: 10.6 / 12.2
+// At ranks 33 to 64 a CTA takes 160 KB of shared memory, so one fits an SM, and
+// above 128 tokens the tiles soon take a second round of clusters:
+//   4096 x 4096:   r 64, 64 tokens 13.2 / 11.4, 128 13.2 / 12.9, 256 25.3 / 14.0; of 8 adapters 12.9 / 12.6, 13.2 / 13.2, 25.2 / 13.6
+//   4096 -> 14336: 128 tokens 18.3 / 14.1, of 8 adapters 18.4 / 23.8, 256 35.0 / 15.6 and 35.0 / 23.3
+// The transposed form (dx) differs from these by less than 1.5 us.
+constexpr int64_t SMALL_MAX_T = 256, SMALL_MAX_T_HIGH = 128;
 
 static int launch(const Args& a, int dtype, bool tr, cudaStream_t st) {
-  return a.T <= SMALL_MAX_T ? launch_small(a, dtype, tr, st) : launch_tiles(a, dtype, tr, st);
+  const bool small = a.T <= (a.r > 32 && a.mid ? SMALL_MAX_T_HIGH : SMALL_MAX_T);
+  return small ? launch_small(a, dtype, tr, st) : launch_tiles(a, dtype, tr, st);
 }
 
 static int check_sizes(const char* what, int64_t T, int64_t D, int64_t N, int64_t r, int64_t L, int dtype) {

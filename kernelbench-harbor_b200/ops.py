@@ -738,7 +738,9 @@ def lora_expand_add(base: torch.Tensor, lo: torch.Tensor, B: torch.Tensor, lora_
     return y
 
 
-_LORA_SMALL = 256  # tokens up to which b200q_lora_apply takes lo = NULL
+def _one_launch(T: int, r: int) -> bool:
+    """Whether b200q_lora_apply runs as one launch: it needs no room for the row between, and has no wait that could run out."""
+    return T <= (256 if r <= 32 else 128)
 
 
 class LoraPlan:
@@ -805,8 +807,7 @@ def _lora_run(x, base, A, B, scaling, plan, out, lo):
     dev = x.device
     sizes = (T, D, B.shape[2], r, n_adapters, _dtype_code(x.dtype))
     with _device(dev):
-        # the one-launch kernel has no wait that could run out
-        status = None if T <= _LORA_SMALL else workspace(dev, 256).data_ptr()
+        status = None if _one_launch(T, r) else workspace(dev, 256).data_ptr()
         _lib.check(_lib.lib().b200q_lora_apply(x.data_ptr(), base.data_ptr(), A.data_ptr(), B.data_ptr(), _ptr(scaling),
                                                plan.data_ptr(), *sizes, out.data_ptr(), _ptr(lo), status,
                                                _stream_ptr(dev)))
@@ -837,7 +838,7 @@ def _lora_grads(sizes, x, d, base, A, B, scaling, plan, lo, dx, want_A, want_B):
     with _device(dev):
         nbytes = _lora_scratch(*sizes, dev.index)
         scratch = plan.new_empty(nbytes // 4)  # fp32 sums
-        status = None if sizes[0] <= _LORA_SMALL else workspace(dev, 256).data_ptr()
+        status = None if _one_launch(sizes[0], sizes[3]) else workspace(dev, 256).data_ptr()
         _lib.check(_lib.lib().b200q_lora_backward(
             x.data_ptr(), d.data_ptr(), _ptr(base), A.data_ptr(), B.data_ptr(), _ptr(scaling), plan.data_ptr(),
             lo.data_ptr(), *sizes, scratch.data_ptr(), nbytes, _ptr(dx), _ptr(dA), _ptr(dB), status, _stream_ptr(dev)))
@@ -1100,8 +1101,8 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
     if out_given and (any(t is not None and _overlap(out, t) for t in (x, A, B, scaling, plan.data)) or
                       (out.data_ptr() != base.data_ptr() and _overlap(out, base))):
         raise ValueError("lora_apply: out shares memory with an input (it may be base itself)")
-    # the one-launch kernel needs no room for the row between
-    lo = None if T <= _LORA_SMALL else _lora_mid(plan, A.shape[2])
+    r = A.shape[2]
+    lo = None if _one_launch(T, r) else _lora_mid(plan, r)
     _lora_run(x, base, A, B, scaling, plan.data, out, lo)
     if out_given:
         _written(out)
@@ -1125,7 +1126,8 @@ def lora_w4a16(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zer
         return _LoRAW4A16.apply(_aligned(x), _aligned(A), _aligned(B), qweight, scales, zeros, group, scaling, plan)
     y = w4a16_gemm(x, qweight, scales, zeros, group)
     x = _aligned(x)
-    lo = None if x.shape[0] <= _LORA_SMALL else _lora_mid(plan, A.shape[2])
+    r = A.shape[2]
+    lo = None if _one_launch(x.shape[0], r) else _lora_mid(plan, r)
     with torch.no_grad():
         _lora_run(x, y, _aligned(A), _aligned(B), scaling, plan.data, y, lo)
     return y
