@@ -264,7 +264,11 @@ int b200q_lora_expand_add(const void* base, const void* lo, const void* B, const
  *   dA[a] = sum_{id_t = a} x[t]^T dlo[t]    dB[a] = sum_{id_t = a} lo[t]^T dy[t]
  * x [T, D], dy and y [T, N], A [L, D, r], B [L, r, N] in fp16 or bf16, s =
  * scaling [L] fp32 or NULL (1).  fp32 accumulation, lo and dlo in fp32, one
- * rounding of each result.  Results do not depend on timing.  1 <= r <= 64,
+ * rounding of each result.  lo and dlo enter the second products as two halves
+ * of the type: 2^-16 (bf16) or 2^-22 (fp16) of a value is lost, in fp16 at
+ * least 2^-39 of the largest value of its row (for dA and dB: of its adapter's
+ * tokens).  An infinity in A or B, for dA and dB in x or dy, gives infinities or
+ * NaN in the results that it enters.  Results do not depend on timing.  1 <= r <= 64,
  * 1 <= L <= 1023, D and N any width up to 2^22 (multiples of 8, with r a
  * multiple of 8, run fastest), 16-byte aligned pointers.
  *

@@ -3,7 +3,7 @@
 // on 128-row tiles of one adapter, 64 columns at a time, the sums in tensor memory.
 //
 // The tile's mid rows are split into two halves of the type once (scaled by a
-// power of two per row, as in lora_tiles.cu) and stay in shared memory as two
+// power of two per row, scale_of) and stay in shared memory as two
 // K-major operands; a ring of 3 stages holds base's 64 columns and the stage of
 // Q (as stored: MN-major forward, K-major backward), both by 16-byte
 // asynchronous copies in the 128-byte swizzle.  One thread issues a stage's 8
@@ -14,7 +14,7 @@
 // Bound: HBM, base and y once; the steps run near the measured copy rate, start
 // (plan, rows, mid, halves: 3 us) beside them.  After the shrink at N=14336, D=4096,
 // r=64, 8192 tokens of two adapters 129 us for both (142 with register fragments);
-// 4096 tokens, N=4096, D=14336: 51.5 and 53.2.
+// 4096 tokens, N=4096, D=14336: 52.4 and 54.1.
 #include "lora_seg.cuh"
 
 namespace b200q {

@@ -7,7 +7,8 @@
 // first positions, and a second walk writes the tokens: a stable counting sort
 // without atomics, so a plan is the same every time.  A batch needs it once for
 // all projections of a model.  Bound: latency, ~T / 1024 dependent steps twice:
-// 4.5 us for 64 tokens, 11.6 us for 8192.
+// 4.6 us for 64 tokens, 8.2 for 8192, 44 for 65536 (one block is enough for a
+// batch of a serving or training step; more would gain from several).
 #include <type_traits>
 
 #include "lora_seg.cuh"

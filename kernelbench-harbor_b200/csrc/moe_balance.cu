@@ -18,9 +18,10 @@
 // that one block adds in block order: no floating-point atomics, the same bits
 // every time.  Counts are integers, where order does not matter.  Batches of
 // at most SINGLE_ELEMS logits take one block and one launch.
-// Measured: 512 tokens, 8 experts 7 us forward and backward; 131072 tokens, 64
-// experts, fp32 (34 MB) 34 us, 18 of them the partial sums -- the latency of a
-// block's rows, under a host call of 90 us.
+// Measured, forward and backward: 512 tokens, 8 experts 8.5 us; 131072 tokens, 64
+// experts, fp32 (34 MB) 31 us, under a host call of 90 (one by one and cold the
+// partial sums 18.8, bound by their instructions at 2 a cycle and SM, the one block
+// that joins them 6.9 and the gradient 16.3).
 #include <algorithm>
 
 #include "common.cuh"

@@ -1115,7 +1115,8 @@ def lora_w4a16(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zer
     """w4a16_gemm(x, qweight, scales, zeros, group) with lora_apply's adapters
     beside it, in place on the projection's output.  Differentiable in x, A and
     B: x's gradient is w4a16_dgrad's with the adapters' part added to it in
-    place."""
+    place.  Both results are rounded twice: as the projection's (the input
+    gradient's) output, and with the adapters' part."""
     A, B, plan, scaling = _lora_check("lora_w4a16", x, A, B, plan, scaling)
     if qweight.dim() != 2 or qweight.shape[1] * 8 != B.shape[2]:
         raise ValueError(f"lora_w4a16: qweight {tuple(qweight.shape)} does not fit B {tuple(B.shape)}")
