@@ -908,6 +908,11 @@ def _lora_backward(sizes, x, d, base, A, B, scaling, plan, lo, dx, want_x, want_
     return (dx, *_lora_grads(sizes, x, d, base, A, B, scaling, plan, lo, dx, want_A, want_B))
 
 
+def _saveable(plan: LoraPlan) -> LoraPlan:
+    """The plan, copied where autograd could not save it (made in inference mode)."""
+    return LoraPlan(plan.data.clone(), plan.tokens, plan.adapters) if plan.data.is_inference() else plan
+
+
 class _LoraApply(torch.autograd.Function):
     @staticmethod
     def forward(ctx, base, x, A, B, scaling, plan):
@@ -1087,7 +1092,7 @@ def lora_apply(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Te
             raise ValueError("lora_apply: out must be a [T, N] tensor of x's dtype")
         return out.copy_(y)
     if wanted:
-        return _LoraApply.apply(_aligned(base), _aligned(x), _aligned(A), _aligned(B), scaling, plan)
+        return _LoraApply.apply(_aligned(base), _aligned(x), _aligned(A), _aligned(B), scaling, _saveable(plan))
     out_given = out is not None
     if not out_given:
         base = _aligned(base)
@@ -1124,7 +1129,8 @@ def lora_w4a16(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zer
     if _dispatched(x):
         return lora_w4a16_op(x, A, B, qweight, scales, zeros, group, scaling, plan.data)[0]
     if torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad):
-        return _LoRAW4A16.apply(_aligned(x), _aligned(A), _aligned(B), qweight, scales, zeros, group, scaling, plan)
+        return _LoRAW4A16.apply(_aligned(x), _aligned(A), _aligned(B), qweight, scales, zeros, group, scaling,
+                                _saveable(plan))
     y = w4a16_gemm(x, qweight, scales, zeros, group)
     x = _aligned(x)
     r = A.shape[2]

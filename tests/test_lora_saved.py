@@ -58,3 +58,15 @@ def test_a_changed_plan_is_seen():
         plan.data.add_(0)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(y, leaves, dy)
+
+
+@pytest.mark.gpu
+def test_a_plan_made_in_inference_mode():
+    """Served first, then fitted on: autograd does not save an inference tensor, so it saves a copy."""
+    for i in range(2):
+        plan, leaves, dy, forms = calls(40)
+        want = torch.autograd.grad(forms[i](*leaves), leaves, dy)
+        with torch.inference_mode():
+            plan.data = plan.data.clone()
+        assert plan.data.is_inference()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(forms[i](*leaves), leaves, dy), want))

@@ -132,3 +132,13 @@ def test_in_place_while_traced():
     got = base.clone()
     torch.compile(f, backend="aot_eager", fullgraph=True)(got)
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_a_plan_handed_to_a_compiled_program():
+    x, q, s, z, A, B, ids, scaling, _ = setup(40)
+    plan = ops.lora_plan(ids, 3)
+    f = torch.compile(lambda x, plan: ops.lora_w4a16(x, q, s, z, 64, A, B, plan, scaling), backend="aot_eager", fullgraph=True)
+    assert torch.equal(f(x, plan), ops.lora_w4a16(x, q, s, z, 64, A, B, plan, scaling))
+    other = ops.lora_plan(ids.flip(0), 3)
+    assert torch.equal(f(x, other), ops.lora_w4a16(x, q, s, z, 64, A, B, other, scaling))
